@@ -1,0 +1,75 @@
+// Element types of activations (fp32, bf16, fp16) and the scalar activation functions, shared by the norm and the
+// int4 product kernels.  Every value is widened to fp32 on load and rounded once on store.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include "common.cuh"
+
+namespace forge {
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+    static __device__ __forceinline__ float to_f(float v) { return v; }
+    static __device__ __forceinline__ float from_f(float v) { return v; }
+};
+template <> struct Elem<__nv_bfloat16> {
+    static __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
+};
+template <> struct Elem<__half> {
+    static __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
+};
+
+// eight consecutive elements, 16-byte aligned (two accesses for fp32)
+template <typename T> __device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+        const uint4 raw = *reinterpret_cast<const uint4 *>(p);
+        const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = Elem<T>::to_f(e[i]);
+    }
+}
+template <typename T> __device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        uint4 raw;
+        T *e = reinterpret_cast<T *>(&raw);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = Elem<T>::from_f(v[i]);
+        *reinterpret_cast<uint4 *>(p) = raw;
+    }
+}
+
+template <int ACT> __device__ __forceinline__ float act_fwd(float z) {
+    if constexpr (ACT == FORGE_ACT_RELU) return z < 0.0f ? 0.0f : z;      // NaN passes through
+    if constexpr (ACT == FORGE_ACT_SILU) return z / (1.0f + expf(-z));
+    if constexpr (ACT == FORGE_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    return z;
+}
+template <int ACT> __device__ __forceinline__ float act_bwd(float z) {
+    if constexpr (ACT == FORGE_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+    if constexpr (ACT == FORGE_ACT_SILU) {
+        const float s = 1.0f / (1.0f + expf(-z));
+        return s * (1.0f + z * (1.0f - s));
+    }
+    if constexpr (ACT == FORGE_ACT_GELU)
+        return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+    return 1.0f;
+}
+__device__ __forceinline__ float act_fwd_rt(int act, float z) {
+    switch (act) {
+        case FORGE_ACT_RELU: return act_fwd<FORGE_ACT_RELU>(z);
+        case FORGE_ACT_SILU: return act_fwd<FORGE_ACT_SILU>(z);
+        case FORGE_ACT_GELU: return act_fwd<FORGE_ACT_GELU>(z);
+        default: return z;
+    }
+}
+
+}  // namespace forge

@@ -1,0 +1,396 @@
+// Products with packed int4 weights (the layout of forge_pack_int4, symmetric codes):
+//   W[r, c] = (nibble(r, c) - 8) * scale[r, c / gs]
+//   linear:  y = act(x W^T + bias) + residual            gated:  h = act(x Wg^T) * (x Wu^T)
+// and their backward passes for frozen weights:
+//   linear:  dz = dy * act'(z),  dx = dz W,  dbias = sum over rows of dz
+//   gated:   dg = dh * u * act'(g),  du = dh * act(g),  dx = dg Wg + du Wu
+//
+// Backward operand: dz is the K operand of the second product and has to be a 16-bit matrix.  It is written as fp16
+// (11 bits, against bf16's 8) times a power of two per token row that puts the row's largest entry just below 2^15;
+// the product is multiplied by the inverse power at the end, so nothing but the 2^-12 relative rounding remains.  The
+// weights' scales are split the same way: a power of two per weight row goes into dz (exactly), the rest is at most 2.
+#include "common.cuh"
+#include "elem.cuh"
+#include "int4_mm.cuh"
+
+using namespace forge;
+
+namespace {
+
+// ---- backward preparation ------------------------------------------------------------------------------------------
+
+// Per weight row r: the power of two f[r] = 2^floor(log2 max_g |s|) and the normalised scales s / f as an fp16 pair
+// (hi, lo), hi + lo = s / f to 22 bits.  One warp per row.
+__global__ void __launch_bounds__(256) scale_prep_kernel(const float *__restrict__ s0, const float *__restrict__ s1,
+                                                         int64_t R, int64_t G, __half2 *__restrict__ pairs,
+                                                         float *__restrict__ f) {
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int64_t rows = s1 ? 2 * R : R;
+    if (row >= rows) return;
+    const int lane = threadIdx.x & 31;
+    const float *s = (row < R ? s0 + row * G : s1 + (row - R) * G);
+    float m = 0.0f;
+    for (int64_t g = lane; g < G; g += 32) m = fmaxf(m, fabsf(s[g]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const int e = (m > 0.0f && isfinite(m)) ? ilogbf(m) : 0;
+    for (int64_t g = lane; g < G; g += 32) {
+        const float v = scalbnf(s[g], -e);
+        const __half hi = __float2half_rn(v);
+        pairs[row * G + g] = __halves2half2(hi, __float2half_rn(v - __half2float(hi)));
+    }
+    if (lane == 0) f[row] = scalbnf(1.0f, e);
+}
+
+struct DzParams {
+    const void *dy, *z, *u;     // z NULL: act is none; u given: gated
+    int64_t lddy, T, R, K, ldk; // ldk: row stride of a, a multiple of 64; K = used columns
+    const float *f;
+    __half *a;
+    float *unscale;
+};
+__device__ __forceinline__ float pow2_of(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
+
+// One CTA per token row: the row of the K operand, its power of two, and zeros up to the padded length.
+template <typename T, int ACT, bool GATED> __global__ void __launch_bounds__(256) dz_kernel(const DzParams P) {
+    __shared__ float slot[8];
+    const int64_t t = blockIdx.x;
+    const T *dy = (const T *)P.dy + t * P.lddy;
+    const T *z = (const T *)P.z + t * P.R, *u = (const T *)P.u + t * P.R;
+    __half *a = P.a + t * P.ldk;
+    float scale = 1.0f;
+    for (int pass = 0; pass < 2; ++pass) {
+        float amax = 0.0f;
+        for (int64_t r = threadIdx.x; r < P.R; r += 256) {
+            const float d = Elem<T>::to_f(dy[r]);
+            const float zv = (ACT == FORGE_ACT_NONE && !GATED) ? 0.0f : Elem<T>::to_f(z[r]);
+            if constexpr (GATED) {
+                const float vg = d * Elem<T>::to_f(u[r]) * act_bwd<ACT>(zv) * P.f[r];
+                const float vu = d * act_fwd<ACT>(zv) * P.f[P.R + r];
+                if (pass == 0) amax = fmaxf(amax, fmaxf(fabsf(vg), fabsf(vu)));
+                else {
+                    a[r] = __float2half_rn(vg * scale);
+                    a[P.R + r] = __float2half_rn(vu * scale);
+                }
+            } else {
+                const float v = d * act_bwd<ACT>(zv) * P.f[r];
+                if (pass == 0) amax = fmaxf(amax, fabsf(v));
+                else a[r] = __float2half_rn(v * scale);
+            }
+        }
+        if (pass == 0) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = amax;
+            __syncthreads();
+            amax = slot[0];
+#pragma unroll
+            for (int w = 1; w < 8; ++w) amax = fmaxf(amax, slot[w]);
+            // the largest entry becomes 2^14 .. 2^15; rows of zeros and of infinities keep the factor 1
+            int e = (amax > 0.0f && isfinite(amax)) ? 14 - ilogbf(amax) : 0;
+            e = e > 126 ? 126 : (e < -126 ? -126 : e);
+            scale = pow2_of(e);
+            if (threadIdx.x == 0) P.unscale[t] = pow2_of(-e);
+        }
+    }
+    for (int64_t k = P.K + threadIdx.x; k < P.ldk; k += 256) a[k] = __float2half_rn(0.0f);
+}
+
+// Partial column sums of dz: CTA (column block, row share)
+template <typename T, int ACT>
+__global__ void __launch_bounds__(256) dbias_kernel(const T *__restrict__ dy, int64_t lddy, const T *__restrict__ z,
+                                                    int64_t n, int64_t R, float *__restrict__ partial) {
+    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (r >= R) return;
+    const int64_t per = cdiv(n, (int64_t)gridDim.y);
+    const int64_t t0 = blockIdx.y * per, t1 = imin64(n, t0 + per);
+    float s = 0.0f;
+#pragma unroll 4
+    for (int64_t t = t0; t < t1; ++t) {
+        const float d = Elem<T>::to_f(dy[t * lddy + r]);
+        s = fmaf(d, ACT == FORGE_ACT_NONE ? 1.0f : act_bwd<ACT>(Elem<T>::to_f(z[t * R + r])), s);
+    }
+    partial[(int64_t)blockIdx.y * R + r] = s;
+}
+template <typename T>
+__global__ void __launch_bounds__(256) dbias_sum_kernel(const float *__restrict__ partial, int n, int64_t R, T *out) {
+    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (r >= R) return;
+    float s = 0.0f;
+    for (int k = 0; k < n; ++k) s += partial[(int64_t)k * R + r];
+    out[r] = Elem<T>::from_f(s);
+}
+
+// ---- products on the FMA pipe: 64 x 64 output tile, 16-deep k-tiles ----------------------------------------------------
+__device__ __forceinline__ float nibble(const uint32_t *packed, int64_t r, int64_t c, int64_t CP) {
+    return (float)(int)((packed[r * CP + (c >> 3)] >> (4 * (int)(c & 7))) & 15u) - 8.0f;
+}
+
+template <typename T, bool GATED> __global__ void __launch_bounds__(256) fwd_fma_kernel(const Int4Fwd P) {
+    constexpr int M = GATED ? 2 : 1;
+    __shared__ float xs[16][65], ws[M][16][65];
+    const int64_t m0 = (int64_t)blockIdx.y * 64, n0 = (int64_t)blockIdx.x * 64;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int64_t CP = P.C / 8;
+    float acc[M][4][4] = {};
+    for (int64_t k0 = 0; k0 < P.C; k0 += 16) {
+        for (int i = threadIdx.x; i < 64 * 16; i += 256) {
+            const int k = i & 15, r = i >> 4;
+            const int64_t kk = k0 + k;
+            xs[k][r] = (m0 + r < P.T && kk < P.C) ? Elem<T>::to_f(((const T *)P.x)[(m0 + r) * P.ldx + kk]) : 0.0f;
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+                ws[m][k][r] = (n0 + r < P.R && kk < P.C)
+                                  ? nibble(P.packed[m], n0 + r, kk, CP) * P.scales[m][(n0 + r) * P.G + kk / P.gs] : 0.0f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        acc[m][i][j] = fmaf(xs[k][ty * 4 + i], ws[m][k][tx * 4 + j], acc[m][i][j]);
+        __syncthreads();
+    }
+    for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < 4; ++j) {
+            const int64_t t = m0 + ty * 4 + i, r = n0 + tx * 4 + j;
+            if (t >= P.T || r >= P.R) continue;
+            float z = acc[0][i][j];
+            if (!GATED && P.bias) z += Elem<T>::to_f(((const T *)P.bias)[r]);
+            if (P.pre0) ((T *)P.pre0)[t * P.R + r] = Elem<T>::from_f(z);
+            float y = act_fwd_rt(P.act, z);
+            if constexpr (GATED) {
+                if (P.pre1) ((T *)P.pre1)[t * P.R + r] = Elem<T>::from_f(acc[M - 1][i][j]);
+                y *= acc[M - 1][i][j];
+            } else if (P.res) {
+                y += Elem<T>::to_f(((const T *)P.res)[t * P.ldres + r]);
+            }
+            ((T *)P.y)[t * P.R + r] = Elem<T>::from_f(y);
+        }
+}
+
+template <typename T> __global__ void __launch_bounds__(256) dgrad_fma_kernel(const Int4Dgrad P) {
+    __shared__ float as[16][65], ws[16][65];
+    const int64_t m0 = (int64_t)blockIdx.y * 64, n0 = (int64_t)blockIdx.x * 64;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int64_t CP = P.C / 8, K = P.mats * P.R;
+    float acc[4][4] = {};
+    for (int64_t k0 = 0; k0 < K; k0 += 16) {
+        for (int i = threadIdx.x; i < 64 * 16; i += 256) {
+            const int k = i >> 6, c = i & 63;
+            const int64_t kk = k0 + k, col = n0 + c;
+            float w = 0.0f;
+            if (kk < K && col < P.C) {
+                const int m = kk >= P.R;
+                const __half2 s = P.pairs[kk * P.G + col / P.gs];
+                w = __half2float(__float2half_rn(nibble(P.packed[m], kk - m * P.R, col, CP) *
+                                                 (__half2float(__low2half(s)) + __half2float(__high2half(s)))));
+            }
+            ws[k][c] = w;
+            as[i & 15][i >> 4] = (m0 + (i >> 4) < P.T && k0 + (i & 15) < K)
+                                     ? __half2float(P.a[(m0 + (i >> 4)) * P.ldk + k0 + (i & 15)]) : 0.0f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(as[k][ty * 4 + i], ws[k][tx * 4 + j], acc[i][j]);
+        __syncthreads();
+    }
+    for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < 4; ++j) {
+            const int64_t t = m0 + ty * 4 + i, c = n0 + tx * 4 + j;
+            if (t < P.T && c < P.C) ((T *)P.dx)[t * P.C + c] = Elem<T>::from_f(acc[i][j] * P.unscale[t]);
+        }
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------
+constexpr int64_t kMaxDim = 1ll << 24;        // rows and columns of a weight matrix
+constexpr int64_t kMaxTokens = 0x7fffffffLL;
+constexpr int kBiasParts = 64;
+
+int check_sizes(const char *who, int dtype, int64_t T, int64_t C, int64_t R, int gs, int act) {
+    const char *msg = nullptr;
+    if (T < 0 || T > kMaxTokens || C <= 0 || C > kMaxDim || R <= 0 || R > kMaxDim) msg = "bad sizes";
+    else if (dtype != FORGE_DTYPE_BF16 && dtype != FORGE_DTYPE_F16) msg = "dtype must be bf16 or fp16";
+    else if (C % 8 != 0) msg = "in_features must be a multiple of 8 (whole packed words)";
+    else if (gs != 32 && gs != 64 && gs != 128) msg = "group size must be 32, 64 or 128";
+    else if (act < FORGE_ACT_NONE || act > FORGE_ACT_GELU) msg = "unknown activation";
+    if (!msg) return FORGE_OK;
+    set_error("%s: %s", who, msg);
+    return FORGE_ERR_INVALID;
+}
+bool rows_ok(const void *p, int64_t ld, int64_t n, int64_t T) {
+    return (uintptr_t)p % 16 == 0 && (T <= 1 || (ld >= n && ld % 8 == 0));
+}
+
+struct BwdLayout {       // byte offsets into the workspace of a backward pass
+    int64_t ldk, a, unscale, pairs, f, partial, total;
+};
+BwdLayout bwd_layout(int64_t T, int64_t C, int64_t R, int gs, int mats) {
+    BwdLayout L{};
+    const auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+    L.ldk = cdiv(mats * R, (int64_t)64) * 64;
+    L.a = 0;
+    L.unscale = up(T * L.ldk * 2);
+    L.pairs = L.unscale + up(T * 4);
+    L.f = L.pairs + up(mats * R * cdiv(C, (int64_t)gs) * 4);
+    L.partial = L.f + up(mats * R * 4);
+    L.total = L.partial + up(kBiasParts * R * 4);
+    return L;
+}
+
+template <typename T, bool GATED> void launch_dz(const DzParams &P, int act, cudaStream_t st) {
+    switch (act) {
+        case FORGE_ACT_RELU: dz_kernel<T, FORGE_ACT_RELU, GATED><<<(unsigned)P.T, 256, 0, st>>>(P); break;
+        case FORGE_ACT_SILU: dz_kernel<T, FORGE_ACT_SILU, GATED><<<(unsigned)P.T, 256, 0, st>>>(P); break;
+        case FORGE_ACT_GELU: dz_kernel<T, FORGE_ACT_GELU, GATED><<<(unsigned)P.T, 256, 0, st>>>(P); break;
+        default: dz_kernel<T, FORGE_ACT_NONE, GATED><<<(unsigned)P.T, 256, 0, st>>>(P);
+    }
+    FORGE_NOTE_LAUNCH();
+}
+template <typename T> void launch_dbias(const void *dy, int64_t lddy, const void *z, int act, int64_t n, int64_t R,
+                                        float *partial, void *out, cudaStream_t st) {
+    const int parts = (int)(n < kBiasParts ? (n > 0 ? n : 0) : kBiasParts);
+    if (parts > 0) {
+        const dim3 grid((unsigned)cdiv(R, (int64_t)256), parts);
+        switch (act) {
+            case FORGE_ACT_RELU: dbias_kernel<T, FORGE_ACT_RELU><<<grid, 256, 0, st>>>((const T *)dy, lddy, (const T *)z, n, R, partial); break;
+            case FORGE_ACT_SILU: dbias_kernel<T, FORGE_ACT_SILU><<<grid, 256, 0, st>>>((const T *)dy, lddy, (const T *)z, n, R, partial); break;
+            case FORGE_ACT_GELU: dbias_kernel<T, FORGE_ACT_GELU><<<grid, 256, 0, st>>>((const T *)dy, lddy, (const T *)z, n, R, partial); break;
+            default: dbias_kernel<T, FORGE_ACT_NONE><<<grid, 256, 0, st>>>((const T *)dy, lddy, (const T *)z, n, R, partial);
+        }
+        FORGE_NOTE_LAUNCH();
+    }
+    dbias_sum_kernel<T><<<(unsigned)cdiv(R, (int64_t)256), 256, 0, st>>>(partial, parts, R, (T *)out); FORGE_NOTE_LAUNCH();
+}
+
+template <typename T, bool GATED> int run_fwd(const Int4Fwd &P, cudaStream_t st) {
+    const int64_t max_rows = 65535 * 64ll;
+    for (int64_t t0 = 0; t0 < P.T; t0 += max_rows) {
+        Int4Fwd Q = P;
+        Q.T = imin64(P.T - t0, max_rows);
+        Q.x = (const T *)P.x + t0 * P.ldx;
+        if (P.res) Q.res = (const T *)P.res + t0 * P.ldres;
+        Q.y = (T *)P.y + t0 * P.R;
+        if (P.pre0) Q.pre0 = (T *)P.pre0 + t0 * P.R;
+        if (P.pre1) Q.pre1 = (T *)P.pre1 + t0 * P.R;
+        fwd_fma_kernel<T, GATED><<<dim3((unsigned)cdiv(P.R, (int64_t)64), (unsigned)cdiv(Q.T, (int64_t)64)), 256, 0, st>>>(Q);
+        FORGE_NOTE_LAUNCH();
+    }
+    return check_launch(GATED ? "forge_int4_gated" : "forge_int4_linear");
+}
+
+template <typename T> int run_dgrad(const Int4Dgrad &P, const char *who, cudaStream_t st) {
+    const int64_t max_rows = 65535 * 64ll;
+    for (int64_t t0 = 0; t0 < P.T; t0 += max_rows) {
+        Int4Dgrad Q = P;
+        Q.T = imin64(P.T - t0, max_rows);
+        Q.a = P.a + t0 * P.ldk;
+        Q.unscale = P.unscale + t0;
+        Q.dx = (T *)P.dx + t0 * P.C;
+        dgrad_fma_kernel<T><<<dim3((unsigned)cdiv(P.C, (int64_t)64), (unsigned)cdiv(Q.T, (int64_t)64)), 256, 0, st>>>(Q);
+        FORGE_NOTE_LAUNCH();
+    }
+    return check_launch(who);
+}
+
+}  // namespace
+
+extern "C" int forge_int4_linear(const void *x, int64_t ldx, int dtype, const int32_t *packed, const float *scales, int gs,
+                                 int64_t T, int64_t C, int64_t R, const void *bias, int act, const void *residual,
+                                 int64_t ldres, void *y, void *preact, int32_t *status, void *stream) {
+    if (int rc = check_sizes(__func__, dtype, T, C, R, gs, act)) return rc;
+    if (T == 0) return FORGE_OK;
+    FORGE_REQUIRE(x && packed && scales && y, "null pointer");
+    FORGE_REQUIRE(rows_ok(x, ldx, C, T), "x must be 16-byte aligned with a row stride >= C that is a multiple of 8");
+    FORGE_REQUIRE(!residual || T == 1 || ldres >= R, "residual row stride below R");
+    FORGE_REQUIRE((uintptr_t)y % 16 == 0 && (uintptr_t)preact % 16 == 0, "outputs must be 16-byte aligned");
+    Int4Fwd P{x, ldx, {(const uint32_t *)packed, nullptr}, {scales, nullptr}, gs, T, C, R, cdiv(C, (int64_t)gs), bias, act,
+              residual, ldres, y, preact, nullptr, status};
+    cudaStream_t st = (cudaStream_t)stream;
+    return dtype == FORGE_DTYPE_BF16 ? run_fwd<__nv_bfloat16, false>(P, st) : run_fwd<__half, false>(P, st);
+}
+
+extern "C" int forge_int4_gated(const void *x, int64_t ldx, int dtype, const int32_t *gate_packed, const float *gate_scales,
+                                const int32_t *up_packed, const float *up_scales, int gs, int64_t T, int64_t C, int64_t R,
+                                int act, void *h, void *g, void *u, int32_t *status, void *stream) {
+    if (int rc = check_sizes(__func__, dtype, T, C, R, gs, act)) return rc;
+    FORGE_REQUIRE(!g == !u, "g and u go together");
+    if (T == 0) return FORGE_OK;
+    FORGE_REQUIRE(x && gate_packed && gate_scales && up_packed && up_scales && h, "null pointer");
+    FORGE_REQUIRE(rows_ok(x, ldx, C, T), "x must be 16-byte aligned with a row stride >= C that is a multiple of 8");
+    FORGE_REQUIRE((uintptr_t)h % 16 == 0 && (uintptr_t)g % 16 == 0 && (uintptr_t)u % 16 == 0, "outputs must be 16-byte aligned");
+    Int4Fwd P{x, ldx, {(const uint32_t *)gate_packed, (const uint32_t *)up_packed}, {gate_scales, up_scales}, gs, T, C, R,
+              cdiv(C, (int64_t)gs), nullptr, act, nullptr, 0, h, g, u, status};
+    cudaStream_t st = (cudaStream_t)stream;
+    return dtype == FORGE_DTYPE_BF16 ? run_fwd<__nv_bfloat16, true>(P, st) : run_fwd<__half, true>(P, st);
+}
+
+extern "C" int64_t forge_int4_backward_workspace_bytes(int64_t T, int64_t C, int64_t R, int gs, int mats) {
+    if (T < 0 || C <= 0 || R <= 0 || gs <= 0 || mats < 1 || mats > 2 || T > kMaxTokens || C > kMaxDim || R > kMaxDim) return 0;
+    return bwd_layout(T, C, R, gs, mats).total;
+}
+
+static int backward(const char *who, const void *dy, int64_t lddy, int dtype, const int32_t *p0, const float *s0,
+                    const int32_t *p1, const float *s1, int gs, int64_t T, int64_t C, int64_t R, const void *z, const void *u,
+                    int act, void *dx, void *dbias, void *ws, int32_t *status, cudaStream_t st) {
+    const int mats = p1 ? 2 : 1;
+    const BwdLayout L = bwd_layout(T, C, R, gs, mats);
+    uint8_t *base = (uint8_t *)ws;
+    if (dbias) {
+        float *partial = (float *)(base + L.partial);
+        if (dtype == FORGE_DTYPE_BF16) launch_dbias<__nv_bfloat16>(dy, lddy, z, act, T, R, partial, dbias, st);
+        else launch_dbias<__half>(dy, lddy, z, act, T, R, partial, dbias, st);
+    }
+    if (!dx || T == 0) return check_launch(who);
+    const int64_t G = cdiv(C, (int64_t)gs);
+    scale_prep_kernel<<<(unsigned)cdiv(mats * R, (int64_t)8), 256, 0, st>>>(s0, s1, R, G, (__half2 *)(base + L.pairs),
+                                                                            (float *)(base + L.f));
+    FORGE_NOTE_LAUNCH();
+    DzParams D{dy, z, u, lddy, T, R, mats * R, L.ldk, (const float *)(base + L.f), (__half *)(base + L.a),
+               (float *)(base + L.unscale)};
+    if (dtype == FORGE_DTYPE_BF16) {
+        if (mats == 2) launch_dz<__nv_bfloat16, true>(D, act, st);
+        else launch_dz<__nv_bfloat16, false>(D, act, st);
+    } else {
+        if (mats == 2) launch_dz<__half, true>(D, act, st);
+        else launch_dz<__half, false>(D, act, st);
+    }
+    Int4Dgrad P{(const __half *)(base + L.a), L.ldk, (const float *)(base + L.unscale),
+                {(const uint32_t *)p0, (const uint32_t *)p1}, (const __half2 *)(base + L.pairs), gs, mats, T, C, R, G, dx, status};
+    return dtype == FORGE_DTYPE_BF16 ? run_dgrad<__nv_bfloat16>(P, who, st) : run_dgrad<__half>(P, who, st);
+}
+
+extern "C" int forge_int4_linear_backward(const void *dy, int64_t lddy, int dtype, const int32_t *packed, const float *scales,
+                                          int gs, int64_t T, int64_t C, int64_t R, const void *preact, int act, void *dx,
+                                          void *dbias, void *ws, int32_t *status, void *stream) {
+    if (int rc = check_sizes(__func__, dtype, T, C, R, gs, act)) return rc;
+    FORGE_REQUIRE(dx || dbias, "nothing to compute");
+    FORGE_REQUIRE(T == 0 || (dy && (!dx || (packed && scales)) && (act == FORGE_ACT_NONE || preact)), "null pointer");
+    FORGE_REQUIRE(ws && (uintptr_t)ws % 256 == 0, "workspace must be 256-byte aligned");
+    FORGE_REQUIRE(T <= 1 || lddy >= R, "dy row stride below R");
+    FORGE_REQUIRE((uintptr_t)dx % 16 == 0, "dx must be 16-byte aligned");
+    return backward(__func__, dy, lddy, dtype, packed, scales, nullptr, nullptr, gs, T, C, R, act == FORGE_ACT_NONE ? nullptr : preact,
+                    nullptr, act, dx, dbias, ws, status, (cudaStream_t)stream);
+}
+
+extern "C" int forge_int4_gated_backward(const void *dh, int64_t lddh, int dtype, const void *g, const void *u,
+                                         const int32_t *gate_packed, const float *gate_scales, const int32_t *up_packed,
+                                         const float *up_scales, int gs, int64_t T, int64_t C, int64_t R, int act, void *dx,
+                                         void *ws, int32_t *status, void *stream) {
+    if (int rc = check_sizes(__func__, dtype, T, C, R, gs, act)) return rc;
+    if (T == 0) return FORGE_OK;
+    FORGE_REQUIRE(dh && g && u && gate_packed && gate_scales && up_packed && up_scales && dx, "null pointer");
+    FORGE_REQUIRE(ws && (uintptr_t)ws % 256 == 0, "workspace must be 256-byte aligned");
+    FORGE_REQUIRE(T <= 1 || lddh >= R, "dh row stride below R");
+    FORGE_REQUIRE((uintptr_t)dx % 16 == 0, "dx must be 16-byte aligned");
+    return backward(__func__, dh, lddh, dtype, gate_packed, gate_scales, up_packed, up_scales, gs, T, C, R, g, u, act, dx,
+                    nullptr, ws, status, (cudaStream_t)stream);
+}

@@ -1,0 +1,459 @@
+// Root-mean-square norm of a row, with the residual's addition in front of it and, optionally, an 8-bit output:
+//   h = x + residual (fp32),   y = h * rsqrt(mean(h^2) + eps) * weight,   r = round(h)
+//   quantised form, per 128 consecutive channels of a row:  s = max(max|y|, 1e-12) / 448,  q = e4m3(y / s)
+// and its backward pass at the stored stream r:
+//   n = r * rstd,  t = dy * weight,  dx = rstd * (t - n * mean(t n)) + dresidual,  dweight = sum over rows of dy * n
+//
+// Bound by HBM: a row is read once, kept in registers across the reduction, and written once.  One row belongs to 32
+// threads (up to 1024 channels), or to a whole CTA of 256 or 1024 threads; a thread holds up to four 8-element vectors.
+// Rows that are longer, not a multiple of 8 channels, or not 16-byte aligned take the strided kernels below, which
+// read a row twice (the second time from cache).
+// dweight: every CTA walks rows and keeps its columns' sums in registers; one fp32 partial row per CTA, summed in a
+// fixed order by a second launch, so results do not depend on scheduling.
+#include "common.cuh"
+#include "elem.cuh"
+
+using namespace forge;
+
+namespace {
+
+constexpr int kQGroup = 128;
+constexpr float kF8Max = 448.0f, kAmaxFloor = 1e-12f;
+
+struct NormParams {
+    const void *x, *res, *w;
+    int64_t ldx, ldres, T, C;
+    int w_f32;
+    float eps;
+    void *y;             // element type, [T, C]; or e4m3 when scales is given
+    float *scales;       // [T, ceil(C/128)]
+    void *r;             // [T, C], written when res is given
+};
+struct NormBwdParams {
+    const void *dy, *x, *w, *dres;
+    int64_t lddy, ldx, lddres, T, C;
+    int w_f32;
+    float eps;
+    void *dx;
+    float *partial;      // [n_partial, C]
+    float *stats;        // [2, T]: rstd, mean(t n) (strided form only)
+    int n_partial;
+};
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
+}
+
+// Sum over the threads of a row: every thread gets it.  `slot` holds one float per warp and is used once per call site
+// and row (two slots alternate where a kernel walks several rows).
+template <int TPR> __device__ __forceinline__ float row_sum(float v, float *slot) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if constexpr (TPR > 32) {
+        constexpr int W = TPR / 32;
+        const int lane = threadIdx.x & 31;
+        if (lane == 0) slot[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = lane < W ? slot[lane] : 0.0f;
+#pragma unroll
+        for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        v = __shfl_sync(0xffffffffu, v, 0);
+    }
+    return v;
+}
+
+template <typename T> __device__ __forceinline__ void load_w8(const NormParams &P, int64_t c, float (&v)[8]) {
+    if (P.w_f32) load8((const float *)P.w + c, v);
+    else load8((const T *)P.w + c, v);
+}
+template <typename T> __device__ __forceinline__ float load_w(const void *w, int w_f32, int64_t c) {
+    return w_f32 ? ((const float *)w)[c] : Elem<T>::to_f(((const T *)w)[c]);
+}
+
+template <typename T, int TPR, int NV>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) rmsnorm_kernel(const NormParams P) {
+    constexpr int kRows = TPR == 32 ? 8 : 1;
+    __shared__ float slot[32];
+    const int64_t row = (int64_t)blockIdx.x * kRows + (TPR == 32 ? threadIdx.x / 32 : 0);
+    if (TPR == 32 && row >= P.T) return;
+    const int t = threadIdx.x % TPR;
+    const int C = (int)P.C;
+    const T *x = (const T *)P.x + row * P.ldx;
+    float h[NV][8], w[NV][8];
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (t + i * TPR) * 8;
+        if (c < C) {
+            load8(x + c, h[i]);
+            load_w8<T>(P, c, w[i]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[i][e] = w[i][e] = 0.0f;
+        }
+    }
+    if (P.res) {
+        const T *res = (const T *)P.res + row * P.ldres;
+        T *r = (T *)P.r + row * P.C;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (t + i * TPR) * 8;
+            if (c < C) {
+                float v[8];
+                load8(res + c, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) h[i][e] += v[e];
+                store8(r + c, h[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fmaf(h[i][e], h[i][e], ss);
+    const float rstd = rsqrtf(row_sum<TPR>(ss, slot) / (float)C + P.eps);
+    if (!P.scales) {
+        T *y = (T *)P.y + row * P.C;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (t + i * TPR) * 8;
+            if (c < C) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) h[i][e] = h[i][e] * rstd * w[i][e];
+                store8(y + c, h[i]);
+            }
+        }
+        return;
+    }
+    uint8_t *q = (uint8_t *)P.y + row * P.C;
+    float *srow = P.scales + row * cdiv(P.C, (int64_t)kQGroup);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (t + i * TPR) * 8;
+        float amax = kAmaxFloor;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            h[i][e] = h[i][e] * rstd * w[i][e];
+            if (c < C) amax = max_nan(amax, fabsf(h[i][e]));   // channels past the row are not part of its group
+        }
+        // 16 neighbouring threads hold a group of 128 channels
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        const float s = amax / kF8Max, inv = 1.0f / s;
+        if (c < C) {
+            uint2 out;
+            out.x = e4m3x4(h[i][0] * inv, h[i][1] * inv, h[i][2] * inv, h[i][3] * inv);
+            out.y = e4m3x4(h[i][4] * inv, h[i][5] * inv, h[i][6] * inv, h[i][7] * inv);
+            *reinterpret_cast<uint2 *>(q + c) = out;
+            if ((t & 15) == 0) srow[c / kQGroup] = s;
+        }
+    }
+}
+
+// Any length, stride and alignment: the row is read twice.
+template <typename T> __global__ void __launch_bounds__(256) rmsnorm_strided_kernel(const NormParams P) {
+    __shared__ float slot[32];
+    const int64_t row = blockIdx.x;
+    const T *x = (const T *)P.x + row * P.ldx;
+    const T *res = P.res ? (const T *)P.res + row * P.ldres : nullptr;
+    float ss = 0.0f;
+    for (int64_t c = threadIdx.x; c < P.C; c += 256) {
+        float h = Elem<T>::to_f(x[c]);
+        if (res) {
+            h += Elem<T>::to_f(res[c]);
+            ((T *)P.r)[row * P.C + c] = Elem<T>::from_f(h);
+        }
+        ss = fmaf(h, h, ss);
+    }
+    const float rstd = rsqrtf(row_sum<256>(ss, slot) / (float)P.C + P.eps);
+    if (!P.scales) {
+        for (int64_t c = threadIdx.x; c < P.C; c += 256) {
+            float h = Elem<T>::to_f(x[c]);
+            if (res) h += Elem<T>::to_f(res[c]);
+            ((T *)P.y)[row * P.C + c] = Elem<T>::from_f(h * rstd * load_w<T>(P.w, P.w_f32, c));
+        }
+        return;
+    }
+    const int64_t G = cdiv(P.C, (int64_t)kQGroup);
+    const int lane = threadIdx.x & 31;
+    for (int64_t g = threadIdx.x >> 5; g < G; g += 8) {      // a warp per group of 128 channels
+        float v[4], amax = kAmaxFloor;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t c = g * kQGroup + k * 32 + lane;
+            v[k] = 0.0f;
+            if (c < P.C) {
+                float h = Elem<T>::to_f(x[c]);
+                if (res) h += Elem<T>::to_f(res[c]);
+                v[k] = h * rstd * load_w<T>(P.w, P.w_f32, c);
+                amax = max_nan(amax, fabsf(v[k]));
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        const float s = amax / kF8Max, inv = 1.0f / s;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t c = g * kQGroup + k * 32 + lane;
+            if (c < P.C)
+                ((uint8_t *)P.y)[row * P.C + c] = __nv_cvt_float_to_fp8(v[k] * inv, __NV_SATFINITE, __NV_E4M3);
+        }
+        if (lane == 0) P.scales[row * G + g] = s;
+    }
+}
+
+// Backward: every CTA (or warp, TPR = 32) walks rows; column sums of dy * n stay in registers.
+template <typename T, int TPR, int NV>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) rmsnorm_bwd_kernel(const NormBwdParams P) {
+    constexpr int kRows = TPR == 32 ? 8 : 1;
+    __shared__ float slot[2][2][32];
+    const int t = threadIdx.x % TPR;
+    const int C = (int)P.C;
+    const int64_t unit = (int64_t)blockIdx.x * kRows + (TPR == 32 ? threadIdx.x / 32 : 0);
+    const int64_t units = (int64_t)gridDim.x * kRows;
+    float w[NV][8], dw[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (t + i * TPR) * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[i][e] = dw[i][e] = 0.0f;
+        if (c < C) {
+            if (P.w_f32) load8((const float *)P.w + c, w[i]);
+            else load8((const T *)P.w + c, w[i]);
+        }
+    }
+    int flip = 0;
+    for (int64_t row = unit; row < P.T; row += units, flip ^= 1) {
+        const T *x = (const T *)P.x + row * P.ldx, *dy = (const T *)P.dy + row * P.lddy;
+        float r[NV][8], g[NV][8];
+        float ss = 0.0f, dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (t + i * TPR) * 8;
+            if (c < C) {
+                load8(x + c, r[i]);
+                load8(dy + c, g[i]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) r[i][e] = g[i][e] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                ss = fmaf(r[i][e], r[i][e], ss);
+                dot = fmaf(g[i][e] * w[i][e], r[i][e], dot);
+            }
+        ss = row_sum<TPR>(ss, slot[flip][0]);
+        dot = row_sum<TPR>(dot, slot[flip][1]);
+        const float rstd = rsqrtf(ss / (float)C + P.eps);
+        const float c1 = dot * rstd / (float)C;                 // mean(t n)
+        T *dx = (T *)P.dx + row * P.C;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (t + i * TPR) * 8;
+            if (c < C) {
+                float o[8], d[8];
+                if (P.dres) load8((const T *)P.dres + row * P.lddres + c, d);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float n = r[i][e] * rstd;
+                    dw[i][e] = fmaf(g[i][e], n, dw[i][e]);
+                    o[e] = rstd * (g[i][e] * w[i][e] - n * c1);
+                    if (P.dres) o[e] += d[e];
+                }
+                store8(dx + c, o);
+            }
+        }
+    }
+    float *part = P.partial + unit * P.C;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (t + i * TPR) * 8;
+        if (c < C) store8(part + c, dw[i]);
+    }
+}
+
+template <typename T> __global__ void __launch_bounds__(256) rmsnorm_bwd_strided_kernel(const NormBwdParams P) {
+    __shared__ float slot[2][32];
+    const int64_t row = blockIdx.x;
+    const T *x = (const T *)P.x + row * P.ldx, *dy = (const T *)P.dy + row * P.lddy;
+    float ss = 0.0f, dot = 0.0f;
+    for (int64_t c = threadIdx.x; c < P.C; c += 256) {
+        const float r = Elem<T>::to_f(x[c]);
+        ss = fmaf(r, r, ss);
+        dot = fmaf(Elem<T>::to_f(dy[c]) * load_w<T>(P.w, P.w_f32, c), r, dot);
+    }
+    ss = row_sum<256>(ss, slot[0]);
+    dot = row_sum<256>(dot, slot[1]);
+    const float rstd = rsqrtf(ss / (float)P.C + P.eps), c1 = dot * rstd / (float)P.C;
+    if (threadIdx.x == 0) P.stats[row] = rstd;
+    for (int64_t c = threadIdx.x; c < P.C; c += 256) {
+        float o = rstd * (Elem<T>::to_f(dy[c]) * load_w<T>(P.w, P.w_f32, c) - Elem<T>::to_f(x[c]) * rstd * c1);
+        if (P.dres) o += Elem<T>::to_f(((const T *)P.dres)[row * P.lddres + c]);
+        ((T *)P.dx)[row * P.C + c] = Elem<T>::from_f(o);
+    }
+}
+// column sums for the strided form: partial row blockIdx.y covers its share of the rows
+template <typename T> __global__ void __launch_bounds__(256) rmsnorm_dw_strided_kernel(const NormBwdParams P) {
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c >= P.C) return;
+    const int64_t per = cdiv(P.T, (int64_t)P.n_partial);
+    const int64_t r0 = blockIdx.y * per, r1 = imin64(P.T, r0 + per);
+    float s = 0.0f;
+#pragma unroll 4
+    for (int64_t row = r0; row < r1; ++row)
+        s = fmaf(Elem<T>::to_f(((const T *)P.dy)[row * P.lddy + c]),
+                 Elem<T>::to_f(((const T *)P.x)[row * P.ldx + c]) * P.stats[row], s);
+    P.partial[(int64_t)blockIdx.y * P.C + c] = s;
+}
+
+// out[c] = sum over n rows of partial[n, C], in a fixed order: 32 columns x 8 row strands per CTA
+template <typename T>
+__global__ void __launch_bounds__(256) column_sum_kernel(const float *__restrict__ partial, int n, int64_t C, T *out) {
+    __shared__ float s[8][33];
+    const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+    const int k = threadIdx.x >> 5;
+    float v = 0.0f;
+    if (c < C)
+#pragma unroll 4
+        for (int r = k; r < n; r += 8) v += partial[(int64_t)r * C + c];
+    s[k][threadIdx.x & 31] = v;
+    __syncthreads();
+    if (k == 0 && c < C) {
+        v = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v += s[j][threadIdx.x];
+        out[c] = Elem<T>::from_f(v);
+    }
+}
+
+constexpr int64_t kMaxRows = 0x7fffffffLL;       // one CTA per row at most
+// Rows per partial sum: up to two CTAs per SM walk the rows
+constexpr int kBwdCtas = 296;
+
+bool vec_ok(const void *p, int64_t ld, size_t es) { return ((uintptr_t)p % 16 == 0) && (ld * (int64_t)es) % 16 == 0; }
+// The row-in-registers kernels: (threads per row, vectors per thread) by length; 0 = strided form.
+struct RowShape { int tpr, nv; };
+RowShape row_shape(int64_t C) {
+    if (C <= 256) return {32, 1};
+    if (C <= 512) return {32, 2};
+    if (C <= 1024) return {32, 4};
+    if (C <= 2048) return {256, 1};
+    if (C <= 4096) return {256, 2};
+    if (C <= 8192) return {256, 4};
+    if (C <= 16384) return {1024, 2};
+    return {0, 0};
+}
+
+template <typename T> void launch_fwd(const NormParams &P, RowShape s, cudaStream_t st) {
+#define FORGE_NORM_CASE(TPR, NV)                                                                            \
+    if (s.tpr == TPR && s.nv == NV) {                                                                       \
+        const int rows = TPR == 32 ? 8 : 1;                                                                 \
+        rmsnorm_kernel<T, TPR, NV><<<(unsigned)cdiv(P.T, (int64_t)rows), TPR == 32 ? 256 : TPR, 0, st>>>(P); \
+        return;                                                                                             \
+    }
+    FORGE_NORM_CASE(32, 1) FORGE_NORM_CASE(32, 2) FORGE_NORM_CASE(32, 4) FORGE_NORM_CASE(256, 1)
+    FORGE_NORM_CASE(256, 2) FORGE_NORM_CASE(256, 4) FORGE_NORM_CASE(1024, 2)
+#undef FORGE_NORM_CASE
+    rmsnorm_strided_kernel<T><<<(unsigned)P.T, 256, 0, st>>>(P);
+}
+
+int bwd_ctas(int64_t T, RowShape s) {
+    const int64_t rows = s.tpr == 32 ? 8 : 1;
+    return (int)imin64(cdiv(T, rows), kBwdCtas);
+}
+int strided_partials(int64_t T) { return (int)imin64(cdiv(T, (int64_t)16), 64); }
+
+template <typename T> void launch_bwd(NormBwdParams &P, RowShape s, cudaStream_t st) {
+#define FORGE_NORM_CASE(TPR, NV)                                                                             \
+    if (s.tpr == TPR && s.nv == NV) {                                                                        \
+        const int ctas = bwd_ctas(P.T, s);                                                                   \
+        P.n_partial = ctas * (TPR == 32 ? 8 : 1);                                                            \
+        rmsnorm_bwd_kernel<T, TPR, NV><<<ctas, TPR == 32 ? 256 : TPR, 0, st>>>(P); FORGE_NOTE_LAUNCH();       \
+        return;                                                                                              \
+    }
+    FORGE_NORM_CASE(32, 1) FORGE_NORM_CASE(32, 2) FORGE_NORM_CASE(32, 4) FORGE_NORM_CASE(256, 1)
+    FORGE_NORM_CASE(256, 2) FORGE_NORM_CASE(256, 4) FORGE_NORM_CASE(1024, 2)
+#undef FORGE_NORM_CASE
+    P.n_partial = strided_partials(P.T);
+    rmsnorm_bwd_strided_kernel<T><<<(unsigned)P.T, 256, 0, st>>>(P); FORGE_NOTE_LAUNCH();
+    rmsnorm_dw_strided_kernel<T><<<dim3((unsigned)cdiv(P.C, (int64_t)256), P.n_partial), 256, 0, st>>>(P);
+    FORGE_NOTE_LAUNCH();
+}
+
+size_t elem_size(int dtype) { return dtype == FORGE_DTYPE_F32 ? 4 : 2; }
+bool known_dtype(int d) { return d == FORGE_DTYPE_F32 || d == FORGE_DTYPE_BF16 || d == FORGE_DTYPE_F16; }
+
+}  // namespace
+
+extern "C" int forge_rmsnorm(const void *x, int64_t ldx, const void *residual, int64_t ldres, const void *weight,
+                             int w_dtype, int dtype, int64_t T, int64_t C, float eps, void *y, float *scales,
+                             void *residual_out, void *stream) {
+    FORGE_REQUIRE(T >= 0 && T <= kMaxRows && C > 0 && C <= kMaxRows, "bad sizes");
+    FORGE_REQUIRE(known_dtype(dtype), "dtype must be fp32, bf16 or fp16");
+    FORGE_REQUIRE(w_dtype == dtype || w_dtype == FORGE_DTYPE_F32, "weight must be fp32 or of x's type");
+    if (T == 0) return FORGE_OK;
+    FORGE_REQUIRE(x && weight && y, "null pointer");
+    FORGE_REQUIRE(!residual == !residual_out, "residual and residual_out go together");
+    FORGE_REQUIRE((T == 1 || ldx >= C) && (!residual || T == 1 || ldres >= C), "row stride below the row length");
+    NormParams P{x, residual, weight, ldx, ldres, T, C, w_dtype == FORGE_DTYPE_F32, eps, y, scales, residual_out};
+    const size_t es = elem_size(dtype), ws = elem_size(w_dtype);
+    const bool vec = C % 8 == 0 && vec_ok(x, ldx, es) && (!residual || (vec_ok(residual, ldres, es) &&
+                     vec_ok(residual_out, C, es))) && vec_ok(weight, 0, ws) && (uintptr_t)y % 16 == 0;
+    const RowShape s = vec ? row_shape(C) : RowShape{0, 0};
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == FORGE_DTYPE_F32) launch_fwd<float>(P, s, st);
+    else if (dtype == FORGE_DTYPE_BF16) launch_fwd<__nv_bfloat16>(P, s, st);
+    else launch_fwd<__half>(P, s, st);
+    FORGE_NOTE_LAUNCH();
+    return check_launch("forge_rmsnorm");
+}
+
+extern "C" int64_t forge_rmsnorm_backward_workspace_bytes(int64_t T, int64_t C) {
+    if (T <= 0 || C <= 0 || T > kMaxRows || C > kMaxRows) return 16;
+    const RowShape s = row_shape(C);
+    const int64_t a = s.tpr ? (int64_t)bwd_ctas(T, s) * (s.tpr == 32 ? 8 : 1) * C * 4 : 0;
+    const int64_t b = (int64_t)strided_partials(T) * C * 4 + T * 4 + 16;
+    return a > b ? a : b;
+}
+
+extern "C" int forge_rmsnorm_backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, const void *weight,
+                                      int w_dtype, int dtype, const void *dresidual, int64_t lddres, int64_t T,
+                                      int64_t C, float eps, void *dx, void *dweight, void *ws, void *stream) {
+    FORGE_REQUIRE(T >= 0 && T <= kMaxRows && C > 0 && C <= kMaxRows, "bad sizes");
+    FORGE_REQUIRE(known_dtype(dtype), "dtype must be fp32, bf16 or fp16");
+    FORGE_REQUIRE(w_dtype == dtype || w_dtype == FORGE_DTYPE_F32, "weight must be fp32 or of x's type");
+    FORGE_REQUIRE(dweight, "null pointer");
+    cudaStream_t st = (cudaStream_t)stream;
+    NormBwdParams P{dy, x, weight, dresidual, lddy, ldx, lddres, T, C, w_dtype == FORGE_DTYPE_F32, eps, dx,
+                    (float *)ws, nullptr, 0};
+    if (T > 0) {
+        FORGE_REQUIRE(dy && x && weight && dx && ws, "null pointer");
+        FORGE_REQUIRE((uintptr_t)ws % 16 == 0, "workspace must be 16-byte aligned");
+        FORGE_REQUIRE(T == 1 || (lddy >= C && ldx >= C && (!dresidual || lddres >= C)), "row stride below the row length");
+        const size_t es = elem_size(dtype), wsz = elem_size(w_dtype);
+        const bool vec = C % 8 == 0 && vec_ok(x, ldx, es) && vec_ok(dy, lddy, es) &&
+                         (!dresidual || vec_ok(dresidual, lddres, es)) && vec_ok(weight, 0, wsz) && (uintptr_t)dx % 16 == 0;
+        const RowShape s = vec ? row_shape(C) : RowShape{0, 0};
+        P.stats = P.partial + (int64_t)strided_partials(T) * C;
+        if (dtype == FORGE_DTYPE_F32) launch_bwd<float>(P, s, st);
+        else if (dtype == FORGE_DTYPE_BF16) launch_bwd<__nv_bfloat16>(P, s, st);
+        else launch_bwd<__half>(P, s, st);
+    }
+    const unsigned blocks = (unsigned)cdiv(C, (int64_t)32);
+    if (w_dtype == FORGE_DTYPE_F32) column_sum_kernel<float><<<blocks, 256, 0, st>>>(P.partial, P.n_partial, C, (float *)dweight);
+    else if (w_dtype == FORGE_DTYPE_BF16)
+        column_sum_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(P.partial, P.n_partial, C, (__nv_bfloat16 *)dweight);
+    else column_sum_kernel<__half><<<blocks, 256, 0, st>>>(P.partial, P.n_partial, C, (__half *)dweight);
+    FORGE_NOTE_LAUNCH();
+    return check_launch("forge_rmsnorm_backward");
+}

@@ -14,10 +14,11 @@ import torch
 _PKG_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(_PKG_ROOT, "libforge_b200.so")
 
-F32, BF16 = 0, 1
+F32, BF16, F16 = 0, 1, 2
 HESS_MIRROR, HESS_SIMT = 1, 2
 FWD_SIMT = 1
 ROUTE_MODES = {"softmax": 0, "sigmoid": 1, "sigmoid_group": 2}
+ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 ERR_INVALID, ERR_TIMEOUT = 1, 3
 
 _c_i64 = ctypes.c_int64
@@ -67,6 +68,19 @@ _PROTOS = {
     "forge_sparse14_gemm": (_c_int, [_ptr, _ptr, _c_i64, _c_i64, _c_i64, _c_i64, _ptr, _ptr]),
     "forge_sparse14_moe_w13_swiglu": (_c_int, [_ptr, _ptr, _c_i64, _c_i64, _ptr, _ptr, _ptr, _c_int, _c_i64, _c_i64, _c_i64, _ptr, _ptr]),
     "forge_sparse14_moe_w2": (_c_int, [_ptr, _ptr, _c_i64, _c_i64, _ptr, _ptr, _ptr, _c_int, _c_i64, _c_i64, _c_i64, _ptr, _ptr]),
+    "forge_rmsnorm": (_c_int, [_ptr, _c_i64, _ptr, _c_i64, _ptr, _c_int, _c_int, _c_i64, _c_i64, _c_f32, _ptr, _ptr, _ptr, _ptr]),
+    "forge_rmsnorm_backward_workspace_bytes": (_c_i64, [_c_i64, _c_i64]),
+    "forge_rmsnorm_backward": (_c_int, [_ptr, _c_i64, _ptr, _c_i64, _ptr, _c_int, _c_int, _ptr, _c_i64, _c_i64, _c_i64, _c_f32,
+                                        _ptr, _ptr, _ptr, _ptr]),
+    "forge_int4_linear": (_c_int, [_ptr, _c_i64, _c_int, _ptr, _ptr, _c_int, _c_i64, _c_i64, _c_i64, _ptr, _c_int, _ptr, _c_i64,
+                                   _ptr, _ptr, _ptr, _ptr]),
+    "forge_int4_gated": (_c_int, [_ptr, _c_i64, _c_int, _ptr, _ptr, _ptr, _ptr, _c_int, _c_i64, _c_i64, _c_i64, _c_int, _ptr,
+                                  _ptr, _ptr, _ptr, _ptr]),
+    "forge_int4_backward_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_int, _c_int]),
+    "forge_int4_linear_backward": (_c_int, [_ptr, _c_i64, _c_int, _ptr, _ptr, _c_int, _c_i64, _c_i64, _c_i64, _ptr, _c_int,
+                                            _ptr, _ptr, _ptr, _ptr, _ptr]),
+    "forge_int4_gated_backward": (_c_int, [_ptr, _c_i64, _c_int, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_i64, _c_i64,
+                                           _c_i64, _c_int, _ptr, _ptr, _ptr, _ptr]),
 }
 
 _lib = None

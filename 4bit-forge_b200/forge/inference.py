@@ -59,3 +59,123 @@ class Sparse14MoERuntime:
             out = torch.zeros((T, H), dtype=torch.float32, device=hidden_states.device)
             out.index_add_(0, tok, out_perm.float() * w[:, None])
         return out.to(hidden_states.dtype)
+
+
+# ---- dense feed-forward block on pack-quantized int4 weights ---------------------------------------------------------
+class _RMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, h = (ops.rmsnorm(x, weight, eps), x) if residual is None else ops.rmsnorm(x, weight, eps, residual=residual)
+        ctx.save_for_backward(h, weight)
+        ctx.eps, ctx.has_residual = eps, residual is not None
+        return (y, h) if residual is not None else (y, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh):
+        h, weight = ctx.saved_tensors
+        dx, dw = ops.rmsnorm_backward(dy, h, weight, ctx.eps, dresidual=dh if ctx.has_residual else None)
+        return dx, dw, dx if ctx.has_residual else None, None
+
+
+class _Int4Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, bias, residual, packed, scales, gs, act):
+        want = act != "none"
+        out = ops.int4_linear(x, packed, scales, gs, bias=bias, act=act, residual=residual, want_preact=want)
+        y, z = out if want else (out, None)
+        ctx.save_for_backward(z, packed, scales)
+        ctx.gs, ctx.act = gs, act
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        z, packed, scales = ctx.saved_tensors
+        need_x, need_b, need_r = ctx.needs_input_grad[:3]
+        dx = db = None
+        if need_x or need_b:
+            dx, db = ops.int4_linear_backward(dy, packed, scales, ctx.gs, preact=z, act=ctx.act, want_dx=need_x,
+                                              want_dbias=need_b)
+        return dx, db, dy if need_r else None, None, None, None, None
+
+
+class _Int4Gated(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, wg, sg, wu, su, gs, act):
+        h, g, u = ops.int4_gated(x, wg, sg, wu, su, gs, act=act, want_preact=True)
+        ctx.save_for_backward(g, u, wg, sg, wu, su)
+        ctx.gs, ctx.act = gs, act
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        g, u, wg, sg, wu, su = ctx.saved_tensors
+        return ops.int4_gated_backward(dh, g, u, wg, sg, wu, su, ctx.gs, act=ctx.act), None, None, None, None, None, None
+
+
+def _grad_wanted(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+class Int4FeedForward(torch.nn.Module):
+    """The dense feed-forward block on the quantiser's own results: a shared expert, or any gated block whose three
+    matrices went through pack_int4 with symmetric codes.
+
+        forward(hidden)            -> down(act(gate(x)) * up(x)) [+ hidden],   x = norm(hidden)
+        forward(hidden, residual)  -> the same with hidden + residual in hidden's place
+
+    gate, up [I, H/8] and down [H, I/8] are (weight_packed, scales) pairs.  With norm_weight [H] the block starts with a
+    root-mean-square norm and its result is added to the residual stream (four kernels less one: norm, gated product,
+    product with the residual in its epilogue); without one it is the bare block and takes no residual.  The int4 weights
+    are frozen; gradients reach hidden, residual and the norm's gain (tuning through the quantised block).  The reference
+    runs its packed dense experts through vLLM and has no such block of its own."""
+
+    def __init__(self, gate, up, down, group_size=128, act="silu", norm_weight=None, eps=1e-6):
+        super().__init__()
+        self.group_size, self.act, self.eps = int(group_size), act, float(eps)
+        for name, (packed, scales) in (("gate", gate), ("up", up), ("down", down)):
+            self.register_buffer(name + "_packed", packed.contiguous())
+            self.register_buffer(name + "_scales", scales.to(torch.float32).contiguous())
+        I, H8 = self.gate_packed.shape
+        if self.up_packed.shape != (I, H8) or self.down_packed.shape != (H8 * 8, I // 8) or I % 8:
+            raise RuntimeError("gate and up must be [I, H/8] and down [H, I/8] packed words")
+        self.norm_weight = None if norm_weight is None else torch.nn.Parameter(norm_weight.detach().clone())
+
+    @classmethod
+    def from_quantized(cls, out, index, group_size=128, **kw):
+        """Matrix `index` of every family of MoELayerQuantizer.quantize_experts(...) (cfg.pack, symmetric, "gptq"): routed
+        experts first, then the shared ones."""
+        pairs = []
+        for fam in ("gate", "up", "down"):
+            packed = out[fam]["weight_packed"][index]
+            pairs.append((packed, out[fam]["scales"][index].view(packed.shape[0], -1)))
+        return cls(*pairs, group_size=group_size, **kw)
+
+    def forward(self, hidden, residual=None):
+        if residual is not None and self.norm_weight is None:
+            raise RuntimeError("a block without a norm takes no residual")
+        shape = hidden.shape
+        x = hidden.reshape(-1, shape[-1])
+        res = None if residual is None else residual.reshape(-1, shape[-1])
+        w, gs, act = self.norm_weight, self.group_size, self.act
+        gate = (self.gate_packed, self.gate_scales, self.up_packed, self.up_scales, gs)
+        down = (self.down_packed, self.down_scales, gs)
+        if _grad_wanted(x, res, w):
+            if w is None:
+                y, h = x, None
+            else:
+                y, h = _RMSNorm.apply(x, w, res, self.eps)
+                h = x if h is None else h
+            a = _Int4Gated.apply(y, *gate, act)
+            out = _Int4Linear.apply(a, None, h, *down, "none")
+        else:
+            if w is None:
+                y, h = x, None
+            elif res is None:
+                y, h = ops.rmsnorm(x, w, self.eps), x
+            else:
+                y, h = ops.rmsnorm(x, w, self.eps, residual=res)
+            out = ops.int4_linear(ops.int4_gated(y, *gate, act=act), *down, residual=h)
+        return out.view(shape)

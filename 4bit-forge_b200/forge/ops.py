@@ -356,3 +356,240 @@ def mma_issue_cycles(N: int = 128, iters: int = 2000, pattern: bool = True) -> f
     if vals[1] != 0:
         raise RuntimeError(f"forge_selftest_mma_rate: status {vals[1]}")
     return vals[0] / float(iters)
+
+
+# ---- the feed-forward block on packed int4 weights -----------------------------------------------------------------
+# Activations are 2-D [tokens, channels].  A row-strided view is read in place (16-byte aligned rows for the products);
+# anything else is copied once.  Outputs are dense.  Every call works on the device of its first argument, on that
+# device's current stream.
+
+_ACT_DTYPES = {torch.float32: _abi.F32, torch.bfloat16: _abi.BF16, torch.float16: _abi.F16}
+
+
+def _require(cond, msg):
+    if not cond:
+        raise RuntimeError(f"forge_b200: {msg}")
+
+
+def _same_device(dev, *tensors):
+    for t in tensors:
+        _require(t is None or t.device == dev, "all tensors must be on the device of the first argument")
+
+
+def _rows(t, aligned: bool):
+    """(tensor, row stride) of a 2-D tensor whose rows are contiguous; aligned: every row starts on 16 bytes."""
+    T, C = t.shape
+    ld = t.stride(0) if T > 1 else C
+    if (t.stride(1) != 1 and C > 1) or ld < C or (aligned and (ld % 8 or t.data_ptr() % 16)):
+        t = t.clone(memory_format=torch.contiguous_format)
+        ld = C
+    return t, ld
+
+
+def _check_rows(t, name, shape=None, dtype=None):
+    _require(t.dim() == 2 and (shape is None or tuple(t.shape) == shape), f"{name} must be 2-D" if shape is None else
+             f"{name} must have the shape {list(shape)}, got {list(t.shape)}")
+    _require(dtype is None or t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}")
+
+
+def rmsnorm(x, weight, eps: float = 1e-6, residual=None, quant_group: int = 0):
+    """Root-mean-square norm of the rows of x [T, C] (fp32, bf16 or fp16), after adding `residual` when given
+    (forge_rmsnorm): y = h / sqrt(mean(h^2) + eps) * weight with h = x + residual in fp32.  weight [C] of x's type or fp32.
+
+    Returns y, or (y, h) with a residual: h rounded to x's type is the new residual stream.  quant_group=128 returns the
+    8-bit form instead of y: (q, scales) or (q, scales, h), q float8_e4m3fn [T, C], scales fp32 [T, ceil(C/128)], such that
+    q * scales, group by group, is y: the layout fp8_block_dequant reads when C is a multiple of 128."""
+    _abi._require_cuda()
+    _require(x.is_cuda, "x must be a CUDA tensor")
+    if x.device.index != torch.cuda.current_device():
+        with torch.cuda.device(x.device):
+            return rmsnorm(x, weight, eps, residual, quant_group)
+    _check_rows(x, "x")
+    T, C = x.shape
+    _require(C > 0, "x has no channels")
+    _require(x.dtype in _ACT_DTYPES, f"x must be float32, bfloat16 or float16, got {x.dtype}")
+    _require(weight.shape == (C,) and weight.dtype in (x.dtype, torch.float32), "weight must be [C], of x's type or float32")
+    _require(quant_group in (0, 128), "quant_group must be 0 (no quantisation) or 128")
+    _same_device(x.device, weight, residual)
+    x, ldx = _rows(x, False)
+    ldres, h = 0, None
+    if residual is not None:
+        _check_rows(residual, "residual", (T, C), x.dtype)
+        residual, ldres = _rows(residual, False)
+        h = torch.empty((T, C), dtype=x.dtype, device=x.device)
+    scales = torch.empty((T, (C + 127) // 128), dtype=torch.float32, device=x.device) if quant_group else None
+    y = torch.empty((T, C), dtype=torch.float8_e4m3fn if quant_group else x.dtype, device=x.device)
+    call("forge_rmsnorm", x.data_ptr(), ldx, None if residual is None else residual.data_ptr(), ldres,
+         ptr(weight.contiguous()), _ACT_DTYPES[weight.dtype], _ACT_DTYPES[x.dtype], T, C, float(eps), ptr(y), ptr(scales),
+         ptr(h), stream_ptr())
+    out = (y, scales) if quant_group else (y,)
+    if h is not None:
+        out += (h,)
+    return out[0] if len(out) == 1 else out
+
+
+def rmsnorm_backward(dy, x, weight, eps: float = 1e-6, dresidual=None):
+    """Gradients of rmsnorm at the normed rows x (the h of the forward call when it had a residual): returns (dx, dweight),
+    dx [T, C] of x's type with `dresidual` (the gradient that reaches h past the norm) added, dweight [C] of the weight's
+    type (forge_rmsnorm_backward).  dx is the gradient of the forward call's x and of its residual alike."""
+    _abi._require_cuda()
+    _require(dy.is_cuda, "dy must be a CUDA tensor")
+    if dy.device.index != torch.cuda.current_device():
+        with torch.cuda.device(dy.device):
+            return rmsnorm_backward(dy, x, weight, eps, dresidual)
+    _check_rows(x, "x")
+    T, C = x.shape
+    _require(C > 0, "x has no channels")
+    _require(x.dtype in _ACT_DTYPES, f"x must be float32, bfloat16 or float16, got {x.dtype}")
+    _check_rows(dy, "dy", (T, C), x.dtype)
+    _require(weight.shape == (C,) and weight.dtype in (x.dtype, torch.float32), "weight must be [C], of x's type or float32")
+    _same_device(dy.device, x, weight, dresidual)
+    (dy, lddy), (x, ldx) = _rows(dy, False), _rows(x, False)
+    lddres = 0
+    if dresidual is not None:
+        _check_rows(dresidual, "dresidual", (T, C), x.dtype)
+        dresidual, lddres = _rows(dresidual, False)
+    dx = torch.empty((T, C), dtype=x.dtype, device=x.device)
+    dw = torch.empty((C,), dtype=weight.dtype, device=x.device)
+    ws = torch.empty(query("forge_rmsnorm_backward_workspace_bytes", T, C), dtype=torch.uint8, device=x.device)
+    call("forge_rmsnorm_backward", dy.data_ptr(), lddy, x.data_ptr(), ldx, ptr(weight.contiguous()),
+         _ACT_DTYPES[weight.dtype], _ACT_DTYPES[x.dtype], None if dresidual is None else dresidual.data_ptr(), lddres, T, C,
+         float(eps), ptr(dx), ptr(dw), ptr(ws), stream_ptr())
+    return dx, dw
+
+
+def _int4_weight(packed, scales, gs, dev, name):
+    """Checks a pack-quantized matrix; returns (packed, scales fp32, R, C)."""
+    _require(gs in (32, 64, 128), "group size must be 32, 64 or 128")
+    _require(packed.dim() == 2 and packed.dtype == torch.int32 and packed.is_contiguous() and packed.numel() > 0,
+             f"{name} must be a contiguous int32 matrix [R, C/8]")
+    R, C = packed.shape[0], packed.shape[1] * 8
+    _require(tuple(scales.shape) == (R, (C + gs - 1) // gs), f"the scales of {name} must be [R, ceil(C/gs)]")
+    _same_device(dev, packed, scales)
+    if scales.dtype != torch.float32 or not scales.is_contiguous():
+        scales = scales.to(torch.float32).contiguous()
+    return packed, scales, R, C
+
+
+def _half_type(t, name):
+    _require(t.dtype in (torch.bfloat16, torch.float16), f"{name} must be bfloat16 or float16, got {t.dtype}")
+    return _ACT_DTYPES[t.dtype]
+
+
+def int4_linear(x, packed, scales, gs: int = 128, bias=None, act: str = "none", residual=None, want_preact: bool = False,
+                status=None):
+    """y = act(x W^T + bias) + residual over a pack-quantized int4 matrix (forge_int4_linear): packed int32 [R, C/8] as
+    pack_int4 writes it for symmetric codes, scales [R, ceil(C/gs)], W = (nibble - 8) * scale.  x [T, C] bf16 or fp16;
+    bias [R] and residual [T, R] of x's type; act "none", "relu", "silu" or "gelu" (erf form).  Returns y [T, R], or
+    (y, z) with want_preact: z = x W^T + bias rounded to x's type, for int4_linear_backward."""
+    _abi._require_cuda()
+    _require(x.is_cuda, "x must be a CUDA tensor")
+    if x.device.index != torch.cuda.current_device():
+        with torch.cuda.device(x.device):
+            return int4_linear(x, packed, scales, gs, bias, act, residual, want_preact, status)
+    packed, scales, R, C = _int4_weight(packed, scales, gs, x.device, "packed")
+    _require(x.dim() == 2 and x.shape[1] == C, f"x must be [T, {C}], got {list(x.shape)}")
+    code = _half_type(x, "x")
+    _require(act in _abi.ACTS, f"unknown activation {act!r}")
+    _same_device(x.device, bias, residual, status)
+    T = x.shape[0]
+    x, ldx = _rows(x, True)
+    if bias is not None:
+        _require(tuple(bias.shape) == (R,) and bias.dtype == x.dtype, "bias must be [R], of x's type")
+        bias = bias.contiguous()
+    ldres = 0
+    if residual is not None:
+        _check_rows(residual, "residual", (T, R), x.dtype)
+        residual, ldres = _rows(residual, False)
+    y = torch.empty((T, R), dtype=x.dtype, device=x.device)
+    z = torch.empty_like(y) if want_preact else None
+    call("forge_int4_linear", x.data_ptr(), ldx, code, packed.data_ptr(), scales.data_ptr(), gs, T, C, R, ptr(bias),
+         _abi.ACTS[act], None if residual is None else residual.data_ptr(), ldres, y.data_ptr(), ptr(z), ptr(status),
+         stream_ptr())
+    return (y, z) if want_preact else y
+
+
+def int4_linear_backward(dy, packed, scales, gs: int = 128, preact=None, act: str = "none", want_dx: bool = True,
+                         want_dbias: bool = False, status=None):
+    """Gradients of int4_linear for frozen weights: dz = dy * act'(preact); returns (dx, dbias), dx = dz W [T, C] and
+    dbias = the column sums of dz [R], both of dy's type, None where not wanted.  preact is the z of the forward call
+    (not needed with act="none"); the residual's gradient is dy itself (forge_int4_linear_backward)."""
+    _abi._require_cuda()
+    _require(dy.is_cuda, "dy must be a CUDA tensor")
+    if dy.device.index != torch.cuda.current_device():
+        with torch.cuda.device(dy.device):
+            return int4_linear_backward(dy, packed, scales, gs, preact, act, want_dx, want_dbias, status)
+    packed, scales, R, C = _int4_weight(packed, scales, gs, dy.device, "packed")
+    _require(want_dx or want_dbias, "nothing to compute")
+    _require(dy.dim() == 2 and dy.shape[1] == R, f"dy must be [T, {R}], got {list(dy.shape)}")
+    code = _half_type(dy, "dy")
+    _require(act in _abi.ACTS, f"unknown activation {act!r}")
+    T = dy.shape[0]
+    if act == "none":
+        preact = None
+    else:
+        _require(preact is not None, "preact is needed for the gradient of an activation")
+        _check_rows(preact, "preact", (T, R), dy.dtype)
+        preact = preact.contiguous()
+    _same_device(dy.device, preact, status)
+    dy, lddy = _rows(dy, False)
+    dx = torch.empty((T, C), dtype=dy.dtype, device=dy.device) if want_dx else None
+    db = torch.empty((R,), dtype=dy.dtype, device=dy.device) if want_dbias else None
+    ws = torch.empty(query("forge_int4_backward_workspace_bytes", T, C, R, gs, 1), dtype=torch.uint8, device=dy.device)
+    call("forge_int4_linear_backward", dy.data_ptr(), lddy, code, packed.data_ptr(), scales.data_ptr(), gs, T, C, R,
+         ptr(preact), _abi.ACTS[act], ptr(dx), ptr(db), ptr(ws), ptr(status), stream_ptr())
+    return dx, db
+
+
+def int4_gated(x, gate_packed, gate_scales, up_packed, up_scales, gs: int = 128, act: str = "silu",
+               want_preact: bool = False, status=None):
+    """h = act(x Wg^T) * (x Wu^T) over two pack-quantized int4 matrices of one shape (see int4_linear), both projections,
+    the activation and the product in one kernel (forge_int4_gated).  Returns h [T, R], or (h, g, u) with want_preact: the
+    two projections rounded to x's type, for int4_gated_backward."""
+    _abi._require_cuda()
+    _require(x.is_cuda, "x must be a CUDA tensor")
+    if x.device.index != torch.cuda.current_device():
+        with torch.cuda.device(x.device):
+            return int4_gated(x, gate_packed, gate_scales, up_packed, up_scales, gs, act, want_preact, status)
+    gate_packed, gate_scales, R, C = _int4_weight(gate_packed, gate_scales, gs, x.device, "gate_packed")
+    up_packed, up_scales, R2, C2 = _int4_weight(up_packed, up_scales, gs, x.device, "up_packed")
+    _require((R, C) == (R2, C2), "gate and up must have one shape")
+    _require(x.dim() == 2 and x.shape[1] == C, f"x must be [T, {C}], got {list(x.shape)}")
+    code = _half_type(x, "x")
+    _require(act in _abi.ACTS, f"unknown activation {act!r}")
+    _same_device(x.device, status)
+    T = x.shape[0]
+    x, ldx = _rows(x, True)
+    h = torch.empty((T, R), dtype=x.dtype, device=x.device)
+    g, u = (torch.empty_like(h), torch.empty_like(h)) if want_preact else (None, None)
+    call("forge_int4_gated", x.data_ptr(), ldx, code, gate_packed.data_ptr(), gate_scales.data_ptr(), up_packed.data_ptr(),
+         up_scales.data_ptr(), gs, T, C, R, _abi.ACTS[act], h.data_ptr(), ptr(g), ptr(u), ptr(status), stream_ptr())
+    return (h, g, u) if want_preact else h
+
+
+def int4_gated_backward(dh, g, u, gate_packed, gate_scales, up_packed, up_scales, gs: int = 128, act: str = "silu",
+                        status=None):
+    """Gradient of int4_gated for frozen weights, at the g and u of the forward call:
+    dx = (dh * u * act'(g)) Wg + (dh * act(g)) Wu, [T, C] of dh's type (forge_int4_gated_backward)."""
+    _abi._require_cuda()
+    _require(dh.is_cuda, "dh must be a CUDA tensor")
+    if dh.device.index != torch.cuda.current_device():
+        with torch.cuda.device(dh.device):
+            return int4_gated_backward(dh, g, u, gate_packed, gate_scales, up_packed, up_scales, gs, act, status)
+    gate_packed, gate_scales, R, C = _int4_weight(gate_packed, gate_scales, gs, dh.device, "gate_packed")
+    up_packed, up_scales, R2, C2 = _int4_weight(up_packed, up_scales, gs, dh.device, "up_packed")
+    _require((R, C) == (R2, C2), "gate and up must have one shape")
+    _require(dh.dim() == 2 and dh.shape[1] == R, f"dh must be [T, {R}], got {list(dh.shape)}")
+    code = _half_type(dh, "dh")
+    _require(act in _abi.ACTS, f"unknown activation {act!r}")
+    T = dh.shape[0]
+    _check_rows(g, "g", (T, R), dh.dtype)
+    _check_rows(u, "u", (T, R), dh.dtype)
+    _same_device(dh.device, g, u, status)
+    dh, lddh = _rows(dh, False)
+    dx = torch.empty((T, C), dtype=dh.dtype, device=dh.device)
+    ws = torch.empty(query("forge_int4_backward_workspace_bytes", T, C, R, gs, 2), dtype=torch.uint8, device=dh.device)
+    call("forge_int4_gated_backward", dh.data_ptr(), lddh, code, ptr(g.contiguous()), ptr(u.contiguous()),
+         gate_packed.data_ptr(), gate_scales.data_ptr(), up_packed.data_ptr(), up_scales.data_ptr(), gs, T, C, R,
+         _abi.ACTS[act], ptr(dx), ptr(ws), ptr(status), stream_ptr())
+    return dx

@@ -33,7 +33,7 @@ enum {
     FORGE_ERR_UNSUPPORTED = 4  /* shape / option outside what the kernels cover */
 };
 
-enum { FORGE_DTYPE_F32 = 0, FORGE_DTYPE_BF16 = 1 };
+enum { FORGE_DTYPE_F32 = 0, FORGE_DTYPE_BF16 = 1, FORGE_DTYPE_F16 = 2 /* norm and int4 products only */ };
 
 /* flags of forge_hessian_grouped */
 enum {
@@ -44,6 +44,9 @@ enum {
 enum { FORGE_FWD_SIMT = 1 }; /* plain-FMA validation kernel instead of tcgen05 */
 /* selection rule of forge_route_topk */
 enum { FORGE_ROUTE_SOFTMAX = 0, FORGE_ROUTE_SIGMOID = 1, FORGE_ROUTE_SIGMOID_GROUPED = 2 };
+
+/* activation of the int4 products: z, max(z, 0), z / (1 + exp(-z)), z (1 + erf(z / sqrt 2)) / 2 */
+enum { FORGE_ACT_NONE = 0, FORGE_ACT_RELU = 1, FORGE_ACT_SILU = 2, FORGE_ACT_GELU = 3 };
 
 int forge_version(void);
 const char *forge_last_error(void);
@@ -325,6 +328,57 @@ int forge_sparse14_moe_w13_swiglu(const uint64_t *w13, const void *X_bf16, int64
 int forge_sparse14_moe_w2(const uint64_t *w2, const void *X2_bf16, int64_t ldx, int64_t x_rows, const int32_t *token_idx,
                           const int64_t *offsets, const int32_t *active, int n_active, int64_t N, int64_t R, int64_t C,
                           void *Y_bf16, void *stream);
+
+/* ---- root-mean-square norm -------------------------------------------------------
+ * For each of T rows of C channels, in fp32 and rounded once per output:
+ *   h = x (+ residual);   y = h / sqrt(mean(h^2) + eps) * weight;   residual_out = h   (with residual only)
+ * x, residual, residual_out and y have the type `dtype` (fp32, bf16, fp16); weight [C] that type or fp32.  With scales
+ * given, y is e4m3 bytes and, per 128 consecutive channels of a row (the last group may be shorter),
+ *   scales[t, g] = max(max |y|, 1e-12) / 448,   y8 = e4m3(y / scales[t, g]):
+ * scales [T, ceil(C/128)] fp32, the layout that forge_fp8_block_dequant reads when C is a multiple of 128.  Row strides ldx, ldres in elements;
+ * y, scales and residual_out are dense and alias no input.  Any C, stride and alignment (16-byte aligned rows of a
+ * multiple of 8 channels up to 16384 are read once, others twice). */
+int forge_rmsnorm(const void *x, int64_t ldx, const void *residual, int64_t ldres, const void *weight, int w_dtype,
+                  int dtype, int64_t T, int64_t C, float eps, void *y, float *scales, void *residual_out, void *stream);
+/* Gradients at the normed rows x (the residual_out of the forward call where there was a residual):
+ *   n = x / sqrt(mean(x^2) + eps),  t = dy * weight,  dx = (t - n * mean(t n)) / sqrt(mean(x^2) + eps) (+ dresidual),
+ *   dweight = sum over rows of dy * n.
+ * dx [T, C] dense, of x's type: the gradient of x and of the residual alike.  dweight [C] of the weight's type, summed in
+ * fp32 in an order that does not depend on scheduling; zeros when T = 0.
+ * ws: forge_rmsnorm_backward_workspace_bytes(T, C), 16-byte aligned. */
+int64_t forge_rmsnorm_backward_workspace_bytes(int64_t T, int64_t C);
+int forge_rmsnorm_backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, const void *weight, int w_dtype,
+                           int dtype, const void *dresidual, int64_t lddres, int64_t T, int64_t C, float eps, void *dx,
+                           void *dweight, void *ws, void *stream);
+
+/* ---- products with packed int4 weights ------------------------------------------------
+ * W[r, c] = (nibble(r, c) - 8) * scales[r, c / gs], nibbles as forge_pack_int4 writes them for symmetric codes:
+ * packed [R, C/8] int32, dense; scales [R, ceil(C/gs)] fp32.  gs 32, 64 or 128; C a multiple of 8.  x bf16 or fp16
+ * (`dtype`), rows 16-byte aligned: ldx a multiple of 8.  Sums in fp32, one rounding per output.
+ *   forge_int4_linear:  z = x W^T (+ bias),  y = act(z) (+ residual);  bias [R], residual [T, ldres], y [T, R] of x's type
+ *   forge_int4_gated:   g = x Wg^T, u = x Wu^T,  h = act(g) * u;  h [T, R]
+ * preact (g and u) may be NULL; given, they receive z (g and u) rounded to x's type, for the backward pass.
+ * `status` (device int32, may be NULL) receives FORGE_ERR_TIMEOUT if a bounded device-side wait ran out. */
+int forge_int4_linear(const void *x, int64_t ldx, int dtype, const int32_t *packed, const float *scales, int gs, int64_t T,
+                      int64_t C, int64_t R, const void *bias, int act, const void *residual, int64_t ldres, void *y,
+                      void *preact, int32_t *status, void *stream);
+int forge_int4_gated(const void *x, int64_t ldx, int dtype, const int32_t *gate_packed, const float *gate_scales,
+                     const int32_t *up_packed, const float *up_scales, int gs, int64_t T, int64_t C, int64_t R, int act,
+                     void *h, void *g, void *u, int32_t *status, void *stream);
+/* Backward for frozen weights, at the pre-activations that the forward call saved:
+ *   linear:  dz = dy * act'(preact),  dx = dz W (NULL: not wanted),  dbias = sum over rows of dz (NULL: not wanted)
+ *   gated:   dx = (dh * u * act'(g)) Wg + (dh * act(g)) Wu
+ * dx [T, C] and dbias [R] of x's type, dense; preact may be NULL when act is FORGE_ACT_NONE.  dz enters its product as
+ * fp16 with a power of two per row, the weights as fp16 with a power of two per weight row.  The order of every sum is
+ * fixed.  ws: forge_int4_backward_workspace_bytes(T, C, R, gs, mats) bytes (mats 1 linear, 2 gated), 256-byte aligned. */
+int64_t forge_int4_backward_workspace_bytes(int64_t T, int64_t C, int64_t R, int gs, int mats);
+int forge_int4_linear_backward(const void *dy, int64_t lddy, int dtype, const int32_t *packed, const float *scales, int gs,
+                               int64_t T, int64_t C, int64_t R, const void *preact, int act, void *dx, void *dbias, void *ws,
+                               int32_t *status, void *stream);
+int forge_int4_gated_backward(const void *dh, int64_t lddh, int dtype, const void *g, const void *u,
+                              const int32_t *gate_packed, const float *gate_scales, const int32_t *up_packed,
+                              const float *up_scales, int gs, int64_t T, int64_t C, int64_t R, int act, void *dx, void *ws,
+                              int32_t *status, void *stream);
 
 #ifdef __cplusplus
 }
