@@ -1,4 +1,4 @@
-// Products with packed int4 weights (the layout of forge_pack_int4, symmetric codes):
+// Entry points and the elementwise part of the products with packed int4 weights (the layout of forge_pack_int4, symmetric codes):
 //   W[r, c] = (nibble(r, c) - 8) * scale[r, c / gs]
 //   linear:  y = act(x W^T + bias) + residual            gated:  h = act(x Wg^T) * (x Wu^T)
 // and their backward passes for frozen weights:
@@ -121,95 +121,6 @@ __global__ void __launch_bounds__(256) dbias_sum_kernel(const float *__restrict_
     out[r] = Elem<T>::from_f(s);
 }
 
-// ---- products on the FMA pipe: 64 x 64 output tile, 16-deep k-tiles ----------------------------------------------------
-__device__ __forceinline__ float nibble(const uint32_t *packed, int64_t r, int64_t c, int64_t CP) {
-    return (float)(int)((packed[r * CP + (c >> 3)] >> (4 * (int)(c & 7))) & 15u) - 8.0f;
-}
-
-template <typename T, bool GATED> __global__ void __launch_bounds__(256) fwd_fma_kernel(const Int4Fwd P) {
-    constexpr int M = GATED ? 2 : 1;
-    __shared__ float xs[16][65], ws[M][16][65];
-    const int64_t m0 = (int64_t)blockIdx.y * 64, n0 = (int64_t)blockIdx.x * 64;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int64_t CP = P.C / 8;
-    float acc[M][4][4] = {};
-    for (int64_t k0 = 0; k0 < P.C; k0 += 16) {
-        for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-            const int k = i & 15, r = i >> 4;
-            const int64_t kk = k0 + k;
-            xs[k][r] = (m0 + r < P.T && kk < P.C) ? Elem<T>::to_f(((const T *)P.x)[(m0 + r) * P.ldx + kk]) : 0.0f;
-#pragma unroll
-            for (int m = 0; m < M; ++m)
-                ws[m][k][r] = (n0 + r < P.R && kk < P.C)
-                                  ? nibble(P.packed[m], n0 + r, kk, CP) * P.scales[m][(n0 + r) * P.G + kk / P.gs] : 0.0f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 16; ++k)
-#pragma unroll
-            for (int m = 0; m < M; ++m)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        acc[m][i][j] = fmaf(xs[k][ty * 4 + i], ws[m][k][tx * 4 + j], acc[m][i][j]);
-        __syncthreads();
-    }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int64_t t = m0 + ty * 4 + i, r = n0 + tx * 4 + j;
-            if (t >= P.T || r >= P.R) continue;
-            float z = acc[0][i][j];
-            if (!GATED && P.bias) z += Elem<T>::to_f(((const T *)P.bias)[r]);
-            if (P.pre0) ((T *)P.pre0)[t * P.R + r] = Elem<T>::from_f(z);
-            float y = act_fwd_rt(P.act, z);
-            if constexpr (GATED) {
-                if (P.pre1) ((T *)P.pre1)[t * P.R + r] = Elem<T>::from_f(acc[M - 1][i][j]);
-                y *= acc[M - 1][i][j];
-            } else if (P.res) {
-                y += Elem<T>::to_f(((const T *)P.res)[t * P.ldres + r]);
-            }
-            ((T *)P.y)[t * P.R + r] = Elem<T>::from_f(y);
-        }
-}
-
-template <typename T> __global__ void __launch_bounds__(256) dgrad_fma_kernel(const Int4Dgrad P) {
-    __shared__ float as[16][65], ws[16][65];
-    const int64_t m0 = (int64_t)blockIdx.y * 64, n0 = (int64_t)blockIdx.x * 64;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int64_t CP = P.C / 8, K = P.mats * P.R;
-    float acc[4][4] = {};
-    for (int64_t k0 = 0; k0 < K; k0 += 16) {
-        for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-            const int k = i >> 6, c = i & 63;
-            const int64_t kk = k0 + k, col = n0 + c;
-            float w = 0.0f;
-            if (kk < K && col < P.C) {
-                const int m = kk >= P.R;
-                const __half2 s = P.pairs[kk * P.G + col / P.gs];
-                w = __half2float(__float2half_rn(nibble(P.packed[m], kk - m * P.R, col, CP) *
-                                                 (__half2float(__low2half(s)) + __half2float(__high2half(s)))));
-            }
-            ws[k][c] = w;
-            as[i & 15][i >> 4] = (m0 + (i >> 4) < P.T && k0 + (i & 15) < K)
-                                     ? __half2float(P.a[(m0 + (i >> 4)) * P.ldk + k0 + (i & 15)]) : 0.0f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 16; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(as[k][ty * 4 + i], ws[k][tx * 4 + j], acc[i][j]);
-        __syncthreads();
-    }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int64_t t = m0 + ty * 4 + i, c = n0 + tx * 4 + j;
-            if (t < P.T && c < P.C) ((T *)P.dx)[t * P.C + c] = Elem<T>::from_f(acc[i][j] * P.unscale[t]);
-        }
-}
-
 // ---- host side -------------------------------------------------------------------------------------------------------
 constexpr int64_t kMaxDim = 1ll << 24;        // rows and columns of a weight matrix
 constexpr int64_t kMaxTokens = 0x7fffffffLL;
@@ -271,34 +182,12 @@ template <typename T> void launch_dbias(const void *dy, int64_t lddy, const void
     dbias_sum_kernel<T><<<(unsigned)cdiv(R, (int64_t)256), 256, 0, st>>>(partial, parts, R, (T *)out); FORGE_NOTE_LAUNCH();
 }
 
-template <typename T, bool GATED> int run_fwd(const Int4Fwd &P, cudaStream_t st) {
-    const int64_t max_rows = 65535 * 64ll;
-    for (int64_t t0 = 0; t0 < P.T; t0 += max_rows) {
-        Int4Fwd Q = P;
-        Q.T = imin64(P.T - t0, max_rows);
-        Q.x = (const T *)P.x + t0 * P.ldx;
-        if (P.res) Q.res = (const T *)P.res + t0 * P.ldres;
-        Q.y = (T *)P.y + t0 * P.R;
-        if (P.pre0) Q.pre0 = (T *)P.pre0 + t0 * P.R;
-        if (P.pre1) Q.pre1 = (T *)P.pre1 + t0 * P.R;
-        fwd_fma_kernel<T, GATED><<<dim3((unsigned)cdiv(P.R, (int64_t)64), (unsigned)cdiv(Q.T, (int64_t)64)), 256, 0, st>>>(Q);
-        FORGE_NOTE_LAUNCH();
-    }
-    return check_launch(GATED ? "forge_int4_gated" : "forge_int4_linear");
-}
-
-template <typename T> int run_dgrad(const Int4Dgrad &P, const char *who, cudaStream_t st) {
-    const int64_t max_rows = 65535 * 64ll;
-    for (int64_t t0 = 0; t0 < P.T; t0 += max_rows) {
-        Int4Dgrad Q = P;
-        Q.T = imin64(P.T - t0, max_rows);
-        Q.a = P.a + t0 * P.ldk;
-        Q.unscale = P.unscale + t0;
-        Q.dx = (T *)P.dx + t0 * P.C;
-        dgrad_fma_kernel<T><<<dim3((unsigned)cdiv(P.C, (int64_t)64), (unsigned)cdiv(Q.T, (int64_t)64)), 256, 0, st>>>(Q);
-        FORGE_NOTE_LAUNCH();
-    }
-    return check_launch(who);
+int run_fwd(Int4Fwd &P, int dtype, bool gated, cudaStream_t st) {
+    const uintptr_t a = (uintptr_t)P.packed[0] | (uintptr_t)P.packed[1];
+    P.vec8 = P.C % 16 == 0 && a % 8 == 0;
+    P.vec16 = P.C % 32 == 0 && a % 16 == 0;
+    const bool bf16 = dtype == FORGE_DTYPE_BF16;
+    return P.T <= kDecodeTokens ? int4_decode(P, bf16, gated, st) : int4_fwd_tc(P, bf16, gated, st);
 }
 
 }  // namespace
@@ -313,9 +202,8 @@ extern "C" int forge_int4_linear(const void *x, int64_t ldx, int dtype, const in
     FORGE_REQUIRE(!residual || T == 1 || ldres >= R, "residual row stride below R");
     FORGE_REQUIRE((uintptr_t)y % 16 == 0 && (uintptr_t)preact % 16 == 0, "outputs must be 16-byte aligned");
     Int4Fwd P{x, ldx, {(const uint32_t *)packed, nullptr}, {scales, nullptr}, gs, T, C, R, cdiv(C, (int64_t)gs), bias, act,
-              residual, ldres, y, preact, nullptr, status};
-    cudaStream_t st = (cudaStream_t)stream;
-    return dtype == FORGE_DTYPE_BF16 ? run_fwd<__nv_bfloat16, false>(P, st) : run_fwd<__half, false>(P, st);
+              residual, ldres, y, preact, nullptr, status, false, false};
+    return run_fwd(P, dtype, false, (cudaStream_t)stream);
 }
 
 extern "C" int forge_int4_gated(const void *x, int64_t ldx, int dtype, const int32_t *gate_packed, const float *gate_scales,
@@ -328,9 +216,8 @@ extern "C" int forge_int4_gated(const void *x, int64_t ldx, int dtype, const int
     FORGE_REQUIRE(rows_ok(x, ldx, C, T), "x must be 16-byte aligned with a row stride >= C that is a multiple of 8");
     FORGE_REQUIRE((uintptr_t)h % 16 == 0 && (uintptr_t)g % 16 == 0 && (uintptr_t)u % 16 == 0, "outputs must be 16-byte aligned");
     Int4Fwd P{x, ldx, {(const uint32_t *)gate_packed, (const uint32_t *)up_packed}, {gate_scales, up_scales}, gs, T, C, R,
-              cdiv(C, (int64_t)gs), nullptr, act, nullptr, 0, h, g, u, status};
-    cudaStream_t st = (cudaStream_t)stream;
-    return dtype == FORGE_DTYPE_BF16 ? run_fwd<__nv_bfloat16, true>(P, st) : run_fwd<__half, true>(P, st);
+              cdiv(C, (int64_t)gs), nullptr, act, nullptr, 0, h, g, u, status, false, false};
+    return run_fwd(P, dtype, true, (cudaStream_t)stream);
 }
 
 extern "C" int64_t forge_int4_backward_workspace_bytes(int64_t T, int64_t C, int64_t R, int gs, int mats) {
@@ -365,7 +252,7 @@ static int backward(const char *who, const void *dy, int64_t lddy, int dtype, co
     }
     Int4Dgrad P{(const __half *)(base + L.a), L.ldk, (const float *)(base + L.unscale),
                 {(const uint32_t *)p0, (const uint32_t *)p1}, (const __half2 *)(base + L.pairs), gs, mats, T, C, R, G, dx, status};
-    return dtype == FORGE_DTYPE_BF16 ? run_dgrad<__nv_bfloat16>(P, who, st) : run_dgrad<__half>(P, who, st);
+    return int4_dgrad_tc(P, dtype == FORGE_DTYPE_BF16, who, st);
 }
 
 extern "C" int forge_int4_linear_backward(const void *dy, int64_t lddy, int dtype, const int32_t *packed, const float *scales,

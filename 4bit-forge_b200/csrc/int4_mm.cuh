@@ -1,6 +1,7 @@
 // Arguments of the int4 product kernels, shared by their translation units.
 #pragma once
 #include <cuda_fp16.h>
+#include <cuda_runtime.h>
 #include <stdint.h>
 
 namespace forge {
@@ -19,6 +20,7 @@ struct Int4Fwd {
     void *y;                     // [T, R]
     void *pre0, *pre1;           // pre-activations [T, R] or NULL (pre1: gated form)
     int32_t *status;
+    bool vec8, vec16;            // rows of packed words start on 8 (16) bytes
 };
 
 struct Int4Dgrad {
@@ -32,5 +34,11 @@ struct Int4Dgrad {
     void *dx;                    // [T, C]
     int32_t *status;
 };
+
+constexpr int kDecodeTokens = 32;      // most tokens that int4_decode takes
+// more tokens than int4_decode takes; the backward product
+int int4_fwd_tc(const Int4Fwd &P, bool bf16, bool gated, cudaStream_t st);
+int int4_dgrad_tc(const Int4Dgrad &P, bool bf16, const char *who, cudaStream_t st);
+int int4_decode(const Int4Fwd &P, bool bf16, bool gated, cudaStream_t st);
 
 }  // namespace forge

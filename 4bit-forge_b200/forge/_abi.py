@@ -107,9 +107,15 @@ def load_library():
     return _lib
 
 
+_cuda_ok = False
+
+
 def _require_cuda():
-    if not torch.cuda.is_available():
-        raise RuntimeError("forge_b200 CUDA kernels are unavailable because torch.cuda.is_available() is False")
+    global _cuda_ok
+    if not _cuda_ok:         # once true it stays true: the query costs most of a microsecond, a call makes several
+        if not torch.cuda.is_available():
+            raise RuntimeError("forge_b200 CUDA kernels are unavailable because torch.cuda.is_available() is False")
+        _cuda_ok = True
 
 
 def ptr(t):
@@ -121,7 +127,13 @@ def ptr(t):
     return t.data_ptr()
 
 
+# the stream handle without building a torch.cuda.Stream object (3 us of the host's time a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_ptr():
+    if _raw_stream is not None:
+        return _raw_stream(torch.cuda.current_device())
     return torch.cuda.current_stream().cuda_stream
 
 
@@ -136,7 +148,7 @@ def dtype_code(t: torch.Tensor) -> int:
 def call(name: str, *args):
     """Invoke an entry point; a non-zero return raises RuntimeError with the library's message."""
     _require_cuda()
-    lib = load_library()
+    lib = _lib or load_library()
     rc = getattr(lib, name)(*args)
     if rc != 0:
         msg = lib.forge_last_error().decode("utf-8", "replace")
@@ -145,4 +157,4 @@ def call(name: str, *args):
 
 
 def query(name: str, *args) -> int:
-    return int(getattr(load_library(), name)(*args))
+    return int(getattr(_lib or load_library(), name)(*args))

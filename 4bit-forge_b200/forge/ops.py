@@ -361,35 +361,56 @@ def mma_issue_cycles(N: int = 128, iters: int = 2000, pattern: bool = True) -> f
 # ---- the feed-forward block on packed int4 weights -----------------------------------------------------------------
 # Activations are 2-D [tokens, channels].  A row-strided view is read in place (16-byte aligned rows for the products);
 # anything else is copied once.  Outputs are dense.  Every call works on the device of its first argument, on that
-# device's current stream.
+# device's current stream.  A decode step makes many of these calls, each a few microseconds long on the device, so the
+# checks are written to cost the host little (no message is built unless it is raised).
 
 _ACT_DTYPES = {torch.float32: _abi.F32, torch.bfloat16: _abi.BF16, torch.float16: _abi.F16}
+_HALF_DTYPES = {torch.bfloat16: _abi.BF16, torch.float16: _abi.F16}
 
 
-def _require(cond, msg):
-    if not cond:
-        raise RuntimeError(f"forge_b200: {msg}")
+def _fail(msg):
+    raise RuntimeError(f"forge_b200: {msg}")
 
 
-def _same_device(dev, *tensors):
-    for t in tensors:
-        _require(t is None or t.device == dev, "all tensors must be on the device of the first argument")
+def _on_device(t, name):
+    """True when t lives on the current device; raises when it is not a CUDA tensor."""
+    _abi._require_cuda()
+    if not t.is_cuda:
+        _fail(f"{name} must be a CUDA tensor (there is no CPU path)")
+    return t.get_device() == torch.cuda.current_device()
 
 
-def _rows(t, aligned: bool):
-    """(tensor, row stride) of a 2-D tensor whose rows are contiguous; aligned: every row starts on 16 bytes."""
-    T, C = t.shape
-    ld = t.stride(0) if T > 1 else C
-    if (t.stride(1) != 1 and C > 1) or ld < C or (aligned and (ld % 8 or t.data_ptr() % 16)):
+def _rows(t, T, C, aligned: bool):
+    """(tensor, row stride) of a [T, C] tensor whose rows are contiguous; aligned: every row starts on 16 bytes."""
+    ld, sc = t.stride()
+    if T <= 1:
+        ld = C
+    if (sc != 1 and C > 1) or ld < C or (aligned and (ld & 7 or t.data_ptr() & 15)):
         t = t.clone(memory_format=torch.contiguous_format)
         ld = C
     return t, ld
 
 
-def _check_rows(t, name, shape=None, dtype=None):
-    _require(t.dim() == 2 and (shape is None or tuple(t.shape) == shape), f"{name} must be 2-D" if shape is None else
-             f"{name} must have the shape {list(shape)}, got {list(t.shape)}")
-    _require(dtype is None or t.dtype == dtype, f"{name} must be {dtype}, got {t.dtype}")
+def _like(t, name, shape, dtype, dev):
+    """t is a tensor of this shape and type on this device."""
+    if t.shape != shape or t.dtype != dtype or t.get_device() != dev:
+        _fail(f"{name} must be {list(shape)} {dtype} on cuda:{dev}, got {list(t.shape)} {t.dtype} on {t.device}")
+
+
+def _dense(t, name, shape, dtype, dev):
+    _like(t, name, shape, dtype, dev)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _norm_args(x, weight):
+    if x.dim() != 2 or x.shape[1] == 0:
+        _fail(f"x must be [T, C], got {list(x.shape)}")
+    if x.dtype not in _ACT_DTYPES:
+        _fail(f"x must be float32, bfloat16 or float16, got {x.dtype}")
+    T, C = x.shape
+    wt = weight.dtype
+    weight = _dense(weight, "weight", (C,), torch.float32 if wt == torch.float32 else x.dtype, x.get_device())
+    return T, C, weight, _ACT_DTYPES[wt], _ACT_DTYPES[x.dtype]
 
 
 def rmsnorm(x, weight, eps: float = 1e-6, residual=None, quant_group: int = 0):
@@ -399,81 +420,83 @@ def rmsnorm(x, weight, eps: float = 1e-6, residual=None, quant_group: int = 0):
     Returns y, or (y, h) with a residual: h rounded to x's type is the new residual stream.  quant_group=128 returns the
     8-bit form instead of y: (q, scales) or (q, scales, h), q float8_e4m3fn [T, C], scales fp32 [T, ceil(C/128)], such that
     q * scales, group by group, is y: the layout fp8_block_dequant reads when C is a multiple of 128."""
-    _abi._require_cuda()
-    _require(x.is_cuda, "x must be a CUDA tensor")
-    if x.device.index != torch.cuda.current_device():
+    if not _on_device(x, "x"):
         with torch.cuda.device(x.device):
             return rmsnorm(x, weight, eps, residual, quant_group)
-    _check_rows(x, "x")
-    T, C = x.shape
-    _require(C > 0, "x has no channels")
-    _require(x.dtype in _ACT_DTYPES, f"x must be float32, bfloat16 or float16, got {x.dtype}")
-    _require(weight.shape == (C,) and weight.dtype in (x.dtype, torch.float32), "weight must be [C], of x's type or float32")
-    _require(quant_group in (0, 128), "quant_group must be 0 (no quantisation) or 128")
-    _same_device(x.device, weight, residual)
-    x, ldx = _rows(x, False)
-    ldres, h = 0, None
+    T, C, weight, wcode, code = _norm_args(x, weight)
+    if quant_group not in (0, 128):
+        _fail("quant_group must be 0 (no quantisation) or 128")
+    x, ldx = _rows(x, T, C, False)
+    h, pres, ldres, ph = None, None, 0, None
     if residual is not None:
-        _check_rows(residual, "residual", (T, C), x.dtype)
-        residual, ldres = _rows(residual, False)
-        h = torch.empty((T, C), dtype=x.dtype, device=x.device)
-    scales = torch.empty((T, (C + 127) // 128), dtype=torch.float32, device=x.device) if quant_group else None
-    y = torch.empty((T, C), dtype=torch.float8_e4m3fn if quant_group else x.dtype, device=x.device)
-    call("forge_rmsnorm", x.data_ptr(), ldx, None if residual is None else residual.data_ptr(), ldres,
-         ptr(weight.contiguous()), _ACT_DTYPES[weight.dtype], _ACT_DTYPES[x.dtype], T, C, float(eps), ptr(y), ptr(scales),
-         ptr(h), stream_ptr())
-    out = (y, scales) if quant_group else (y,)
-    if h is not None:
-        out += (h,)
-    return out[0] if len(out) == 1 else out
+        _like(residual, "residual", x.shape, x.dtype, x.get_device())
+        residual, ldres = _rows(residual, T, C, False)
+        h = torch.empty_like(x, memory_format=torch.contiguous_format)
+        pres, ph = residual.data_ptr(), h.data_ptr()
+    if quant_group:
+        y = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
+        scales = torch.empty((T, (C + 127) // 128), dtype=torch.float32, device=x.device)
+    else:
+        y, scales = torch.empty_like(x, memory_format=torch.contiguous_format), None
+    call("forge_rmsnorm", x.data_ptr(), ldx, pres, ldres, weight.data_ptr(), wcode, code, T, C, eps, y.data_ptr(),
+         None if scales is None else scales.data_ptr(), ph, stream_ptr())
+    if scales is None:
+        return y if h is None else (y, h)
+    return (y, scales) if h is None else (y, scales, h)
 
 
 def rmsnorm_backward(dy, x, weight, eps: float = 1e-6, dresidual=None):
     """Gradients of rmsnorm at the normed rows x (the h of the forward call when it had a residual): returns (dx, dweight),
     dx [T, C] of x's type with `dresidual` (the gradient that reaches h past the norm) added, dweight [C] of the weight's
     type (forge_rmsnorm_backward).  dx is the gradient of the forward call's x and of its residual alike."""
-    _abi._require_cuda()
-    _require(dy.is_cuda, "dy must be a CUDA tensor")
-    if dy.device.index != torch.cuda.current_device():
-        with torch.cuda.device(dy.device):
+    if not _on_device(x, "x"):
+        with torch.cuda.device(x.device):
             return rmsnorm_backward(dy, x, weight, eps, dresidual)
-    _check_rows(x, "x")
-    T, C = x.shape
-    _require(C > 0, "x has no channels")
-    _require(x.dtype in _ACT_DTYPES, f"x must be float32, bfloat16 or float16, got {x.dtype}")
-    _check_rows(dy, "dy", (T, C), x.dtype)
-    _require(weight.shape == (C,) and weight.dtype in (x.dtype, torch.float32), "weight must be [C], of x's type or float32")
-    _same_device(dy.device, x, weight, dresidual)
-    (dy, lddy), (x, ldx) = _rows(dy, False), _rows(x, False)
-    lddres = 0
+    T, C, weight, wcode, code = _norm_args(x, weight)
+    _like(dy, "dy", x.shape, x.dtype, x.get_device())
+    (dy, lddy), (x, ldx) = _rows(dy, T, C, False), _rows(x, T, C, False)
+    pres, ldres = None, 0
     if dresidual is not None:
-        _check_rows(dresidual, "dresidual", (T, C), x.dtype)
-        dresidual, lddres = _rows(dresidual, False)
-    dx = torch.empty((T, C), dtype=x.dtype, device=x.device)
-    dw = torch.empty((C,), dtype=weight.dtype, device=x.device)
+        _like(dresidual, "dresidual", x.shape, x.dtype, x.get_device())
+        dresidual, ldres = _rows(dresidual, T, C, False)
+        pres = dresidual.data_ptr()
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    dw = torch.empty_like(weight)
     ws = torch.empty(query("forge_rmsnorm_backward_workspace_bytes", T, C), dtype=torch.uint8, device=x.device)
-    call("forge_rmsnorm_backward", dy.data_ptr(), lddy, x.data_ptr(), ldx, ptr(weight.contiguous()),
-         _ACT_DTYPES[weight.dtype], _ACT_DTYPES[x.dtype], None if dresidual is None else dresidual.data_ptr(), lddres, T, C,
-         float(eps), ptr(dx), ptr(dw), ptr(ws), stream_ptr())
+    call("forge_rmsnorm_backward", dy.data_ptr(), lddy, x.data_ptr(), ldx, weight.data_ptr(), wcode, code, pres, ldres, T, C,
+         eps, dx.data_ptr(), dw.data_ptr(), ws.data_ptr(), stream_ptr())
     return dx, dw
 
 
 def _int4_weight(packed, scales, gs, dev, name):
     """Checks a pack-quantized matrix; returns (packed, scales fp32, R, C)."""
-    _require(gs in (32, 64, 128), "group size must be 32, 64 or 128")
-    _require(packed.dim() == 2 and packed.dtype == torch.int32 and packed.is_contiguous() and packed.numel() > 0,
-             f"{name} must be a contiguous int32 matrix [R, C/8]")
-    R, C = packed.shape[0], packed.shape[1] * 8
-    _require(tuple(scales.shape) == (R, (C + gs - 1) // gs), f"the scales of {name} must be [R, ceil(C/gs)]")
-    _same_device(dev, packed, scales)
+    if gs not in (32, 64, 128):
+        _fail("group size must be 32, 64 or 128")
+    if packed.dim() != 2 or packed.dtype != torch.int32 or not packed.is_contiguous() or packed.get_device() != dev:
+        _fail(f"{name} must be a contiguous int32 matrix [R, C/8] on cuda:{dev}")
+    R, C = packed.shape
+    C *= 8
+    if scales.shape != (R, (C + gs - 1) // gs) or scales.get_device() != dev:
+        _fail(f"the scales of {name} must be [R, ceil(C/gs)] = {[R, (C + gs - 1) // gs]} on cuda:{dev}, got "
+              f"{list(scales.shape)} on {scales.device}")
     if scales.dtype != torch.float32 or not scales.is_contiguous():
         scales = scales.to(torch.float32).contiguous()
     return packed, scales, R, C
 
 
-def _half_type(t, name):
-    _require(t.dtype in (torch.bfloat16, torch.float16), f"{name} must be bfloat16 or float16, got {t.dtype}")
-    return _ACT_DTYPES[t.dtype]
+def _product_args(t, name, cols, act, status):
+    """Checks the 16-bit operand [T, cols] of a product; returns (T, type code, activation code, status pointer)."""
+    if t.dim() != 2 or t.shape[1] != cols:
+        _fail(f"{name} must be [T, {cols}], got {list(t.shape)}")
+    code, ac = _HALF_DTYPES.get(t.dtype), _abi.ACTS.get(act)
+    if code is None:
+        _fail(f"{name} must be bfloat16 or float16, got {t.dtype}")
+    if ac is None:
+        _fail(f"unknown activation {act!r} (one of {', '.join(_abi.ACTS)})")
+    if status is not None:
+        _like(status, "status", (1,), torch.int32, t.get_device())
+        return t.shape[0], code, ac, status.data_ptr()
+    return t.shape[0], code, ac, None
 
 
 def int4_linear(x, packed, scales, gs: int = 128, bias=None, act: str = "none", residual=None, want_preact: bool = False,
@@ -482,31 +505,26 @@ def int4_linear(x, packed, scales, gs: int = 128, bias=None, act: str = "none", 
     pack_int4 writes it for symmetric codes, scales [R, ceil(C/gs)], W = (nibble - 8) * scale.  x [T, C] bf16 or fp16;
     bias [R] and residual [T, R] of x's type; act "none", "relu", "silu" or "gelu" (erf form).  Returns y [T, R], or
     (y, z) with want_preact: z = x W^T + bias rounded to x's type, for int4_linear_backward."""
-    _abi._require_cuda()
-    _require(x.is_cuda, "x must be a CUDA tensor")
-    if x.device.index != torch.cuda.current_device():
+    if not _on_device(x, "x"):
         with torch.cuda.device(x.device):
             return int4_linear(x, packed, scales, gs, bias, act, residual, want_preact, status)
-    packed, scales, R, C = _int4_weight(packed, scales, gs, x.device, "packed")
-    _require(x.dim() == 2 and x.shape[1] == C, f"x must be [T, {C}], got {list(x.shape)}")
-    code = _half_type(x, "x")
-    _require(act in _abi.ACTS, f"unknown activation {act!r}")
-    _same_device(x.device, bias, residual, status)
-    T = x.shape[0]
-    x, ldx = _rows(x, True)
+    dev = x.get_device()
+    packed, scales, R, C = _int4_weight(packed, scales, gs, dev, "packed")
+    T, code, ac, pst = _product_args(x, "x", C, act, status)
+    x, ldx = _rows(x, T, C, True)
+    pb, pres, ldres = None, None, 0
     if bias is not None:
-        _require(tuple(bias.shape) == (R,) and bias.dtype == x.dtype, "bias must be [R], of x's type")
-        bias = bias.contiguous()
-    ldres = 0
+        bias = _dense(bias, "bias", (R,), x.dtype, dev)
+        pb = bias.data_ptr()
     if residual is not None:
-        _check_rows(residual, "residual", (T, R), x.dtype)
-        residual, ldres = _rows(residual, False)
-    y = torch.empty((T, R), dtype=x.dtype, device=x.device)
+        _like(residual, "residual", (T, R), x.dtype, dev)
+        residual, ldres = _rows(residual, T, R, False)
+        pres = residual.data_ptr()
+    y = x.new_empty((T, R))
     z = torch.empty_like(y) if want_preact else None
-    call("forge_int4_linear", x.data_ptr(), ldx, code, packed.data_ptr(), scales.data_ptr(), gs, T, C, R, ptr(bias),
-         _abi.ACTS[act], None if residual is None else residual.data_ptr(), ldres, y.data_ptr(), ptr(z), ptr(status),
-         stream_ptr())
-    return (y, z) if want_preact else y
+    call("forge_int4_linear", x.data_ptr(), ldx, code, packed.data_ptr(), scales.data_ptr(), gs, T, C, R, pb, ac, pres, ldres,
+         y.data_ptr(), None if z is None else z.data_ptr(), pst, stream_ptr())
+    return y if z is None else (y, z)
 
 
 def int4_linear_backward(dy, packed, scales, gs: int = 128, preact=None, act: str = "none", want_dx: bool = True,
@@ -514,30 +532,26 @@ def int4_linear_backward(dy, packed, scales, gs: int = 128, preact=None, act: st
     """Gradients of int4_linear for frozen weights: dz = dy * act'(preact); returns (dx, dbias), dx = dz W [T, C] and
     dbias = the column sums of dz [R], both of dy's type, None where not wanted.  preact is the z of the forward call
     (not needed with act="none"); the residual's gradient is dy itself (forge_int4_linear_backward)."""
-    _abi._require_cuda()
-    _require(dy.is_cuda, "dy must be a CUDA tensor")
-    if dy.device.index != torch.cuda.current_device():
+    if not _on_device(dy, "dy"):
         with torch.cuda.device(dy.device):
             return int4_linear_backward(dy, packed, scales, gs, preact, act, want_dx, want_dbias, status)
-    packed, scales, R, C = _int4_weight(packed, scales, gs, dy.device, "packed")
-    _require(want_dx or want_dbias, "nothing to compute")
-    _require(dy.dim() == 2 and dy.shape[1] == R, f"dy must be [T, {R}], got {list(dy.shape)}")
-    code = _half_type(dy, "dy")
-    _require(act in _abi.ACTS, f"unknown activation {act!r}")
-    T = dy.shape[0]
-    if act == "none":
-        preact = None
-    else:
-        _require(preact is not None, "preact is needed for the gradient of an activation")
-        _check_rows(preact, "preact", (T, R), dy.dtype)
-        preact = preact.contiguous()
-    _same_device(dy.device, preact, status)
-    dy, lddy = _rows(dy, False)
-    dx = torch.empty((T, C), dtype=dy.dtype, device=dy.device) if want_dx else None
-    db = torch.empty((R,), dtype=dy.dtype, device=dy.device) if want_dbias else None
+    dev = dy.get_device()
+    packed, scales, R, C = _int4_weight(packed, scales, gs, dev, "packed")
+    T, code, ac, pst = _product_args(dy, "dy", R, act, status)
+    if not (want_dx or want_dbias):
+        _fail("nothing to compute")
+    pz = None
+    if act != "none":
+        if preact is None:
+            _fail("preact is needed for the gradient of an activation")
+        preact = _dense(preact, "preact", (T, R), dy.dtype, dev)
+        pz = preact.data_ptr()
+    dy, lddy = _rows(dy, T, R, False)
+    dx = dy.new_empty((T, C)) if want_dx else None
+    db = dy.new_empty((R,)) if want_dbias else None
     ws = torch.empty(query("forge_int4_backward_workspace_bytes", T, C, R, gs, 1), dtype=torch.uint8, device=dy.device)
-    call("forge_int4_linear_backward", dy.data_ptr(), lddy, code, packed.data_ptr(), scales.data_ptr(), gs, T, C, R,
-         ptr(preact), _abi.ACTS[act], ptr(dx), ptr(db), ptr(ws), ptr(status), stream_ptr())
+    call("forge_int4_linear_backward", dy.data_ptr(), lddy, code, packed.data_ptr(), scales.data_ptr(), gs, T, C, R, pz, ac,
+         None if dx is None else dx.data_ptr(), None if db is None else db.data_ptr(), ws.data_ptr(), pst, stream_ptr())
     return dx, db
 
 
@@ -546,24 +560,23 @@ def int4_gated(x, gate_packed, gate_scales, up_packed, up_scales, gs: int = 128,
     """h = act(x Wg^T) * (x Wu^T) over two pack-quantized int4 matrices of one shape (see int4_linear), both projections,
     the activation and the product in one kernel (forge_int4_gated).  Returns h [T, R], or (h, g, u) with want_preact: the
     two projections rounded to x's type, for int4_gated_backward."""
-    _abi._require_cuda()
-    _require(x.is_cuda, "x must be a CUDA tensor")
-    if x.device.index != torch.cuda.current_device():
+    if not _on_device(x, "x"):
         with torch.cuda.device(x.device):
             return int4_gated(x, gate_packed, gate_scales, up_packed, up_scales, gs, act, want_preact, status)
-    gate_packed, gate_scales, R, C = _int4_weight(gate_packed, gate_scales, gs, x.device, "gate_packed")
-    up_packed, up_scales, R2, C2 = _int4_weight(up_packed, up_scales, gs, x.device, "up_packed")
-    _require((R, C) == (R2, C2), "gate and up must have one shape")
-    _require(x.dim() == 2 and x.shape[1] == C, f"x must be [T, {C}], got {list(x.shape)}")
-    code = _half_type(x, "x")
-    _require(act in _abi.ACTS, f"unknown activation {act!r}")
-    _same_device(x.device, status)
-    T = x.shape[0]
-    x, ldx = _rows(x, True)
-    h = torch.empty((T, R), dtype=x.dtype, device=x.device)
-    g, u = (torch.empty_like(h), torch.empty_like(h)) if want_preact else (None, None)
+    dev = x.get_device()
+    gate_packed, gate_scales, R, C = _int4_weight(gate_packed, gate_scales, gs, dev, "gate_packed")
+    up_packed, up_scales, R2, C2 = _int4_weight(up_packed, up_scales, gs, dev, "up_packed")
+    if R != R2 or C != C2:
+        _fail("gate and up must have one shape")
+    T, code, ac, pst = _product_args(x, "x", C, act, status)
+    x, ldx = _rows(x, T, C, True)
+    h = x.new_empty((T, R))
+    g, u, pg, pu = None, None, None, None
+    if want_preact:
+        g, u = torch.empty_like(h), torch.empty_like(h)
+        pg, pu = g.data_ptr(), u.data_ptr()
     call("forge_int4_gated", x.data_ptr(), ldx, code, gate_packed.data_ptr(), gate_scales.data_ptr(), up_packed.data_ptr(),
-         up_scales.data_ptr(), gs, T, C, R, _abi.ACTS[act], h.data_ptr(), ptr(g), ptr(u), ptr(status), stream_ptr())
+         up_scales.data_ptr(), gs, T, C, R, ac, h.data_ptr(), pg, pu, pst, stream_ptr())
     return (h, g, u) if want_preact else h
 
 
@@ -571,25 +584,20 @@ def int4_gated_backward(dh, g, u, gate_packed, gate_scales, up_packed, up_scales
                         status=None):
     """Gradient of int4_gated for frozen weights, at the g and u of the forward call:
     dx = (dh * u * act'(g)) Wg + (dh * act(g)) Wu, [T, C] of dh's type (forge_int4_gated_backward)."""
-    _abi._require_cuda()
-    _require(dh.is_cuda, "dh must be a CUDA tensor")
-    if dh.device.index != torch.cuda.current_device():
+    if not _on_device(dh, "dh"):
         with torch.cuda.device(dh.device):
             return int4_gated_backward(dh, g, u, gate_packed, gate_scales, up_packed, up_scales, gs, act, status)
-    gate_packed, gate_scales, R, C = _int4_weight(gate_packed, gate_scales, gs, dh.device, "gate_packed")
-    up_packed, up_scales, R2, C2 = _int4_weight(up_packed, up_scales, gs, dh.device, "up_packed")
-    _require((R, C) == (R2, C2), "gate and up must have one shape")
-    _require(dh.dim() == 2 and dh.shape[1] == R, f"dh must be [T, {R}], got {list(dh.shape)}")
-    code = _half_type(dh, "dh")
-    _require(act in _abi.ACTS, f"unknown activation {act!r}")
-    T = dh.shape[0]
-    _check_rows(g, "g", (T, R), dh.dtype)
-    _check_rows(u, "u", (T, R), dh.dtype)
-    _same_device(dh.device, g, u, status)
-    dh, lddh = _rows(dh, False)
-    dx = torch.empty((T, C), dtype=dh.dtype, device=dh.device)
+    dev = dh.get_device()
+    gate_packed, gate_scales, R, C = _int4_weight(gate_packed, gate_scales, gs, dev, "gate_packed")
+    up_packed, up_scales, R2, C2 = _int4_weight(up_packed, up_scales, gs, dev, "up_packed")
+    if R != R2 or C != C2:
+        _fail("gate and up must have one shape")
+    T, code, ac, pst = _product_args(dh, "dh", R, act, status)
+    g, u = _dense(g, "g", (T, R), dh.dtype, dev), _dense(u, "u", (T, R), dh.dtype, dev)
+    dh, lddh = _rows(dh, T, R, False)
+    dx = dh.new_empty((T, C))
     ws = torch.empty(query("forge_int4_backward_workspace_bytes", T, C, R, gs, 2), dtype=torch.uint8, device=dh.device)
-    call("forge_int4_gated_backward", dh.data_ptr(), lddh, code, ptr(g.contiguous()), ptr(u.contiguous()),
-         gate_packed.data_ptr(), gate_scales.data_ptr(), up_packed.data_ptr(), up_scales.data_ptr(), gs, T, C, R,
-         _abi.ACTS[act], ptr(dx), ptr(ws), ptr(status), stream_ptr())
+    call("forge_int4_gated_backward", dh.data_ptr(), lddh, code, g.data_ptr(), u.data_ptr(), gate_packed.data_ptr(),
+         gate_scales.data_ptr(), up_packed.data_ptr(), up_scales.data_ptr(), gs, T, C, R, ac, dx.data_ptr(), ws.data_ptr(),
+         pst, stream_ptr())
     return dx
