@@ -1,25 +1,26 @@
 // int4 products for many tokens on the tensor cores (tcgen05, accumulators in tensor memory), forward and backward.
 //
-// Forward (linear, gated), per 128-token x 256-weight-row tile:
-//   acc[t, r] = sum over chunks  scale[r, g] * ( sum over the chunk's channels  x[t, c] * (nibble(r, c) - 8) )
+// Forward (linear, gated): the weight rows are the M side (a row of the accumulator is a lane of tensor memory), the tokens
+// the N side:
+//   acc[r, t] = sum over chunks  scale[r, g] * ( sum over the chunk's channels  (nibble(r, c) - 8) * x[t, c] )
 // A chunk is a scale group (gs channels).  The inner sum is one accumulation in tensor memory whose operands are exact
-// (nibble - 8 is an integer of four bits); the scale is applied in fp32 when the chunk's accumulator is added to the
-// running sums, which live in registers.  So nothing is rounded before the result, and the tensor core's truncating
-// accumulation covers 128 terms at most.  Gated form: 128 gate rows and the 128 up rows of the same channels make the 256.
+// (nibble - 8 is an integer of four bits); a thread then adds its row's chunk to running sums in registers, times ONE
+// scale, since a thread sees one row only.  So nothing is rounded before the result, and the tensor core's truncating
+// accumulation covers 128 terms at most.  Gated form: a block of 32 rows is 16 gate rows and the 16 up rows of the same
+// channels, so both halves of a product meet in one warp.
 //
-// Backward (dx = dz W):  the K axis is the weight rows, so a chunk has many scales and they have to be in the operand:
-// W' = fp16((nibble - 8) * s'), s' the scale without its row's power of two (which dz carries exactly), from an fp16 pair
-// (hi, lo) so that W' is rounded once.  W is read along its rows, which are the N side here: an MN-major operand.
-// Chunks of 512 weight rows are added up in registers.
+// Backward (dx = dz W): M is the channels, read along the rows of W (an MN-major operand), K the weight rows.  A chunk has
+// many scales there, so they have to be in the operand: W' = fp16((nibble - 8) * s'), s' the scale without its row's power
+// of two (which dz carries exactly), from an fp16 pair (hi, lo) so that W' is rounded once.  Chunks of 512 weight rows are
+// added up in registers.
 //
 // A CTA (one per SM, 512 threads): warps 0-7 add finished chunks to the sums and run the epilogue, warps 8-11 turn packed
-// words into 16-bit operand tiles (read two stages ahead into registers, written with the 128-byte swizzle), warp 12
-// brings the token tile in with TMA, warp 13 owns tensor memory and issues the MMAs.  Four 48 KB stages of 64 channels,
-// two 256-column accumulators.  Registers move from the loading warps to the summing ones (setmaxnreg; 2 x 192 + 88 + 40
-// is the 4 x 128 that the CTA starts with).
+// words into 16-bit operand tiles (words read ahead into registers, tiles written with the 128-byte swizzle), warp 12
+// brings the token tile in with TMA, warp 13 owns tensor memory and issues the MMAs.  Stages of 64 channels, two
+// accumulators.  Registers move from the loading warps to the summing ones (setmaxnreg).
 //
 // With fewer tiles than SMs the K axis is shared by the CTAs of a cluster: each leaves its sums in its shared memory and
-// every CTA adds up a slice of the columns from all of them, in rank order, over distributed shared memory.
+// every CTA adds up a slice of the tokens from all of them, in rank order, over distributed shared memory.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -36,25 +37,25 @@ namespace {
 
 constexpr int kLinear = 0, kGated = 1, kDgrad = 2;
 
-constexpr int kMT = 128, kNT = 256, kKT = 64;
-constexpr int kABytes = kMT * 128, kBBytes = kNT * 128;
-constexpr int kStageBytes = kABytes + kBBytes;
-constexpr int kStages = 4;
-constexpr int kSlots = 8;                       // scale ring: one slot of 256 scales per chunk
+constexpr int kMT = 128, kKT = 64;              // rows of a CTA tile, channels of a stage
+constexpr int kABytes = kMT * 128;
 constexpr int kThreads = 512;
-constexpr int kRegsSum = 192, kRegsLoad = 88, kRegsMisc = 40;
+constexpr int kRegsSum = 176, kRegsLoad = 112, kRegsMisc = 48;
 static_assert(2 * kRegsSum + kRegsLoad + kRegsMisc <= 4 * 128, "register shares within the launch's total");
-constexpr int kOffScales = kStages * kStageBytes;
-constexpr int kOffBars = kOffScales + kSlots * kNT * 4;
+constexpr int kOutBytes = 32 * 128;             // a summing warp's block: 32 tokens x 32 rows, fp32
+constexpr int kRing = 196608;                   // operand stages
+constexpr int kOffOut = kRing;
+constexpr int kOffBars = kOffOut + 8 * kOutBytes;
 constexpr size_t kSmemBytes = kOffBars + 256 + 1024;
 
 struct TcParams {
     Int4Fwd f;
     Int4Dgrad d;
-    int64_t T, N;        // token rows, output columns (weight rows, or channels in the backward form)
-    int mt, nt;          // tiles
+    int64_t T, N;        // token rows, output columns (weight rows; channels in the backward form)
+    int rt, tt;          // row tiles, token tiles
     int nst;             // 64-wide k stages in all
     int split, per;      // cluster size along K, stages per member (a multiple of 2)
+    bool res_vec;        // residual rows start on 16 bytes
     int32_t *status;
 };
 
@@ -67,9 +68,10 @@ __device__ __forceinline__ uint64_t desc_mnmajor(uint32_t saddr) {
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(8192 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
            (2ull << 61);
 }
-template <int MODE, bool BF16> constexpr uint32_t idesc() {
-    return (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (MODE == kDgrad ? 1u << 16 : 0u) | ((kNT >> 3) << 17) |
-           ((kMT >> 4) << 24);
+// D fp32, A and B both bf16 or both fp16; the backward form's A is MN-major
+template <int MODE, bool BF16> constexpr uint32_t idesc(int m, int n) {
+    return (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (MODE == kDgrad ? 1u << 15 : 0u) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(m >> 4) << 24);
 }
 __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -101,10 +103,8 @@ __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
     asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
     return d;
 }
-__device__ __forceinline__ float2 unpack2(uint64_t v) {
-    uint32_t lo, hi;
+__device__ __forceinline__ void unpack2(uint64_t v, uint32_t &lo, uint32_t &hi) {
     asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
-    return make_float2(__uint_as_float(lo), __uint_as_float(hi));
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -118,26 +118,36 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t addr, uint32_t rank) {
                  : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
     return v;
 }
+__device__ __forceinline__ float4 lds_f4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
+__device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
 
-// eight codes of a word as (nibble - 8) in the 16-bit type, in channel order
+// eight codes of a word as (nibble - 8) in the 16-bit type, in channel order: a byte of w has the even code in its low
+// nibble, the same byte of w >> 4 the odd one; the pair goes into the low mantissa bits of 128 (bf16) or 1024 (fp16)
 template <bool BF16> __device__ __forceinline__ uint4 word_to_half(uint32_t w) {
+    const uint32_t w4 = w >> 4;
     uint32_t p[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t v = ((w >> (4 * i)) & 0x000F000Fu) | (BF16 ? 0x43004300u : 0x64006400u);
+        const uint32_t v = __byte_perm(w, w4, ((4 + i) << 8) | i) & 0x000F000Fu;
+        const uint32_t m = v | (BF16 ? 0x43004300u : 0x64006400u);
         if constexpr (BF16) {
-            const __nv_bfloat162 h = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&v), __floats2bfloat162_rn(136.0f, 136.0f));
+            const __nv_bfloat162 h = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&m), __floats2bfloat162_rn(136.0f, 136.0f));
             p[i] = *reinterpret_cast<const uint32_t *>(&h);
         } else {
-            const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&v), __floats2half2_rn(1032.0f, 1032.0f));
+            const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&m), __floats2half2_rn(1032.0f, 1032.0f));
             p[i] = *reinterpret_cast<const uint32_t *>(&h);
         }
     }
-    return make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410), __byte_perm(p[0], p[1], 0x7632),
-                      __byte_perm(p[2], p[3], 0x7632));
+    return make_uint4(p[0], p[1], p[2], p[3]);
 }
 __device__ __forceinline__ uint32_t scaled(uint32_t v, __half2 hi, __half2 lo) {
     const __half2 q = *reinterpret_cast<const __half2 *>(&v);
@@ -147,94 +157,121 @@ __device__ __forceinline__ uint32_t scaled(uint32_t v, __half2 hi, __half2 lo) {
 
 constexpr uint32_t kZeroWord = 0x88888888u;
 
-// where the four 32-column blocks of a summing warp lie in the tile: its half of the columns; in the gated form two
-// blocks of gate and the same two of up
-template <int MODE> __device__ __forceinline__ int block_col(int half, int j) {
-    return MODE == kGated ? (j >> 1) * 128 + half * 64 + (j & 1) * 32 : half * 128 + j * 32;
+// Polls without a pause first: the partner is a few hundred cycles away.  Then the bounded wait.
+__device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
+    return mbar_wait(bar, parity, abort_flag);
 }
 
-// Eight neighbouring outputs of one token row, starting at column c (a multiple of 8); u: the up projections (gated).
-template <typename T, int MODE, int W>
-__device__ __forceinline__ void emit(const TcParams &P, int64_t t, int64_t c, const float (&v)[W], const float (&u)[W]) {
-    const int64_t N = P.N;
-    if (c >= N) return;
-    const int64_t o = t * N + c;
-    float y[W];
+// Eight neighbouring outputs of token t, columns c .. c + 7 (c a multiple of 8); u: the up projections (gated).
+template <typename T, int MODE>
+__device__ __forceinline__ void emit8(const TcParams &P, int64_t t, int64_t c, float (&z)[8], const float (&u)[8]) {
+    const int64_t N = P.N, o = t * N + c;
+    if (t >= P.T || c >= N) return;
+    const bool vec = N % 8 == 0;
+    const auto put = [&](void *base, const float (&v)[8]) {
+        T *dst = (T *)base + o;
+        if (vec) {
+            store8(dst, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < N) dst[i] = Elem<T>::from_f(v[i]);
+        }
+    };
     if constexpr (MODE == kDgrad) {
-        const float s = P.d.unscale[t];
+        const float s = __ldg(P.d.unscale + t);
 #pragma unroll
-        for (int i = 0; i < W; ++i) y[i] = v[i] * s;
+        for (int i = 0; i < 8; ++i) z[i] *= s;
+        put(P.d.dx, z);
     } else {
-        const T *bias = (const T *)P.f.bias, *res = (const T *)P.f.res;
+        float r[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (MODE == kLinear && P.f.res) {
+            const T *res = (const T *)P.f.res + t * P.f.ldres + c;
+            if (P.res_vec && vec) {
+                load8(res, r);
+            } else {
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-            float z = v[i];
-            if (MODE == kLinear && bias && c + i < N) z += Elem<T>::to_f(bias[c + i]);
-            y[i] = z;
+                for (int i = 0; i < 8; ++i)
+                    if (c + i < N) r[i] = Elem<T>::to_f(res[i]);
+            }
         }
+        if (MODE == kLinear && P.f.bias)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < N) z[i] += Elem<T>::to_f(((const T *)P.f.bias)[c + i]);
         if (P.f.pre0) {
+            put(P.f.pre0, z);
+            if (MODE == kGated) put(P.f.pre1, u);
+        }
+        switch (P.f.act) {
+            case FORGE_ACT_RELU:
 #pragma unroll
-            for (int i = 0; i < W; ++i)
-                if (c + i < N) {
-                    ((T *)P.f.pre0)[o + i] = Elem<T>::from_f(y[i]);
-                    if (MODE == kGated) ((T *)P.f.pre1)[o + i] = Elem<T>::from_f(u[i]);
-                }
+                for (int i = 0; i < 8; ++i) z[i] = act_fwd<FORGE_ACT_RELU>(z[i]);
+                break;
+            case FORGE_ACT_SILU:
+#pragma unroll
+                for (int i = 0; i < 8; ++i) z[i] = act_fwd<FORGE_ACT_SILU>(z[i]);
+                break;
+            case FORGE_ACT_GELU:
+#pragma unroll
+                for (int i = 0; i < 8; ++i) z[i] = act_fwd<FORGE_ACT_GELU>(z[i]);
+                break;
+            default: break;
         }
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-            y[i] = act_fwd_rt(P.f.act, y[i]);
-            if (MODE == kGated) y[i] *= u[i];
-            if (MODE == kLinear && res && c + i < N) y[i] += Elem<T>::to_f(res[t * P.f.ldres + c + i]);
-        }
-    }
-    T *out = (T *)(MODE == kDgrad ? P.d.dx : P.f.y) + o;
-    if (W == 8 && N % 8 == 0) {
-        float w8[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w8[i] = y[i % W];
-        store8(out, w8);
-    } else {
-#pragma unroll
-        for (int i = 0; i < W; ++i)
-            if (c + i < N) out[i] = Elem<T>::from_f(y[i]);
+        for (int i = 0; i < 8; ++i) z[i] = MODE == kGated ? z[i] * u[i] : z[i] + r[i];
+        put(P.f.y, z);
     }
 }
 
-// T: output type; MODE; CH: channels per chunk (forward: the group size; backward: 512 weight rows)
-template <typename T, int MODE, int CH>
+// A summing warp's block of 32 tokens x 32 rows in shared memory: [token][row] fp32, the 16-byte piece index XORed with the
+// token, so lanes (rows) write one token and 4-lane groups read eight rows of a token without bank conflicts.
+__device__ __forceinline__ uint32_t blk(uint32_t buf, int token, int row) {
+    return buf + (uint32_t)(token * 128 + ((((row >> 2) ^ (token & 7)) << 4) | ((row & 3) << 2)));
+}
+__device__ __forceinline__ void rows8(uint32_t buf, int token, int row, float (&v)[8]) {
+    const float4 a = lds_f4(blk(buf, token, row)), b = lds_f4(blk(buf, token, row + 4));
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+
+// T: output type; MODE; CH: channels per chunk (forward: the group size; backward: 512 weight rows); NT: tokens per tile
+template <typename T, int MODE, int CH, int NT>
 __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_constant__ TcParams P,
                                                               const __grid_constant__ CUtensorMap tmap) {
     constexpr bool kBf16 = MODE != kDgrad && std::is_same<T, __nv_bfloat16>::value;
+    constexpr int kBBytes = NT * 128, kStageBytes = kABytes + kBBytes;
+    constexpr int kStages = kRing / kStageBytes < 8 ? kRing / kStageBytes : 8;
+    constexpr int kCols = NT / 2;                                     // tokens of a summing warp
+    constexpr int kTileCols = MODE == kGated ? 64 : kMT;              // output columns of a tile
+    constexpr int kPerStage = CH < kKT ? kKT / CH : 1, kStagesPer = CH > kKT ? CH / kKT : 1;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *smem_al = smem_raw + (smem_base - smem_u32(smem_raw));
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem_al + kOffBars);
-    const uint32_t b_full = smem_u32(bars), b_empty = b_full + 8 * kStages, b_afull = b_empty + 8 * kStages,
-                   b_aempty = b_afull + 16, b_sfull = b_aempty + 16, b_sempty = b_sfull + 8 * kSlots;
-    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 2 * kStages + 4 + 2 * kSlots);
+    const uint32_t b_full = smem_u32(bars), b_empty = b_full + 8 * kStages, b_afull = b_empty + 8 * kStages, b_aempty = b_afull + 16;
+    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 2 * kStages + 4);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
-    static_assert((2 * kStages + 4 + 2 * kSlots) * 8 + 8 <= 256, "barrier block");
+    static_assert((2 * kStages + 4) * 8 + 8 <= 256, "barrier block");
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int s = 0; s < kStages; ++s) {
-            mbar_init(b_full + 8 * s, 1 + 128);
+            mbar_init(b_full + 8 * s, 1 + 4);      // the TMA issuer and four loading warps
             mbar_init(b_empty + 8 * s, 1);
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(b_afull + 8 * a, 1);
             mbar_init(b_aempty + 8 * a, 8);
         }
-        for (int s = 0; s < kSlots; ++s) {
-            mbar_init(b_sfull + 8 * s, 128);
-            mbar_init(b_sempty + 8 * s, 8);
-        }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 13) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)), "r"(512u)
-                     : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                     "r"(2u * NT) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
@@ -244,206 +281,203 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
 
     const int rank = P.split > 1 ? (int)(blockIdx.x % P.split) : 0;
     const int st0 = rank * P.per, st1 = min(P.nst, st0 + P.per);      // may be empty
-    const int ntiles = P.mt * P.nt;
+    const int ntiles = P.rt * P.tt;
     const int tile0 = P.split > 1 ? (int)(blockIdx.x / P.split) : (int)blockIdx.x;
     const int tile_step = P.split > 1 ? ntiles : (int)gridDim.x;
-    constexpr int kRowsN = MODE == kGated ? 128 : kNT;                // output columns of a tile
 
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSum));
         const int quarter = warp & 3, half = warp >> 2;
-        const uint32_t tlane = tmem_base + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t tlane = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * kCols;
         uint32_t chunk = 0;
         bool ok = true;
         for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
-            const int64_t m0 = (int64_t)(tile / P.nt) * kMT, n0 = (int64_t)(tile % P.nt) * kRowsN;
-            uint64_t acc[4][16];
+            const int64_t t0 = (int64_t)(tile / P.rt) * NT, c0 = (int64_t)(tile % P.rt) * kTileCols;
+            uint64_t acc[kCols / 2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[j][i] = 0ull;
-            constexpr int kPerStage = CH < kKT ? kKT / CH : 1, kStagesPer = CH > kKT ? CH / kKT : 1;
+            for (int i = 0; i < kCols / 2; ++i) acc[i] = 0ull;
+            const float *sp = nullptr;                                // this lane's scales
+            int64_t g = 0;
+            float s_next = 0.0f;
+            if constexpr (MODE != kDgrad) {
+                int64_t row = MODE == kGated ? c0 + quarter * 16 + (lane & 15) : c0 + quarter * 32 + lane;
+                row = row < P.f.R ? row : P.f.R - 1;
+                sp = P.f.scales[MODE == kGated && lane >= 16 ? 1 : 0] + row * P.f.G;
+                g = (int64_t)st0 * kKT / CH;
+                s_next = g < P.f.G ? __ldg(sp + g) : 0.0f;
+            }
             const int nch = (st1 - st0 + kStagesPer - 1) / kStagesPer * kPerStage;
             for (int ch = 0; ch < nch; ++ch, ++chunk) {
-                const uint32_t buf = chunk & 1u, slot = chunk % kSlots;
-                ok = mbar_wait(b_afull + 8 * buf, (chunk >> 1) & 1u, abort_flag);
-                if (MODE != kDgrad) ok = ok && mbar_wait(b_sfull + 8 * slot, (chunk / kSlots) & 1u, abort_flag);
+                const uint32_t buf = chunk & 1u;
+                const float sc = s_next;
+                if constexpr (MODE != kDgrad) {
+                    ++g;
+                    s_next = g < P.f.G ? __ldg(sp + g) : 0.0f;
+                }
+                ok = wait_on(b_afull + 8 * buf, (chunk >> 1) & 1u, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
-                const uint8_t *sc = smem_al + kOffScales + slot * (kNT * 4);
+                const uint64_t sc2 = pack2(__float_as_uint(sc), __float_as_uint(sc));
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int col = block_col<MODE>(half, j >> 1) + (j & 1) * 16;
-                    uint32_t v[16];
-                    tmem_ld16(tlane + buf * kNT + col, v);
+                for (int j = 0; j < kCols / 32; ++j) {
+                    uint32_t v[32];
+                    tmem_ld32(tlane + buf * NT + j * 32, v);
                     tmem_ld_wait();
-                    if (j == 7) {      // the accumulator is free once everything is in registers
+                    if (j == kCols / 32 - 1) {      // the accumulator is free once everything is in registers
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(b_aempty + 8 * buf);
                     }
-                    uint64_t *a = acc[j >> 1] + (j & 1) * 8;
 #pragma unroll
-                    for (int i = 0; i < 8; i += 2) {
-                        if constexpr (MODE == kDgrad) {
-                            a[i] = add2(a[i], pack2(v[2 * i], v[2 * i + 1]));
-                            a[i + 1] = add2(a[i + 1], pack2(v[2 * i + 2], v[2 * i + 3]));
-                        } else {
-                            const ulonglong2 s = *reinterpret_cast<const ulonglong2 *>(sc + (col + 2 * i) * 4);
-                            a[i] = fma2(pack2(v[2 * i], v[2 * i + 1]), s.x, a[i]);
-                            a[i + 1] = fma2(pack2(v[2 * i + 2], v[2 * i + 3]), s.y, a[i + 1]);
-                        }
+                    for (int i = 0; i < 16; ++i) {
+                        if constexpr (MODE == kDgrad) acc[j * 16 + i] = add2(acc[j * 16 + i], pack2(v[2 * i], v[2 * i + 1]));
+                        else acc[j * 16 + i] = fma2(pack2(v[2 * i], v[2 * i + 1]), sc2, acc[j * 16 + i]);
                     }
-                }
-                if (MODE != kDgrad) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(b_sempty + 8 * slot);
                 }
             }
             if (!ok) break;
             if (P.split == 1) {
-                const int64_t t = m0 + quarter * 32 + lane;
-                if (t < P.T) {
+                const uint32_t buf = smem_base + kOffOut + warp * kOutBytes;
+                const uint32_t wb = blk(buf, 0, lane) - buf;          // piece index without the token's bits
 #pragma unroll
-                    for (int j = 0; j < (MODE == kGated ? 2 : 4); ++j)
+                for (int j = 0; j < kCols / 32; ++j) {
+                    const int64_t tb = t0 + half * kCols + j * 32;
+                    if (tb >= P.T) break;
+                    __syncwarp();
 #pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                            float a[8], b[8];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float2 p = unpack2(acc[j][i + e]);
-                                a[2 * e] = p.x; a[2 * e + 1] = p.y;
-                                const float2 r = unpack2(acc[MODE == kGated ? j + 2 : j][i + e]);
-                                b[2 * e] = r.x; b[2 * e + 1] = r.y;
-                            }
-                            emit<T, MODE, 8>(P, t, n0 + block_col<MODE>(half, j) + 2 * i, a, b);
+                    for (int i = 0; i < 16; ++i) {
+                        uint32_t lo, hi;
+                        unpack2(acc[j * 16 + i], lo, hi);
+                        sts32(buf + (2 * i) * 128 + (wb ^ (((2 * i) & 7) << 4)), lo);
+                        sts32(buf + (2 * i + 1) * 128 + (wb ^ (((2 * i + 1) & 7) << 4)), hi);
+                    }
+                    __syncwarp();
+                    if constexpr (MODE == kGated) {
+#pragma unroll 1
+                        for (int k = 0; k < 2; ++k) {
+                            const int tok = k * 16 + (lane >> 1), p = (lane & 1) * 8;
+                            float z[8], u[8];
+                            rows8(buf, tok, p, z);
+                            rows8(buf, tok, 16 + p, u);
+                            emit8<T, MODE>(P, tb + tok, c0 + quarter * 16 + p, z, u);
                         }
+                    } else {
+#pragma unroll 1
+                        for (int k = 0; k < 4; ++k) {
+                            const int tok = k * 8 + (lane >> 2), p = (lane & 3) * 8;
+                            float z[8];
+                            rows8(buf, tok, p, z);
+                            emit8<T, MODE>(P, tb + tok, c0 + quarter * 32 + p, z, z);
+                        }
+                    }
                 }
             } else {
-                // sums to shared memory (every MMA of this CTA is complete, the stages are free): [column / 4][row] float4
-                const int row = quarter * 32 + lane;
+                // sums to shared memory (every MMA of this CTA is complete, the stages are free): [token][row] fp32
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        const int c4 = (block_col<MODE>(half, j) + 2 * i) >> 2;
-                        const float2 p = unpack2(acc[j][i]), r = unpack2(acc[j][i + 1]);
-                        sts128(smem_base + (uint32_t)(c4 * kMT + row) * 16u,
-                               make_uint4(__float_as_uint(p.x), __float_as_uint(p.y), __float_as_uint(r.x), __float_as_uint(r.y)));
-                    }
+                for (int i = 0; i < kCols / 2; ++i) {
+                    uint32_t lo, hi;
+                    unpack2(acc[i], lo, hi);
+                    const uint32_t a = smem_base + (uint32_t)((half * kCols + 2 * i) * kMT + quarter * 32 + lane) * 4u;
+                    sts32(a, lo);
+                    sts32(a + kMT * 4, hi);
+                }
             }
         }
         if (P.split > 1) {
             cluster_sync();
-            const int64_t m0 = (int64_t)(tile0 / P.nt) * kMT, n0 = (int64_t)(tile0 % P.nt) * kRowsN;
-            const int per4 = kRowsN / 4 / P.split;                    // column quads of this CTA's slice
-            for (int i = tid; i < per4 * kMT && ok; i += 256) {
-                const int c4 = rank * per4 + i / kMT, row = i % kMT;
-                const int64_t t = m0 + row;
-                if (t >= P.T) continue;
-                float a[4] = {0.0f, 0.0f, 0.0f, 0.0f}, b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const int64_t t0 = (int64_t)(tile0 / P.rt) * NT, c0 = (int64_t)(tile0 % P.rt) * kTileCols;
+            const int per = NT / P.split;                             // tokens of this CTA's slice
+            constexpr int kGroups = kTileCols / 8;
+            for (int i = tid; i < per * kGroups && ok; i += 256) {
+                const int tok = rank * per + i / kGroups, cg = i % kGroups;
+                if (t0 + tok >= P.T) continue;
+                // gated: channels cg * 8 .. are gate rows of the 32-row block cg / 2, the up rows 16 further
+                const int row = MODE == kGated ? (cg >> 1) * 32 + (cg & 1) * 8 : cg * 8;
+                float z[8] = {}, u[8] = {};
                 for (int r = 0; r < P.split; ++r) {
-                    const float4 v = ld_cluster(smem_base + (uint32_t)(c4 * kMT + row) * 16u, r);
-                    a[0] += v.x; a[1] += v.y; a[2] += v.z; a[3] += v.w;
+                    const uint32_t a = smem_base + (uint32_t)(tok * kMT + row) * 4u;
+                    const float4 v = ld_cluster(a, r), w = ld_cluster(a + 16, r);
+                    z[0] += v.x; z[1] += v.y; z[2] += v.z; z[3] += v.w;
+                    z[4] += w.x; z[5] += w.y; z[6] += w.z; z[7] += w.w;
                     if constexpr (MODE == kGated) {
-                        const float4 w = ld_cluster(smem_base + (uint32_t)((c4 + 32) * kMT + row) * 16u, r);
-                        b[0] += w.x; b[1] += w.y; b[2] += w.z; b[3] += w.w;
+                        const float4 v2 = ld_cluster(a + 64, r), w2 = ld_cluster(a + 80, r);
+                        u[0] += v2.x; u[1] += v2.y; u[2] += v2.z; u[3] += v2.w;
+                        u[4] += w2.x; u[5] += w2.y; u[6] += w2.z; u[7] += w2.w;
                     }
                 }
-                emit<T, MODE, 4>(P, t, n0 + c4 * 4, a, b);
+                emit8<T, MODE>(P, t0 + tok, c0 + cg * 8, z, u);
             }
+            __syncwarp();
         }
     } else if (warp < 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
         const int lt = tid - 256;                                     // 0..127
-        uint32_t it = 0, chunk = 0;
+        uint32_t it = 0;
         bool ok = true;
         if constexpr (MODE != kDgrad) {
-            const int CP = (int)(P.f.C / 8);
-            const bool vec = P.f.vec8;
-            const int q = lt & 3, r0 = lt >> 2;                       // words 2q, 2q+1 of rows r0 + 32 p
+            // four lanes share a row of the stage: words 2q, 2q+1 of rows r0 + 32 p
+            const int CP = (int)(P.f.C / 8), q = lt & 3, r0 = lt >> 2;
+            const uint32_t d0 = (uint32_t)((r0 >> 3) * 1024 + (r0 & 7) * 128), x0 = (uint32_t)(((2 * q) ^ (r0 & 7)) << 4),
+                           x1 = (uint32_t)(((2 * q + 1) ^ (r0 & 7)) << 4);
+            constexpr int kAhead = 4;
             for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
-                const int64_t n0 = (int64_t)(tile % P.nt) * kRowsN;
-                uint2 w[2][8];
-                const auto row_of = [&](int p, const uint32_t *&base) -> int64_t {
-                    const int r = r0 + 32 * p;
-                    const bool second = MODE == kGated && r >= 128;
-                    base = P.f.packed[second ? 1 : 0];
-                    const int64_t row = n0 + (second ? r - 128 : r);
-                    return row < P.f.R ? row : P.f.R - 1;             // rows past the matrix: computed, never stored
-                };
-                const auto fetch = [&](int st, uint2 (&d)[8]) {
+                const int64_t c0 = (int64_t)(tile % P.rt) * kTileCols;
+                const uint32_t *rp[4];
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    int64_t row = MODE == kGated ? c0 + p * 16 + (r0 & 15) : c0 + p * 32 + r0;
+                    row = row < P.f.R ? row : P.f.R - 1;              // rows past the matrix: computed, never stored
+                    rp[p] = P.f.packed[MODE == kGated && r0 >= 16 ? 1 : 0] + row * CP + 2 * q;
+                }
+                uint2 w[kAhead][4];
+                const auto fetch = [&](int st, uint2 (&d)[4]) {
                     const int word = st * 8 + 2 * q;
+                    if (P.f.vec8 && st * 8 + 8 <= CP) {
 #pragma unroll
-                    for (int p = 0; p < 8; ++p) {
-                        const uint32_t *base;
-                        const int64_t row = row_of(p, base);
-                        const uint32_t *src = base + row * CP + word;
-                        if (vec && word < CP) {
-                            d[p] = __ldg(reinterpret_cast<const uint2 *>(src));
-                        } else {
-                            d[p].x = word < CP ? __ldg(src) : kZeroWord;
-                            d[p].y = word + 1 < CP ? __ldg(src + 1) : kZeroWord;
+                        for (int p = 0; p < 4; ++p) d[p] = __ldg(reinterpret_cast<const uint2 *>(rp[p] + st * 8));
+                    } else {
+#pragma unroll
+                        for (int p = 0; p < 4; ++p) {
+                            d[p].x = word < CP ? __ldg(rp[p] + st * 8) : kZeroWord;
+                            d[p].y = word + 1 < CP ? __ldg(rp[p] + st * 8 + 1) : kZeroWord;
                         }
                     }
                 };
-                if (st0 < st1) fetch(st0, w[0]);
-                if (st0 + 1 < st1) fetch(st0 + 1, w[1]);
-                const auto stage_work = [&](int st, uint2 (&d)[8]) {
-                    const uint32_t s = it % kStages;
-                    // the chunk's scales (rows lt and lt + 128 of the tile)
-                    constexpr int kPerStage = CH < kKT ? kKT / CH : 1, kStagesPer = CH > kKT ? CH / kKT : 1;
-                    if ((st - st0) % kStagesPer == 0) {
 #pragma unroll
-                        for (int e = 0; e < kPerStage; ++e, ++chunk) {
-                            const int64_t g = (int64_t)st * kKT / CH + e;
-                            float v[2];
+                for (int a = 0; a < kAhead; ++a)
+                    if (st0 + a < st1) fetch(st0 + a, w[a]);
+                for (int stb = st0; stb < st1 && ok; stb += kAhead) {
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const bool second = MODE == kGated && h == 1;
-                                int64_t row = n0 + lt + (MODE == kGated ? 0 : h * 128);
-                                row = row < P.f.R ? row : P.f.R - 1;
-                                v[h] = g < P.f.G ? __ldg(P.f.scales[second ? 1 : 0] + row * P.f.G + g) : 0.0f;
-                            }
-                            const uint32_t slot = chunk % kSlots;
-                            ok = ok && mbar_wait(b_sempty + 8 * slot, ((chunk / kSlots) & 1u) ^ 1u, abort_flag);
-                            if (!ok) return;
-                            float *dst = reinterpret_cast<float *>(smem_al + kOffScales + slot * (kNT * 4));
-                            dst[lt] = v[0];
-                            dst[lt + 128] = v[1];
-                            mbar_arrive(b_sfull + 8 * slot);
+                    for (int a = 0; a < kAhead; ++a) {
+                        const int st = stb + a;
+                        if (st >= st1) break;
+                        const uint32_t s = it % kStages;
+                        ok = wait_on(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
+                        if (!ok) break;
+                        const uint32_t tileb = smem_base + s * kStageBytes + d0;
+#pragma unroll
+                        for (int p = 0; p < 4; ++p) {
+                            sts128(tileb + p * 4096 + x0, word_to_half<kBf16>(w[a][p].x));
+                            sts128(tileb + p * 4096 + x1, word_to_half<kBf16>(w[a][p].y));
                         }
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(b_full + 8 * s);
+                        ++it;
+                        if (st + kAhead < st1) fetch(st + kAhead, w[a]);
                     }
-                    ok = mbar_wait(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
-                    if (!ok) return;
-                    const uint32_t tileb = smem_base + s * kStageBytes + kABytes;
-#pragma unroll
-                    for (int p = 0; p < 8; ++p) {
-                        const int r = r0 + 32 * p;
-                        const uint32_t rowb = tileb + (uint32_t)((r >> 3) * 1024 + (r & 7) * 128);
-                        sts128(rowb + (uint32_t)(((2 * q) ^ (r & 7)) << 4), word_to_half<kBf16>(d[p].x));
-                        sts128(rowb + (uint32_t)(((2 * q + 1) ^ (r & 7)) << 4), word_to_half<kBf16>(d[p].y));
-                    }
-                    fence_proxy_async();
-                    mbar_arrive(b_full + 8 * s);
-                    ++it;
-                    if (st + 2 < st1) fetch(st + 2, d);
-                };
-                for (int st = st0; st < st1 && ok; st += 2) {
-                    stage_work(st, w[0]);
-                    if (ok && st + 1 < st1) stage_work(st + 1, w[1]);
                 }
             }
         } else {
-            const int CP = (int)(P.d.C / 8);
-            const int l8 = lt & 7, k0 = lt >> 3;                      // words l8 + 8 i of K rows k0 + 16 p
+            // words l8 + 8 i of K rows k0 + 16 p: eight lanes read 32 bytes of a row, the 64 channels of block i
+            const int CP = (int)(P.d.C / 8), l8 = lt & 7, k0 = lt >> 3;
             const int64_t K = (int64_t)P.d.mats * P.d.R;
             for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
-                const int64_t n0 = (int64_t)(tile % P.nt) * kNT;
-                uint32_t w[4][4];
-                __half2 sc[4][4];
-                const auto fetch = [&](int st) {
+                const int64_t c0 = (int64_t)(tile % P.rt) * kTileCols;
+                uint32_t w[2][4][2];
+                __half2 sc[2][4][2];
+                const auto fetch = [&](int st, uint32_t (&wd)[4][2], __half2 (&sd)[4][2]) {
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
                         const int64_t k = (int64_t)st * kKT + k0 + 16 * p;
@@ -451,39 +485,47 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                         const uint32_t *src = P.d.packed[second ? 1 : 0] + (k - (second ? P.d.R : 0)) * CP;
                         const __half2 *ss = P.d.pairs + k * P.d.G;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int64_t word = n0 / 8 + l8 + 8 * i;
+                        for (int i = 0; i < 2; ++i) {
+                            const int64_t word = c0 / 8 + l8 + 8 * i;
                             const bool in = k < K && word < CP;
-                            w[p][i] = in ? __ldg(src + word) : kZeroWord;
-                            sc[p][i] = in ? ss[(word * 8) / P.d.gs] : __half2(__ushort_as_half(0), __ushort_as_half(0));
+                            wd[p][i] = in ? __ldg(src + word) : kZeroWord;
+                            sd[p][i] = in ? __ldg(ss + (word * 8) / P.d.gs) : __half2(__ushort_as_half(0), __ushort_as_half(0));
                         }
                     }
                 };
-                if (st0 < st1) fetch(st0);
-                for (int st = st0; st < st1; ++st) {
-                    const uint32_t s = it % kStages;
-                    ok = mbar_wait(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
-                    if (!ok) break;
-                    const uint32_t tileb = smem_base + s * kStageBytes + kABytes;
 #pragma unroll
-                    for (int p = 0; p < 4; ++p) {
-                        const int k = k0 + 16 * p;
+                for (int a = 0; a < 2; ++a)
+                    if (st0 + a < st1) fetch(st0 + a, w[a], sc[a]);
+                for (int stb = st0; stb < st1 && ok; stb += 2) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint4 v = word_to_half<false>(w[p][i]);
-                            const __half2 hi = __low2half2(sc[p][i]), lo = __high2half2(sc[p][i]);
-                            sts128(tileb + (uint32_t)(i * 8192 + (k >> 3) * 1024 + (k & 7) * 128 + ((l8 ^ (k & 7)) << 4)),
-                                   make_uint4(scaled(v.x, hi, lo), scaled(v.y, hi, lo), scaled(v.z, hi, lo), scaled(v.w, hi, lo)));
-                        }
+                    for (int a = 0; a < 2; ++a) {
+                        const int st = stb + a;
+                        if (st >= st1) break;
+                        const uint32_t s = it % kStages;
+                        ok = wait_on(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
+                        if (!ok) break;
+                        const uint32_t tileb = smem_base + s * kStageBytes + (uint32_t)((k0 >> 3) * 1024 + (k0 & 7) * 128 +
+                                                                                       ((l8 ^ (k0 & 7)) << 4));
+#pragma unroll
+                        for (int p = 0; p < 4; ++p)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const uint4 v = word_to_half<false>(w[a][p][i]);
+                                const __half2 hi = __low2half2(sc[a][p][i]), lo = __high2half2(sc[a][p][i]);
+                                sts128(tileb + i * 8192 + p * 2048,
+                                       make_uint4(scaled(v.x, hi, lo), scaled(v.y, hi, lo), scaled(v.z, hi, lo), scaled(v.w, hi, lo)));
+                            }
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(b_full + 8 * s);
+                        ++it;
+                        if (st + 2 < st1) fetch(st + 2, w[a], sc[a]);
                     }
-                    fence_proxy_async();
-                    mbar_arrive(b_full + 8 * s);
-                    ++it;
-                    if (st + 1 < st1) fetch(st + 1);
                 }
             }
         }
-        if (P.split > 1) { __syncwarp(); cluster_sync(); }
+        __syncwarp();
+        if (P.split > 1) cluster_sync();
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMisc));
         if (warp == 12) {
@@ -492,28 +534,26 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
             bool ok = true;
             if (lane == 0) {
                 for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
-                    const int m0 = (tile / P.nt) * kMT;
+                    const int t0 = (tile / P.rt) * NT;
                     for (int st = st0; st < st1; ++st, ++it) {
                         const uint32_t s = it % kStages;
-                        ok = mbar_wait(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
+                        ok = wait_on(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
                         if (!ok) break;
-                        mbar_arrive_expect_tx(b_full + 8 * s, kABytes);
-                        tma_load_2d(smem_base + s * kStageBytes, &tmap, st * kKT, m0, b_full + 8 * s);
+                        mbar_arrive_expect_tx(b_full + 8 * s, kBBytes);
+                        tma_load_2d(smem_base + s * kStageBytes + kABytes, &tmap, st * kKT, t0, b_full + 8 * s);
                     }
                 }
             }
-            __syncwarp();
         } else if (warp == 13) {
             // ------------------------------ MMA issuer ------------------------------
             uint32_t it = 0, chunk = 0;
             bool ok = true;
             constexpr int kStepsPer = (CH < kKT ? CH : kKT) / 16;     // k-steps of a chunk inside a stage
-            constexpr int kStagesPer = CH > kKT ? CH / kKT : 1;
             if (lane == 0) {
                 for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
                     for (int st = st0; st < st1 && ok; ++st, ++it) {
                         const uint32_t s = it % kStages;
-                        ok = mbar_wait(b_full + 8 * s, (it / kStages) & 1u, abort_flag);
+                        ok = wait_on(b_full + 8 * s, (it / kStages) & 1u, abort_flag);
                         if (!ok) break;
                         tc_fence_after();
                         const uint32_t abase = smem_base + s * kStageBytes, bbase = abase + kABytes;
@@ -523,13 +563,13 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                         for (int kk = 0; kk < kKT / 16; ++kk) {
                             const bool starts = kk % kStepsPer == 0 && first_stage;
                             if (starts) {
-                                ok = mbar_wait(b_aempty + 8 * (chunk & 1u), ((chunk >> 1) & 1u) ^ 1u, abort_flag);
+                                ok = wait_on(b_aempty + 8 * (chunk & 1u), ((chunk >> 1) & 1u) ^ 1u, abort_flag);
                                 if (!ok) break;
                                 tc_fence_after();
                             }
-                            umma_f16(tmem_base + (chunk & 1u) * kNT, desc_kmajor(abase + kk * 32),
-                                     MODE == kDgrad ? desc_mnmajor(bbase + kk * 2048) : desc_kmajor(bbase + kk * 32),
-                                     idesc<MODE, kBf16>(), starts ? 0u : 1u);
+                            umma_f16(tmem_base + (chunk & 1u) * NT,
+                                     MODE == kDgrad ? desc_mnmajor(abase + kk * 2048) : desc_kmajor(abase + kk * 32),
+                                     desc_kmajor(bbase + kk * 32), idesc<MODE, kBf16>(kMT, NT), starts ? 0u : 1u);
                             if (kk % kStepsPer == kStepsPer - 1 && last_stage) {
                                 umma_commit(b_afull + 8 * (chunk & 1u));
                                 ++chunk;
@@ -540,8 +580,8 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                     }
                 }
             }
-            __syncwarp();
         }
+        __syncwarp();
         if (P.split > 1) cluster_sync();
     }
     // ------------------------------ teardown ------------------------------
@@ -552,14 +592,14 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
     tc_fence_before();
     __syncthreads();
     if (*abort_flag) {           // gave up: let copies and MMAs in flight land before shared and tensor memory are given back
-        const long long t0 = clock64();
-        while (clock64() - t0 < 200000) __nanosleep(1000);
+        const long long c0 = clock64();
+        while (clock64() - c0 < 200000) __nanosleep(1000);
         if (tid == 0 && P.status) atomicExch(P.status, FORGE_ERR_TIMEOUT);
         __syncthreads();
     }
     if (warp == 13) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2u * NT) : "memory");
     }
 }
 
@@ -578,31 +618,45 @@ EncodeFn encode_fn() {
     }();
     return fn;
 }
-// [rows, cols] of 16-bit elements, row stride ld elements; box of 64 columns x 128 rows, 128-byte swizzle, zero fill
-bool make_map(CUtensorMap *m, const void *base, bool bf16, int64_t rows, int64_t cols, int64_t ld) {
+// [rows, cols] of 16-bit elements, row stride ld elements; box of 64 columns x box_rows rows, 128-byte swizzle, zero fill
+bool make_map(CUtensorMap *m, const void *base, bool bf16, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
     EncodeFn fn = encode_fn();
     if (!fn) return false;
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
-    const cuuint32_t box[2] = {kKT, kMT}, es[2] = {1, 1};
+    const cuuint32_t box[2] = {kKT, (cuuint32_t)box_rows}, es[2] = {1, 1};
     return fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(base), dims,
               strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int MODE, int CH> int launch(TcParams &P, const CUtensorMap &map, const char *who, cudaStream_t st) {
+struct TokenSource {
+    const void *base;
+    bool bf16;
+    int64_t rows, cols, ld;
+};
+
+template <typename T, int MODE, int CH, int NT>
+int launch(TcParams &P, const TokenSource &src, const char *who, cudaStream_t st) {
     int dev = 0, sms = 148;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    const int64_t tiles = (int64_t)P.mt * P.nt;
-    if (tiles > 0x3fffffff) {
-        set_error("%s: more than 2^30 output tiles", who);
+    const int64_t rt = cdiv(P.N, (int64_t)(MODE == kGated ? 64 : kMT)), tt = cdiv(P.T, (int64_t)NT), tiles = rt * tt;
+    if (tiles > 0x0fffffff) {
+        set_error("%s: more than 2^28 output tiles", who);
         return FORGE_ERR_UNSUPPORTED;
     }
+    alignas(64) CUtensorMap map;
+    if (!make_map(&map, src.base, src.bf16, src.rows, src.cols, src.ld, NT)) {
+        set_error("%s: no tensor map could be made", who);
+        return FORGE_ERR_LAUNCH;
+    }
+    P.rt = (int)rt;
+    P.tt = (int)tt;
     const int units = (P.nst + 1) / 2;                                 // 128-wide pieces of K
     P.split = 1;
     while (P.split < 8 && tiles * P.split * 2 <= sms && units >= P.split * 4) P.split *= 2;
     P.per = (units + P.split - 1) / P.split * 2;
-    const auto kernel = int4_tc_kernel<T, MODE, CH>;
+    const auto kernel = int4_tc_kernel<T, MODE, CH, NT>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
     if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg{};
@@ -626,10 +680,15 @@ template <typename T, int MODE, int CH> int launch(TcParams &P, const CUtensorMa
     FORGE_NOTE_LAUNCH();
     return FORGE_OK;
 }
-template <typename T, int MODE> int launch_gs(TcParams &P, const CUtensorMap &map, const char *who, cudaStream_t st) {
-    if (P.f.gs == 32) return launch<T, MODE, 32>(P, map, who, st);
-    if (P.f.gs == 64) return launch<T, MODE, 64>(P, map, who, st);
-    return launch<T, MODE, 128>(P, map, who, st);
+// token tiles of 64 when one or two of them cover all tokens, else of 256
+template <typename T, int MODE, int CH> int launch_nt(TcParams &P, const TokenSource &src, const char *who, cudaStream_t st) {
+    if (P.T <= 128) return launch<T, MODE, CH, 64>(P, src, who, st);
+    return launch<T, MODE, CH, 256>(P, src, who, st);
+}
+template <typename T, int MODE> int launch_gs(TcParams &P, const TokenSource &src, const char *who, cudaStream_t st) {
+    if (P.f.gs == 32) return launch_nt<T, MODE, 32>(P, src, who, st);
+    if (P.f.gs == 64) return launch_nt<T, MODE, 64>(P, src, who, st);
+    return launch_nt<T, MODE, 128>(P, src, who, st);
 }
 
 }  // namespace
@@ -640,30 +699,19 @@ int int4_fwd_tc(const Int4Fwd &F, bool bf16, bool gated, cudaStream_t st) {
     const char *who = gated ? "forge_int4_gated" : "forge_int4_linear";
     TcParams P{};
     P.f = F; P.T = F.T; P.N = F.R; P.status = F.status;
-    P.mt = (int)cdiv(F.T, (int64_t)kMT);
-    P.nt = (int)cdiv(F.R, (int64_t)(gated ? 128 : kNT));
     P.nst = (int)cdiv(F.C, (int64_t)kKT);
-    alignas(64) CUtensorMap map;
-    if (!make_map(&map, F.x, bf16, F.T, F.C, F.ldx)) {
-        set_error("%s: no tensor map could be made", who);
-        return FORGE_ERR_LAUNCH;
-    }
-    if (bf16) return gated ? launch_gs<__nv_bfloat16, kGated>(P, map, who, st) : launch_gs<__nv_bfloat16, kLinear>(P, map, who, st);
-    return gated ? launch_gs<__half, kGated>(P, map, who, st) : launch_gs<__half, kLinear>(P, map, who, st);
+    P.res_vec = F.ldres % 8 == 0 && (uintptr_t)F.res % 16 == 0;
+    const TokenSource src{F.x, bf16, F.T, F.C, F.ldx};
+    if (bf16) return gated ? launch_gs<__nv_bfloat16, kGated>(P, src, who, st) : launch_gs<__nv_bfloat16, kLinear>(P, src, who, st);
+    return gated ? launch_gs<__half, kGated>(P, src, who, st) : launch_gs<__half, kLinear>(P, src, who, st);
 }
 
 int int4_dgrad_tc(const Int4Dgrad &D, bool bf16, const char *who, cudaStream_t st) {
     TcParams P{};
     P.d = D; P.T = D.T; P.N = D.C; P.status = D.status;
-    P.mt = (int)cdiv(D.T, (int64_t)kMT);
-    P.nt = (int)cdiv(D.C, (int64_t)kNT);
     P.nst = (int)(D.ldk / kKT);
-    alignas(64) CUtensorMap map;
-    if (!make_map(&map, D.a, false, D.T, D.ldk, D.ldk)) {
-        set_error("%s: no tensor map could be made", who);
-        return FORGE_ERR_LAUNCH;
-    }
-    return bf16 ? launch<__nv_bfloat16, kDgrad, 512>(P, map, who, st) : launch<__half, kDgrad, 512>(P, map, who, st);
+    const TokenSource src{D.a, false, D.T, D.ldk, D.ldk};
+    return bf16 ? launch_nt<__nv_bfloat16, kDgrad, 512>(P, src, who, st) : launch_nt<__half, kDgrad, 512>(P, src, who, st);
 }
 
 }  // namespace forge
