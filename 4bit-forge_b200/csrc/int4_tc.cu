@@ -14,10 +14,14 @@
 // of two (which dz carries exactly), from an fp16 pair (hi, lo) so that W' is rounded once.  Chunks of 512 weight rows are
 // added up in registers.
 //
-// A CTA (one per SM, 512 threads): warps 0-7 add finished chunks to the sums and run the epilogue, warps 8-11 turn packed
-// words into 16-bit operand tiles (words read ahead into registers, tiles written with the 128-byte swizzle), warp 12
-// brings the token tile in with TMA, warp 13 owns tensor memory and issues the MMAs.  Stages of 64 channels, two
-// accumulators.  Registers move from the loading warps to the summing ones (setmaxnreg).
+// A CTA (one per SM, 640 threads): warps 0-7 add finished chunks to the sums and run the epilogue, warps 8-11 and 12-15
+// turn packed words into 16-bit operand tiles, one stage each in turn (words read ahead into registers, tiles written with
+// the 128-byte swizzle), warp 16 brings the token tile in with TMA, warp 17 owns tensor memory and issues the MMAs.  Stages
+// of 64 channels, two accumulators.  Registers move from the loading warps to the summing ones (setmaxnreg).
+//
+// Two CTAs of a pair share a tile of 256 rows x 256 tokens (cta_group::2): each turns its own 128 weight rows and loads
+// half of the tokens, the even one issues the MMAs for both.  One CTA alone moves 192 KB through its shared memory per
+// 128-channel step (operands written and read), 1.5 times what the 1024 cycles of the MMAs allow; a pair's CTA moves 128.
 //
 // With fewer tiles than SMs the K axis is shared by the CTAs of a cluster: each leaves its sums in its shared memory and
 // every CTA adds up a slice of the tokens from all of them, in rank order, over distributed shared memory.
@@ -39,9 +43,9 @@ constexpr int kLinear = 0, kGated = 1, kDgrad = 2;
 
 constexpr int kMT = 128, kKT = 64;              // rows of a CTA tile, channels of a stage
 constexpr int kABytes = kMT * 128;
-constexpr int kThreads = 512;
-constexpr int kRegsSum = 176, kRegsLoad = 112, kRegsMisc = 48;
-static_assert(2 * kRegsSum + kRegsLoad + kRegsMisc <= 4 * 128, "register shares within the launch's total");
+constexpr int kThreads = 640;
+constexpr int kRegsSum = 168, kRegsLoad = 56, kRegsMisc = 32;
+static_assert(2 * kRegsSum + 2 * kRegsLoad + kRegsMisc <= 5 * 96, "register shares within the launch's total");
 constexpr int kOutBytes = 32 * 128;             // a summing warp's block: 32 tokens x 32 rows, fp32
 constexpr int kRing = 196608;                   // operand stages
 constexpr int kOffOut = kRing;
@@ -80,6 +84,37 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t adesc, uint64
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
         :
         : "r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+        : "memory");
+}
+// the same over a pair: M = 256, each CTA holds its half of A's rows, of B's rows and of the accumulator's lanes
+__device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}"
+        :
+        : "r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u)
+        : "memory");
+}
+// arrives on the barrier at the same place of both CTAs of the pair
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                 "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ uint32_t even_cta(uint32_t addr) {       // the same shared-memory place in the pair's even CTA
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(addr));
+    return a;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// completes on the barrier of the even CTA
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t even_bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            dst),
+        "l"(map), "r"(x), "r"(y), "r"(even_bar)
         : "memory");
 }
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
@@ -157,12 +192,21 @@ __device__ __forceinline__ uint32_t scaled(uint32_t v, __half2 hi, __half2 lo) {
 
 constexpr uint32_t kZeroWord = 0x88888888u;
 
-// Polls without a pause first: the partner is a few hundred cycles away.  Then the bounded wait.
+// Polls without a pause first: the partner is a few hundred cycles away.  Then with pauses, within the time limit.
 __device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
 #pragma unroll 1
     for (int i = 0; i < 64; ++i)
         if (mbar_try_wait(bar, parity)) return true;
-    return mbar_wait(bar, parity, abort_flag);
+    const long long t0 = clock64();
+    while (true) {
+        if (mbar_try_wait(bar, parity)) return true;
+        __nanosleep(64);
+        if (*abort_flag) return false;
+        if (clock64() - t0 > kWaitBudget) {
+            *abort_flag = 1;
+            return false;
+        }
+    }
 }
 
 // Eight neighbouring outputs of token t, columns c .. c + 7 (c a multiple of 8); u: the up projections (gated).
@@ -237,12 +281,14 @@ __device__ __forceinline__ void rows8(uint32_t buf, int token, int row, float (&
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
 
-// T: output type; MODE; CH: channels per chunk (forward: the group size; backward: 512 weight rows); NT: tokens per tile
-template <typename T, int MODE, int CH, int NT>
+// T: output type; MODE; CH: channels per chunk (forward: the group size; backward: 512 weight rows); NT: tokens per tile;
+// PAIR: two CTAs per tile
+template <typename T, int MODE, int CH, int NT, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_constant__ TcParams P,
                                                               const __grid_constant__ CUtensorMap tmap) {
     constexpr bool kBf16 = MODE != kDgrad && std::is_same<T, __nv_bfloat16>::value;
-    constexpr int kBBytes = NT * 128, kStageBytes = kABytes + kBBytes;
+    constexpr int kBRows = PAIR ? NT / 2 : NT;                        // tokens that this CTA loads
+    constexpr int kBBytes = kBRows * 128, kStageBytes = kABytes + kBBytes;
     constexpr int kStages = kRing / kStageBytes < 8 ? kRing / kStageBytes : 8;
     constexpr int kCols = NT / 2;                                     // tokens of a summing warp
     constexpr int kTileCols = MODE == kGated ? 64 : kMT;              // output columns of a tile
@@ -259,31 +305,43 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int s = 0; s < kStages; ++s) {
-            mbar_init(b_full + 8 * s, 1 + 4);      // the TMA issuer and four loading warps
+            mbar_init(b_full + 8 * s, PAIR ? 1 + 8 : 1 + 4);   // the TMA issuer and four loading warps a CTA
             mbar_init(b_empty + 8 * s, 1);
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(b_afull + 8 * a, 1);
-            mbar_init(b_aempty + 8 * a, 8);
+            mbar_init(b_aempty + 8 * a, PAIR ? 16 : 8);
         }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 13) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
-                     "r"(2u * NT) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if (warp == 17) {
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                         "r"(2u * NT) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                         "r"(2u * NT) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     tc_fence_before();
     __syncthreads();
+    if (PAIR) cluster_sync();        // the partner's barriers exist before anything arrives on them
     tc_fence_after();
     const uint32_t tmem_base = *tmem_holder;
 
-    const int rank = P.split > 1 ? (int)(blockIdx.x % P.split) : 0;
+    // PAIR: the cluster is the pair; else the cluster (if any) shares the K axis
+    const int member = (int)(blockIdx.x % (PAIR ? 2 : P.split));
+    const int rank = PAIR ? 0 : member;
     const int st0 = rank * P.per, st1 = min(P.nst, st0 + P.per);      // may be empty
     const int ntiles = P.rt * P.tt;
-    const int tile0 = P.split > 1 ? (int)(blockIdx.x / P.split) : (int)blockIdx.x;
-    const int tile_step = P.split > 1 ? ntiles : (int)gridDim.x;
+    const int tile0 = (int)blockIdx.x / (PAIR ? 2 : P.split);
+    const int tile_step = PAIR ? (int)gridDim.x / 2 : P.split > 1 ? ntiles : (int)gridDim.x;
+    const auto tile_col = [&](int tile) -> int64_t {                  // first output column of this CTA's rows
+        return PAIR ? ((int64_t)(tile % P.rt) * 2 + member) * kTileCols : (int64_t)(tile % P.rt) * kTileCols;
+    };
 
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSum));
@@ -292,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
         uint32_t chunk = 0;
         bool ok = true;
         for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
-            const int64_t t0 = (int64_t)(tile / P.rt) * NT, c0 = (int64_t)(tile % P.rt) * kTileCols;
+            const int64_t t0 = (int64_t)(tile / P.rt) * NT, c0 = tile_col(tile);
             uint64_t acc[kCols / 2];
 #pragma unroll
             for (int i = 0; i < kCols / 2; ++i) acc[i] = 0ull;
@@ -320,19 +378,22 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                 tc_fence_after();
                 const uint64_t sc2 = pack2(__float_as_uint(sc), __float_as_uint(sc));
 #pragma unroll
-                for (int j = 0; j < kCols / 32; ++j) {
-                    uint32_t v[32];
-                    tmem_ld32(tlane + buf * NT + j * 32, v);
+                for (int j = 0; j < kCols / 16; ++j) {
+                    uint32_t v[16];
+                    tmem_ld16(tlane + buf * NT + j * 16, v);
                     tmem_ld_wait();
-                    if (j == kCols / 32 - 1) {      // the accumulator is free once everything is in registers
+                    if (j == kCols / 16 - 1) {      // the accumulator is free once everything is in registers
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(b_aempty + 8 * buf);
+                        if (lane == 0) {
+                            if (PAIR) arrive_cluster(even_cta(b_aempty + 8 * buf));
+                            else mbar_arrive(b_aempty + 8 * buf);
+                        }
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        if constexpr (MODE == kDgrad) acc[j * 16 + i] = add2(acc[j * 16 + i], pack2(v[2 * i], v[2 * i + 1]));
-                        else acc[j * 16 + i] = fma2(pack2(v[2 * i], v[2 * i + 1]), sc2, acc[j * 16 + i]);
+                    for (int i = 0; i < 8; ++i) {
+                        if constexpr (MODE == kDgrad) acc[j * 8 + i] = add2(acc[j * 8 + i], pack2(v[2 * i], v[2 * i + 1]));
+                        else acc[j * 8 + i] = fma2(pack2(v[2 * i], v[2 * i + 1]), sc2, acc[j * 8 + i]);
                     }
                 }
             }
@@ -386,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
         }
         if (P.split > 1) {
             cluster_sync();
-            const int64_t t0 = (int64_t)(tile0 / P.rt) * NT, c0 = (int64_t)(tile0 % P.rt) * kTileCols;
+            const int64_t t0 = (int64_t)(tile0 / P.rt) * NT, c0 = tile_col(tile0);
             const int per = NT / P.split;                             // tokens of this CTA's slice
             constexpr int kGroups = kTileCols / 8;
             for (int i = tid; i < per * kGroups && ok; i += 256) {
@@ -410,19 +471,27 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
             }
             __syncwarp();
         }
-    } else if (warp < 12) {
+    } else if (warp < 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
-        const int lt = tid - 256;                                     // 0..127
-        uint32_t it = 0;
+        const int lt = tid & 127, group = (warp >> 2) & 1;            // groups of four warps take the stages in turn
+        int base = 0;                                                 // stages before this tile
         bool ok = true;
+        const auto publish = [&](uint32_t s) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+                if (PAIR) arrive_cluster(even_cta(b_full + 8 * s));
+                else mbar_arrive(b_full + 8 * s);
+            }
+        };
         if constexpr (MODE != kDgrad) {
             // four lanes share a row of the stage: words 2q, 2q+1 of rows r0 + 32 p
             const int CP = (int)(P.f.C / 8), q = lt & 3, r0 = lt >> 2;
             const uint32_t d0 = (uint32_t)((r0 >> 3) * 1024 + (r0 & 7) * 128), x0 = (uint32_t)(((2 * q) ^ (r0 & 7)) << 4),
                            x1 = (uint32_t)(((2 * q + 1) ^ (r0 & 7)) << 4);
-            constexpr int kAhead = 4;
-            for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
-                const int64_t c0 = (int64_t)(tile % P.rt) * kTileCols;
+            constexpr int kAhead = 2;                                 // stages of this group in registers
+            for (int tile = tile0; tile < ntiles && ok; tile += tile_step, base += st1 - st0) {
+                const int64_t c0 = tile_col(tile);
                 const uint32_t *rp[4];
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
@@ -444,15 +513,16 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                         }
                     }
                 };
+                const int first = st0 + ((group + base) & 1);
 #pragma unroll
                 for (int a = 0; a < kAhead; ++a)
-                    if (st0 + a < st1) fetch(st0 + a, w[a]);
-                for (int stb = st0; stb < st1 && ok; stb += kAhead) {
+                    if (first + 2 * a < st1) fetch(first + 2 * a, w[a]);
+                for (int stb = first; stb < st1 && ok; stb += 2 * kAhead) {
 #pragma unroll
                     for (int a = 0; a < kAhead; ++a) {
-                        const int st = stb + a;
+                        const int st = stb + 2 * a;
                         if (st >= st1) break;
-                        const uint32_t s = it % kStages;
+                        const uint32_t it = (uint32_t)(base + st - st0), s = it % kStages;
                         ok = wait_on(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
                         if (!ok) break;
                         const uint32_t tileb = smem_base + s * kStageBytes + d0;
@@ -461,51 +531,50 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                             sts128(tileb + p * 4096 + x0, word_to_half<kBf16>(w[a][p].x));
                             sts128(tileb + p * 4096 + x1, word_to_half<kBf16>(w[a][p].y));
                         }
-                        fence_proxy_async();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(b_full + 8 * s);
-                        ++it;
-                        if (st + kAhead < st1) fetch(st + kAhead, w[a]);
+                        publish(s);
+                        if (st + 2 * kAhead < st1) fetch(st + 2 * kAhead, w[a]);
                     }
                 }
             }
         } else {
             // words l8 + 8 i of K rows k0 + 16 p: eight lanes read 32 bytes of a row, the 64 channels of block i
-            const int CP = (int)(P.d.C / 8), l8 = lt & 7, k0 = lt >> 3;
-            const int64_t K = (int64_t)P.d.mats * P.d.R;
-            for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
-                const int64_t c0 = (int64_t)(tile % P.rt) * kTileCols;
+            const int CP = (int)(P.d.C / 8), l8 = lt & 7, k0 = lt >> 3, K = (int)(P.d.mats * P.d.R), R = (int)P.d.R;
+            const int G = (int)P.d.G, sh = P.d.gs == 32 ? 5 : P.d.gs == 64 ? 6 : 7;
+            const uint32_t d0 = (uint32_t)((k0 >> 3) * 1024 + (k0 & 7) * 128 + ((l8 ^ (k0 & 7)) << 4));
+            for (int tile = tile0; tile < ntiles && ok; tile += tile_step, base += st1 - st0) {
+                const int c = (int)tile_col(tile) + l8 * 8;           // this lane's channels: c + 64 i
+                const bool in0 = c < (int)P.d.C, in1 = c + 64 < (int)P.d.C;
+                const uint32_t *w0 = P.d.packed[0] + c / 8, *w1 = P.d.mats == 2 ? P.d.packed[1] + c / 8 : w0;
+                const __half2 *sp = P.d.pairs + (c >> sh);
+                const int so = ((c + 64) >> sh) - (c >> sh);
                 uint32_t w[2][4][2];
                 __half2 sc[2][4][2];
                 const auto fetch = [&](int st, uint32_t (&wd)[4][2], __half2 (&sd)[4][2]) {
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
-                        const int64_t k = (int64_t)st * kKT + k0 + 16 * p;
-                        const bool second = k >= P.d.R;
-                        const uint32_t *src = P.d.packed[second ? 1 : 0] + (k - (second ? P.d.R : 0)) * CP;
-                        const __half2 *ss = P.d.pairs + k * P.d.G;
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const int64_t word = c0 / 8 + l8 + 8 * i;
-                            const bool in = k < K && word < CP;
-                            wd[p][i] = in ? __ldg(src + word) : kZeroWord;
-                            sd[p][i] = in ? __ldg(ss + (word * 8) / P.d.gs) : __half2(__ushort_as_half(0), __ushort_as_half(0));
-                        }
+                        const int k = st * kKT + k0 + 16 * p;
+                        const uint32_t *src = (k < R ? w0 : w1) + (int64_t)(k < R ? k : k - R) * CP;
+                        const __half2 *ss = sp + (int64_t)k * G;
+                        const __half2 zero = __half2(__ushort_as_half(0), __ushort_as_half(0));
+                        wd[p][0] = k < K && in0 ? __ldg(src) : kZeroWord;
+                        wd[p][1] = k < K && in1 ? __ldg(src + 8) : kZeroWord;
+                        sd[p][0] = k < K && in0 ? __ldg(ss) : zero;
+                        sd[p][1] = k < K && in1 ? __ldg(ss + so) : zero;
                     }
                 };
+                const int first = st0 + ((group + base) & 1);
 #pragma unroll
                 for (int a = 0; a < 2; ++a)
-                    if (st0 + a < st1) fetch(st0 + a, w[a], sc[a]);
-                for (int stb = st0; stb < st1 && ok; stb += 2) {
+                    if (first + 2 * a < st1) fetch(first + 2 * a, w[a], sc[a]);
+                for (int stb = first; stb < st1 && ok; stb += 4) {
 #pragma unroll
                     for (int a = 0; a < 2; ++a) {
-                        const int st = stb + a;
+                        const int st = stb + 2 * a;
                         if (st >= st1) break;
-                        const uint32_t s = it % kStages;
+                        const uint32_t it = (uint32_t)(base + st - st0), s = it % kStages;
                         ok = wait_on(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
                         if (!ok) break;
-                        const uint32_t tileb = smem_base + s * kStageBytes + (uint32_t)((k0 >> 3) * 1024 + (k0 & 7) * 128 +
-                                                                                       ((l8 ^ (k0 & 7)) << 4));
+                        const uint32_t tileb = smem_base + s * kStageBytes + d0;
 #pragma unroll
                         for (int p = 0; p < 4; ++p)
 #pragma unroll
@@ -515,11 +584,8 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                                 sts128(tileb + i * 8192 + p * 2048,
                                        make_uint4(scaled(v.x, hi, lo), scaled(v.y, hi, lo), scaled(v.z, hi, lo), scaled(v.w, hi, lo)));
                             }
-                        fence_proxy_async();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(b_full + 8 * s);
-                        ++it;
-                        if (st + 2 < st1) fetch(st + 2, w[a], sc[a]);
+                        publish(s);
+                        if (st + 4 < st1) fetch(st + 4, w[a], sc[a]);
                     }
                 }
             }
@@ -528,28 +594,34 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
         if (P.split > 1) cluster_sync();
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMisc));
-        if (warp == 12) {
+        if (warp == 16) {
             // ------------------------------ token tile by TMA ------------------------------
             uint32_t it = 0;
             bool ok = true;
             if (lane == 0) {
                 for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
-                    const int t0 = (tile / P.rt) * NT;
+                    const int t0 = (tile / P.rt) * NT + (PAIR ? member * kBRows : 0);
                     for (int st = st0; st < st1; ++st, ++it) {
                         const uint32_t s = it % kStages;
                         ok = wait_on(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
                         if (!ok) break;
-                        mbar_arrive_expect_tx(b_full + 8 * s, kBBytes);
-                        tma_load_2d(smem_base + s * kStageBytes + kABytes, &tmap, st * kKT, t0, b_full + 8 * s);
+                        const uint32_t dst = smem_base + s * kStageBytes + kABytes;
+                        if constexpr (PAIR) {
+                            if (member == 0) mbar_arrive_expect_tx(b_full + 8 * s, 2 * kBBytes);
+                            tma_load_2d_pair(dst, &tmap, st * kKT, t0, even_cta(b_full + 8 * s));
+                        } else {
+                            mbar_arrive_expect_tx(b_full + 8 * s, kBBytes);
+                            tma_load_2d(dst, &tmap, st * kKT, t0, b_full + 8 * s);
+                        }
                     }
                 }
             }
-        } else if (warp == 13) {
+        } else if (warp == 17) {
             // ------------------------------ MMA issuer ------------------------------
             uint32_t it = 0, chunk = 0;
             bool ok = true;
             constexpr int kStepsPer = (CH < kKT ? CH : kKT) / 16;     // k-steps of a chunk inside a stage
-            if (lane == 0) {
+            if (lane == 0 && (!PAIR || member == 0)) {
                 for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
                     for (int st = st0; st < st1 && ok; ++st, ++it) {
                         const uint32_t s = it % kStages;
@@ -567,16 +639,20 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                                 if (!ok) break;
                                 tc_fence_after();
                             }
-                            umma_f16(tmem_base + (chunk & 1u) * NT,
-                                     MODE == kDgrad ? desc_mnmajor(abase + kk * 2048) : desc_kmajor(abase + kk * 32),
-                                     desc_kmajor(bbase + kk * 32), idesc<MODE, kBf16>(kMT, NT), starts ? 0u : 1u);
+                            const uint32_t d = tmem_base + (chunk & 1u) * NT;
+                            const uint64_t ad = MODE == kDgrad ? desc_mnmajor(abase + kk * 2048) : desc_kmajor(abase + kk * 32);
+                            const uint64_t bd = desc_kmajor(bbase + kk * 32);
+                            if constexpr (PAIR) umma_f16_pair(d, ad, bd, idesc<MODE, kBf16>(2 * kMT, NT), starts ? 0u : 1u);
+                            else umma_f16(d, ad, bd, idesc<MODE, kBf16>(kMT, NT), starts ? 0u : 1u);
                             if (kk % kStepsPer == kStepsPer - 1 && last_stage) {
-                                umma_commit(b_afull + 8 * (chunk & 1u));
+                                if (PAIR) umma_commit_pair(b_afull + 8 * (chunk & 1u));
+                                else umma_commit(b_afull + 8 * (chunk & 1u));
                                 ++chunk;
                             }
                         }
                         if (!ok) break;
-                        umma_commit(b_empty + 8 * s);
+                        if (PAIR) umma_commit_pair(b_empty + 8 * s);
+                        else umma_commit(b_empty + 8 * s);
                     }
                 }
             }
@@ -585,9 +661,9 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
         if (P.split > 1) cluster_sync();
     }
     // ------------------------------ teardown ------------------------------
-    if (P.split > 1) {
+    if (PAIR || P.split > 1) {
         __syncwarp();
-        cluster_sync();          // nobody leaves while its sums are being read
+        cluster_sync();          // nobody leaves while its sums or operands are being read, or its barriers arrived on
     }
     tc_fence_before();
     __syncthreads();
@@ -597,9 +673,12 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
         if (tid == 0 && P.status) atomicExch(P.status, FORGE_ERR_TIMEOUT);
         __syncthreads();
     }
-    if (warp == 13) {
+    if (warp == 17) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2u * NT) : "memory");
+        if constexpr (PAIR)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2u * NT) : "memory");
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2u * NT) : "memory");
     }
 }
 
@@ -635,18 +714,18 @@ struct TokenSource {
     int64_t rows, cols, ld;
 };
 
-template <typename T, int MODE, int CH, int NT>
+template <typename T, int MODE, int CH, int NT, bool PAIR>
 int launch(TcParams &P, const TokenSource &src, const char *who, cudaStream_t st) {
     int dev = 0, sms = 148;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    const int64_t rt = cdiv(P.N, (int64_t)(MODE == kGated ? 64 : kMT)), tt = cdiv(P.T, (int64_t)NT), tiles = rt * tt;
+    const int64_t rt = cdiv(P.N, (int64_t)(MODE == kGated ? 64 : kMT) * (PAIR ? 2 : 1)), tt = cdiv(P.T, (int64_t)NT), tiles = rt * tt;
     if (tiles > 0x0fffffff) {
         set_error("%s: more than 2^28 output tiles", who);
         return FORGE_ERR_UNSUPPORTED;
     }
     alignas(64) CUtensorMap map;
-    if (!make_map(&map, src.base, src.bf16, src.rows, src.cols, src.ld, NT)) {
+    if (!make_map(&map, src.base, src.bf16, src.rows, src.cols, src.ld, PAIR ? NT / 2 : NT)) {
         set_error("%s: no tensor map could be made", who);
         return FORGE_ERR_LAUNCH;
     }
@@ -654,19 +733,19 @@ int launch(TcParams &P, const TokenSource &src, const char *who, cudaStream_t st
     P.tt = (int)tt;
     const int units = (P.nst + 1) / 2;                                 // 128-wide pieces of K
     P.split = 1;
-    while (P.split < 8 && tiles * P.split * 2 <= sms && units >= P.split * 4) P.split *= 2;
+    while (!PAIR && P.split < 8 && tiles * P.split * 2 <= sms && units >= P.split * 4) P.split *= 2;
     P.per = (units + P.split - 1) / P.split * 2;
-    const auto kernel = int4_tc_kernel<T, MODE, CH, NT>;
+    const auto kernel = int4_tc_kernel<T, MODE, CH, NT, PAIR>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
     if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3((unsigned)(P.split > 1 ? tiles * P.split : imin64(tiles, sms)));
+        cfg.gridDim = dim3((unsigned)(PAIR ? 2 * imin64(tiles, sms / 2) : P.split > 1 ? tiles * P.split : imin64(tiles, sms)));
         cfg.blockDim = dim3(kThreads);
         cfg.dynamicSmemBytes = kSmemBytes;
         cfg.stream = st;
         cudaLaunchAttribute at{};
         at.id = cudaLaunchAttributeClusterDimension;
-        at.val.clusterDim.x = (unsigned)P.split;
+        at.val.clusterDim.x = (unsigned)(PAIR ? 2 : P.split);
         at.val.clusterDim.y = at.val.clusterDim.z = 1;
         cfg.attrs = &at;
         cfg.numAttrs = 1;
@@ -680,10 +759,13 @@ int launch(TcParams &P, const TokenSource &src, const char *who, cudaStream_t st
     FORGE_NOTE_LAUNCH();
     return FORGE_OK;
 }
-// token tiles of 64 when one or two of them cover all tokens, else of 256
+// Token tiles of 64 when one or two of them cover all tokens, else of 256; pairs as soon as their tiles keep more than half
+// of the SMs busy (below that, sharing the K axis among more CTAs counts for more).
 template <typename T, int MODE, int CH> int launch_nt(TcParams &P, const TokenSource &src, const char *who, cudaStream_t st) {
-    if (P.T <= 128) return launch<T, MODE, CH, 64>(P, src, who, st);
-    return launch<T, MODE, CH, 256>(P, src, who, st);
+    if (P.T <= 128) return launch<T, MODE, CH, 64, false>(P, src, who, st);
+    const int64_t tiles = cdiv(P.N, (int64_t)(MODE == kGated ? 64 : kMT)) * cdiv(P.T, (int64_t)256);
+    if (tiles > 74) return launch<T, MODE, CH, 256, true>(P, src, who, st);
+    return launch<T, MODE, CH, 256, false>(P, src, who, st);
 }
 template <typename T, int MODE> int launch_gs(TcParams &P, const TokenSource &src, const char *who, cudaStream_t st) {
     if (P.f.gs == 32) return launch_nt<T, MODE, 32>(P, src, who, st);
