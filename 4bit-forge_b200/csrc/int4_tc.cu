@@ -17,7 +17,7 @@
 // A CTA (one per SM, 640 threads): warps 0-7 add finished chunks to the sums and run the epilogue, warps 8-11 and 12-15
 // turn packed words into 16-bit operand tiles, one stage each in turn (words read ahead into registers, tiles written with
 // the 128-byte swizzle), warp 16 brings the token tile in with TMA, warp 17 owns tensor memory and issues the MMAs.  Stages
-// of 64 channels, two accumulators.  Registers move from the loading warps to the summing ones (setmaxnreg).
+// of 128 channels, two accumulators.  Registers move from the loading warps to the summing ones (setmaxnreg).
 //
 // Two CTAs of a pair share a tile of 256 rows x 256 tokens (cta_group::2): each turns its own 128 weight rows and loads
 // half of the tokens, the even one issues the MMAs for both.  One CTA alone moves 192 KB through its shared memory per
@@ -41,10 +41,10 @@ namespace {
 
 constexpr int kLinear = 0, kGated = 1, kDgrad = 2;
 
-constexpr int kMT = 128, kKT = 64;              // rows of a CTA tile, channels of a stage
-constexpr int kABytes = kMT * 128;
+constexpr int kMT = 128, kKT = 128;             // rows of a CTA tile, channels of a stage
+constexpr int kSubA = kMT * 128, kABytes = 2 * kSubA;   // K-major: two sub-tiles of 64 channels (128 bytes a row)
 constexpr int kThreads = 640;
-constexpr int kRegsSum = 168, kRegsLoad = 56, kRegsMisc = 32;
+constexpr int kRegsSum = 160, kRegsLoad = 56, kRegsMisc = 48;
 static_assert(2 * kRegsSum + 2 * kRegsLoad + kRegsMisc <= 5 * 96, "register shares within the launch's total");
 constexpr int kOutBytes = 32 * 128;             // a summing warp's block: 32 tokens x 32 rows, fp32
 constexpr int kRing = 196608;                   // operand stages
@@ -57,9 +57,10 @@ struct TcParams {
     Int4Dgrad d;
     int64_t T, N;        // token rows, output columns (weight rows; channels in the backward form)
     int rt, tt;          // row tiles, token tiles
-    int nst;             // 64-wide k stages in all
-    int split, per;      // cluster size along K, stages per member (a multiple of 2)
+    int nst;             // k stages in all
+    int split, per;      // cluster size along K, stages per member
     bool res_vec;        // residual rows start on 16 bytes
+    bool simple;         // linear: no bias, activation or pre-activation, and 16-byte rows throughout
     int32_t *status;
 };
 
@@ -67,9 +68,9 @@ struct TcParams {
 __device__ __forceinline__ uint64_t desc_kmajor(uint32_t saddr) {
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-// MN-major operand, 128-byte swizzle: blocks of 64 MN elements x 64 K rows, 8 KB apart; groups of 8 K rows 1 KB apart
+// MN-major operand, 128-byte swizzle: blocks of 64 MN elements x 128 K rows, 16 KB apart; groups of 8 K rows 1 KB apart
 __device__ __forceinline__ uint64_t desc_mnmajor(uint32_t saddr) {
-    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(8192 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(16384 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
            (2ull << 61);
 }
 // D fp32, A and B both bf16 or both fp16; the backward form's A is MN-major
@@ -192,6 +193,11 @@ __device__ __forceinline__ uint32_t scaled(uint32_t v, __half2 hi, __half2 lo) {
 
 constexpr uint32_t kZeroWord = 0x88888888u;
 
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
 // Polls without a pause first: the partner is a few hundred cycles away.  Then with pauses, within the time limit.
 __device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
 #pragma unroll 1
@@ -288,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                                                               const __grid_constant__ CUtensorMap tmap) {
     constexpr bool kBf16 = MODE != kDgrad && std::is_same<T, __nv_bfloat16>::value;
     constexpr int kBRows = PAIR ? NT / 2 : NT;                        // tokens that this CTA loads
-    constexpr int kBBytes = kBRows * 128, kStageBytes = kABytes + kBBytes;
+    constexpr int kSubB = kBRows * 128, kBBytes = 2 * kSubB, kStageBytes = kABytes + kBBytes;
     constexpr int kStages = kRing / kStageBytes < 8 ? kRing / kStageBytes : 8;
     constexpr int kCols = NT / 2;                                     // tokens of a summing warp
     constexpr int kTileCols = MODE == kGated ? 64 : kMT;              // output columns of a tile
@@ -405,6 +411,24 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                 for (int j = 0; j < kCols / 32; ++j) {
                     const int64_t tb = t0 + half * kCols + j * 32;
                     if (tb >= P.T) break;
+                    // what the outputs need from memory is requested before the block goes through shared memory
+                    const int64_t cl = c0 + quarter * 32 + (lane & 3) * 8;
+                    const bool simple = MODE == kDgrad || (MODE == kLinear && P.simple);
+                    uint4 rv[4];
+                    float us[4];
+                    if (MODE == kLinear && simple && P.f.res)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int64_t t = tb + k * 8 + (lane >> 2);
+                            rv[k] = t < P.T && cl < P.N ? __ldg(reinterpret_cast<const uint4 *>((const T *)P.f.res + t * P.f.ldres + cl))
+                                                        : make_uint4(0u, 0u, 0u, 0u);
+                        }
+                    if (MODE == kDgrad)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int64_t t = tb + k * 8 + (lane >> 2);
+                            us[k] = t < P.T ? __ldg(P.d.unscale + t) : 0.0f;
+                        }
                     __syncwarp();
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
@@ -415,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                     }
                     __syncwarp();
                     if constexpr (MODE == kGated) {
-#pragma unroll 1
+#pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             const int tok = k * 16 + (lane >> 1), p = (lane & 1) * 8;
                             float z[8], u[8];
@@ -423,13 +447,30 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                             rows8(buf, tok, 16 + p, u);
                             emit8<T, MODE>(P, tb + tok, c0 + quarter * 16 + p, z, u);
                         }
+                    } else if (simple) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int tok = k * 8 + (lane >> 2);
+                            const int64_t t = tb + tok;
+                            float z[8];
+                            rows8(buf, tok, (lane & 3) * 8, z);
+                            if constexpr (MODE == kDgrad) {
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) z[i] *= us[k];
+                            } else if (P.f.res) {
+                                const T *e = reinterpret_cast<const T *>(&rv[k]);
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) z[i] += Elem<T>::to_f(e[i]);
+                            }
+                            if (t < P.T && cl < P.N) store8((T *)(MODE == kDgrad ? P.d.dx : P.f.y) + t * P.N + cl, z);
+                        }
                     } else {
 #pragma unroll 1
                         for (int k = 0; k < 4; ++k) {
-                            const int tok = k * 8 + (lane >> 2), p = (lane & 3) * 8;
+                            const int tok = k * 8 + (lane >> 2);
                             float z[8];
-                            rows8(buf, tok, p, z);
-                            emit8<T, MODE>(P, tb + tok, c0 + quarter * 32 + p, z, z);
+                            rows8(buf, tok, (lane & 3) * 8, z);
+                            emit8<T, MODE>(P, tb + tok, cl, z, z);
                         }
                     }
                 }
@@ -489,7 +530,6 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
             const int CP = (int)(P.f.C / 8), q = lt & 3, r0 = lt >> 2;
             const uint32_t d0 = (uint32_t)((r0 >> 3) * 1024 + (r0 & 7) * 128), x0 = (uint32_t)(((2 * q) ^ (r0 & 7)) << 4),
                            x1 = (uint32_t)(((2 * q + 1) ^ (r0 & 7)) << 4);
-            constexpr int kAhead = 2;                                 // stages of this group in registers
             for (int tile = tile0; tile < ntiles && ok; tile += tile_step, base += st1 - st0) {
                 const int64_t c0 = tile_col(tile);
                 const uint32_t *rp[4];
@@ -499,45 +539,40 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                     row = row < P.f.R ? row : P.f.R - 1;              // rows past the matrix: computed, never stored
                     rp[p] = P.f.packed[MODE == kGated && r0 >= 16 ? 1 : 0] + row * CP + 2 * q;
                 }
-                uint2 w[kAhead][4];
-                const auto fetch = [&](int st, uint2 (&d)[4]) {
-                    const int word = st * 8 + 2 * q;
-                    if (P.f.vec8 && st * 8 + 8 <= CP) {
+                uint2 w[8];                                           // [sub-tile][row]
+                const auto fetch = [&](int st) {
+                    const int word = st * 16;
+                    if (P.f.vec8 && word + 16 <= CP) {
 #pragma unroll
-                        for (int p = 0; p < 4; ++p) d[p] = __ldg(reinterpret_cast<const uint2 *>(rp[p] + st * 8));
+                        for (int p = 0; p < 8; ++p) w[p] = __ldg(reinterpret_cast<const uint2 *>(rp[p & 3] + word + (p >> 2) * 8));
                     } else {
 #pragma unroll
-                        for (int p = 0; p < 4; ++p) {
-                            d[p].x = word < CP ? __ldg(rp[p] + st * 8) : kZeroWord;
-                            d[p].y = word + 1 < CP ? __ldg(rp[p] + st * 8 + 1) : kZeroWord;
+                        for (int p = 0; p < 8; ++p) {
+                            const int j = word + (p >> 2) * 8 + 2 * q;
+                            w[p].x = j < CP ? __ldg(rp[p & 3] + word + (p >> 2) * 8) : kZeroWord;
+                            w[p].y = j + 1 < CP ? __ldg(rp[p & 3] + word + (p >> 2) * 8 + 1) : kZeroWord;
                         }
                     }
                 };
                 const int first = st0 + ((group + base) & 1);
+                if (first < st1) fetch(first);
+                for (int st = first; st < st1; st += 2) {
+                    const uint32_t it = (uint32_t)(base + st - st0), s = it % kStages;
+                    ok = wait_on(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
+                    if (!ok) break;
+                    const uint32_t tileb = smem_base + s * kStageBytes + d0;
 #pragma unroll
-                for (int a = 0; a < kAhead; ++a)
-                    if (first + 2 * a < st1) fetch(first + 2 * a, w[a]);
-                for (int stb = first; stb < st1 && ok; stb += 2 * kAhead) {
-#pragma unroll
-                    for (int a = 0; a < kAhead; ++a) {
-                        const int st = stb + 2 * a;
-                        if (st >= st1) break;
-                        const uint32_t it = (uint32_t)(base + st - st0), s = it % kStages;
-                        ok = wait_on(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
-                        if (!ok) break;
-                        const uint32_t tileb = smem_base + s * kStageBytes + d0;
-#pragma unroll
-                        for (int p = 0; p < 4; ++p) {
-                            sts128(tileb + p * 4096 + x0, word_to_half<kBf16>(w[a][p].x));
-                            sts128(tileb + p * 4096 + x1, word_to_half<kBf16>(w[a][p].y));
-                        }
-                        publish(s);
-                        if (st + 2 * kAhead < st1) fetch(st + 2 * kAhead, w[a]);
+                    for (int p = 0; p < 8; ++p) {
+                        sts128(tileb + (p >> 2) * kSubA + (p & 3) * 4096 + x0, word_to_half<kBf16>(w[p].x));
+                        sts128(tileb + (p >> 2) * kSubA + (p & 3) * 4096 + x1, word_to_half<kBf16>(w[p].y));
                     }
+                    publish(s);
+                    if (st + 2 < st1) fetch(st + 2);
                 }
             }
         } else {
-            // words l8 + 8 i of K rows k0 + 16 p: eight lanes read 32 bytes of a row, the 64 channels of block i
+            // words l8 + 8 i of K rows k0 + 16 p (p < 8, four at a time): eight lanes read 32 bytes of a row, the 64 channels
+            // of block i
             const int CP = (int)(P.d.C / 8), l8 = lt & 7, k0 = lt >> 3, K = (int)(P.d.mats * P.d.R), R = (int)P.d.R;
             const int G = (int)P.d.G, sh = P.d.gs == 32 ? 5 : P.d.gs == 64 ? 6 : 7;
             const uint32_t d0 = (uint32_t)((k0 >> 3) * 1024 + (k0 & 7) * 128 + ((l8 ^ (k0 & 7)) << 4));
@@ -547,46 +582,43 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                 const uint32_t *w0 = P.d.packed[0] + c / 8, *w1 = P.d.mats == 2 ? P.d.packed[1] + c / 8 : w0;
                 const __half2 *sp = P.d.pairs + (c >> sh);
                 const int so = ((c + 64) >> sh) - (c >> sh);
-                uint32_t w[2][4][2];
-                __half2 sc[2][4][2];
-                const auto fetch = [&](int st, uint32_t (&wd)[4][2], __half2 (&sd)[4][2]) {
+                uint32_t w[4][2];
+                __half2 sc[4][2];
+                const auto fetch = [&](int k1) {
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
-                        const int k = st * kKT + k0 + 16 * p;
+                        const int k = k1 + k0 + 16 * p;
                         const uint32_t *src = (k < R ? w0 : w1) + (int64_t)(k < R ? k : k - R) * CP;
                         const __half2 *ss = sp + (int64_t)k * G;
                         const __half2 zero = __half2(__ushort_as_half(0), __ushort_as_half(0));
-                        wd[p][0] = k < K && in0 ? __ldg(src) : kZeroWord;
-                        wd[p][1] = k < K && in1 ? __ldg(src + 8) : kZeroWord;
-                        sd[p][0] = k < K && in0 ? __ldg(ss) : zero;
-                        sd[p][1] = k < K && in1 ? __ldg(ss + so) : zero;
+                        w[p][0] = k < K && in0 ? __ldg(src) : kZeroWord;
+                        w[p][1] = k < K && in1 ? __ldg(src + 8) : kZeroWord;
+                        sc[p][0] = k < K && in0 ? __ldg(ss) : zero;
+                        sc[p][1] = k < K && in1 ? __ldg(ss + so) : zero;
                     }
                 };
                 const int first = st0 + ((group + base) & 1);
-#pragma unroll
-                for (int a = 0; a < 2; ++a)
-                    if (first + 2 * a < st1) fetch(first + 2 * a, w[a], sc[a]);
-                for (int stb = first; stb < st1 && ok; stb += 4) {
-#pragma unroll
-                    for (int a = 0; a < 2; ++a) {
-                        const int st = stb + 2 * a;
-                        if (st >= st1) break;
-                        const uint32_t it = (uint32_t)(base + st - st0), s = it % kStages;
-                        ok = wait_on(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
-                        if (!ok) break;
-                        const uint32_t tileb = smem_base + s * kStageBytes + d0;
+                if (first < st1) fetch(first * kKT);
+                for (int st = first; st < st1; st += 2) {
+                    const uint32_t it = (uint32_t)(base + st - st0), s = it % kStages;
+                    ok = wait_on(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
+                    if (!ok) break;
+#pragma unroll 1
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t tileb = smem_base + s * kStageBytes + h * 8192 + d0;
 #pragma unroll
                         for (int p = 0; p < 4; ++p)
 #pragma unroll
                             for (int i = 0; i < 2; ++i) {
-                                const uint4 v = word_to_half<false>(w[a][p][i]);
-                                const __half2 hi = __low2half2(sc[a][p][i]), lo = __high2half2(sc[a][p][i]);
-                                sts128(tileb + i * 8192 + p * 2048,
+                                const uint4 v = word_to_half<false>(w[p][i]);
+                                const __half2 hi = __low2half2(sc[p][i]), lo = __high2half2(sc[p][i]);
+                                sts128(tileb + i * 16384 + p * 2048,
                                        make_uint4(scaled(v.x, hi, lo), scaled(v.y, hi, lo), scaled(v.z, hi, lo), scaled(v.w, hi, lo)));
                             }
-                        publish(s);
-                        if (st + 4 < st1) fetch(st + 4, w[a], sc[a]);
+                        if (h == 0) fetch(st * kKT + 64);
                     }
+                    publish(s);
+                    if (st + 2 < st1) fetch((st + 2) * kKT);
                 }
             }
         }
@@ -609,51 +641,65 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                         if constexpr (PAIR) {
                             if (member == 0) mbar_arrive_expect_tx(b_full + 8 * s, 2 * kBBytes);
                             tma_load_2d_pair(dst, &tmap, st * kKT, t0, even_cta(b_full + 8 * s));
+                            tma_load_2d_pair(dst + kSubB, &tmap, st * kKT + 64, t0, even_cta(b_full + 8 * s));
                         } else {
                             mbar_arrive_expect_tx(b_full + 8 * s, kBBytes);
                             tma_load_2d(dst, &tmap, st * kKT, t0, b_full + 8 * s);
+                            tma_load_2d(dst + kSubB, &tmap, st * kKT + 64, t0, b_full + 8 * s);
                         }
                     }
                 }
             }
         } else if (warp == 17) {
             // ------------------------------ MMA issuer ------------------------------
-            uint32_t it = 0, chunk = 0;
-            bool ok = true;
+            // the whole warp walks the loop and one elected lane issues, so addresses and descriptors stay uniform
+            uint32_t s = 0, phase = 0, chunk = 0;
+            bool ok = !PAIR || member == 0;
             constexpr int kStepsPer = (CH < kKT ? CH : kKT) / 16;     // k-steps of a chunk inside a stage
-            if (lane == 0 && (!PAIR || member == 0)) {
-                for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
-                    for (int st = st0; st < st1 && ok; ++st, ++it) {
-                        const uint32_t s = it % kStages;
-                        ok = wait_on(b_full + 8 * s, (it / kStages) & 1u, abort_flag);
-                        if (!ok) break;
-                        tc_fence_after();
-                        const uint32_t abase = smem_base + s * kStageBytes, bbase = abase + kABytes;
-                        const bool first_stage = (st - st0) % kStagesPer == 0;
-                        const bool last_stage = (st - st0) % kStagesPer == kStagesPer - 1 || st + 1 == st1;
+            const uint64_t ad0 = MODE == kDgrad ? desc_mnmajor(smem_base) : desc_kmajor(smem_base);
+            const uint64_t bd0 = desc_kmajor(smem_base + kABytes);
+            for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
+                for (int st = st0; st < st1; ++st) {
+                    ok = wait_on(b_full + 8 * s, phase, abort_flag);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const bool first_stage = (st - st0) % kStagesPer == 0;
+                    const bool last_stage = (st - st0) % kStagesPer == kStagesPer - 1 || st + 1 == st1;
+                    const uint64_t ad = ad0 + (uint64_t)(s * (kStageBytes >> 4)), bd = bd0 + (uint64_t)(s * (kStageBytes >> 4));
 #pragma unroll
-                        for (int kk = 0; kk < kKT / 16; ++kk) {
-                            const bool starts = kk % kStepsPer == 0 && first_stage;
-                            if (starts) {
-                                ok = wait_on(b_aempty + 8 * (chunk & 1u), ((chunk >> 1) & 1u) ^ 1u, abort_flag);
-                                if (!ok) break;
-                                tc_fence_after();
-                            }
+                    for (int e = 0; e < kPerStage; ++e) {
+                        if (first_stage) {
+                            ok = wait_on(b_aempty + 8 * (chunk & 1u), ((chunk >> 1) & 1u) ^ 1u, abort_flag);
+                            ok = __all_sync(0xffffffffu, ok);
+                            if (!ok) break;
+                            tc_fence_after();
+                        }
+                        if (elect_one()) {
                             const uint32_t d = tmem_base + (chunk & 1u) * NT;
-                            const uint64_t ad = MODE == kDgrad ? desc_mnmajor(abase + kk * 2048) : desc_kmajor(abase + kk * 32);
-                            const uint64_t bd = desc_kmajor(bbase + kk * 32);
-                            if constexpr (PAIR) umma_f16_pair(d, ad, bd, idesc<MODE, kBf16>(2 * kMT, NT), starts ? 0u : 1u);
-                            else umma_f16(d, ad, bd, idesc<MODE, kBf16>(kMT, NT), starts ? 0u : 1u);
-                            if (kk % kStepsPer == kStepsPer - 1 && last_stage) {
+#pragma unroll
+                            for (int i = 0; i < kStepsPer; ++i) {
+                                const int kk = e * kStepsPer + i;
+                                const uint64_t a = ad + (MODE == kDgrad ? kk * 2048 : (kk >> 2) * kSubA + (kk & 3) * 32) / 16;
+                                const uint64_t bb = bd + ((kk >> 2) * kSubB + (kk & 3) * 32) / 16;
+                                const uint32_t more = (i == 0 && first_stage) ? 0u : 1u;
+                                if constexpr (PAIR) umma_f16_pair(d, a, bb, idesc<MODE, kBf16>(2 * kMT, NT), more);
+                                else umma_f16(d, a, bb, idesc<MODE, kBf16>(kMT, NT), more);
+                            }
+                            if (last_stage) {
                                 if (PAIR) umma_commit_pair(b_afull + 8 * (chunk & 1u));
                                 else umma_commit(b_afull + 8 * (chunk & 1u));
-                                ++chunk;
+                            }
+                            if (e == kPerStage - 1) {
+                                if (PAIR) umma_commit_pair(b_empty + 8 * s);
+                                else umma_commit(b_empty + 8 * s);
                             }
                         }
-                        if (!ok) break;
-                        if (PAIR) umma_commit_pair(b_empty + 8 * s);
-                        else umma_commit(b_empty + 8 * s);
+                        __syncwarp();
+                        if (last_stage) ++chunk;
                     }
+                    if (!ok) break;
+                    if (++s == kStages) { s = 0; phase ^= 1u; }
                 }
             }
         }
@@ -702,7 +748,7 @@ bool make_map(CUtensorMap *m, const void *base, bool bf16, int64_t rows, int64_t
     EncodeFn fn = encode_fn();
     if (!fn) return false;
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
-    const cuuint32_t box[2] = {kKT, (cuuint32_t)box_rows}, es[2] = {1, 1};
+    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, es[2] = {1, 1};
     return fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(base), dims,
               strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -731,10 +777,9 @@ int launch(TcParams &P, const TokenSource &src, const char *who, cudaStream_t st
     }
     P.rt = (int)rt;
     P.tt = (int)tt;
-    const int units = (P.nst + 1) / 2;                                 // 128-wide pieces of K
     P.split = 1;
-    while (!PAIR && P.split < 8 && tiles * P.split * 2 <= sms && units >= P.split * 4) P.split *= 2;
-    P.per = (units + P.split - 1) / P.split * 2;
+    while (!PAIR && P.split < 8 && tiles * P.split * 2 <= sms && P.nst >= P.split * 4) P.split *= 2;
+    P.per = (P.nst + P.split - 1) / P.split;
     const auto kernel = int4_tc_kernel<T, MODE, CH, NT, PAIR>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
     if (e == cudaSuccess) {
@@ -759,13 +804,13 @@ int launch(TcParams &P, const TokenSource &src, const char *who, cudaStream_t st
     FORGE_NOTE_LAUNCH();
     return FORGE_OK;
 }
-// Token tiles of 64 when one or two of them cover all tokens, else of 256; pairs as soon as their tiles keep more than half
-// of the SMs busy (below that, sharing the K axis among more CTAs counts for more).
+// Token tiles of 64 or 128 for one CTA; pairs with 256 as soon as their tiles keep more than half of the SMs busy (below
+// that, sharing the K axis among more CTAs counts for more).
 template <typename T, int MODE, int CH> int launch_nt(TcParams &P, const TokenSource &src, const char *who, cudaStream_t st) {
-    if (P.T <= 128) return launch<T, MODE, CH, 64, false>(P, src, who, st);
-    const int64_t tiles = cdiv(P.N, (int64_t)(MODE == kGated ? 64 : kMT)) * cdiv(P.T, (int64_t)256);
-    if (tiles > 74) return launch<T, MODE, CH, 256, true>(P, src, who, st);
-    return launch<T, MODE, CH, 256, false>(P, src, who, st);
+    if (P.T <= 64) return launch<T, MODE, CH, 64, false>(P, src, who, st);
+    const int64_t pairs = cdiv(P.N, (int64_t)(MODE == kGated ? 128 : 2 * kMT)) * cdiv(P.T, (int64_t)256);
+    if (pairs > 37) return launch<T, MODE, CH, 256, true>(P, src, who, st);
+    return launch<T, MODE, CH, 128, false>(P, src, who, st);
 }
 template <typename T, int MODE> int launch_gs(TcParams &P, const TokenSource &src, const char *who, cudaStream_t st) {
     if (P.f.gs == 32) return launch_nt<T, MODE, 32>(P, src, who, st);
@@ -783,6 +828,7 @@ int int4_fwd_tc(const Int4Fwd &F, bool bf16, bool gated, cudaStream_t st) {
     P.f = F; P.T = F.T; P.N = F.R; P.status = F.status;
     P.nst = (int)cdiv(F.C, (int64_t)kKT);
     P.res_vec = F.ldres % 8 == 0 && (uintptr_t)F.res % 16 == 0;
+    P.simple = !F.bias && !F.pre0 && F.act == FORGE_ACT_NONE && F.R % 8 == 0 && (!F.res || P.res_vec);
     const TokenSource src{F.x, bf16, F.T, F.C, F.ldx};
     if (bf16) return gated ? launch_gs<__nv_bfloat16, kGated>(P, src, who, st) : launch_gs<__nv_bfloat16, kLinear>(P, src, who, st);
     return gated ? launch_gs<__half, kGated>(P, src, who, st) : launch_gs<__half, kLinear>(P, src, who, st);
@@ -791,7 +837,7 @@ int int4_fwd_tc(const Int4Fwd &F, bool bf16, bool gated, cudaStream_t st) {
 int int4_dgrad_tc(const Int4Dgrad &D, bool bf16, const char *who, cudaStream_t st) {
     TcParams P{};
     P.d = D; P.T = D.T; P.N = D.C; P.status = D.status;
-    P.nst = (int)(D.ldk / kKT);
+    P.nst = (int)cdiv(D.ldk, (int64_t)kKT);
     const TokenSource src{D.a, false, D.T, D.ldk, D.ldk};
     return bf16 ? launch_nt<__nv_bfloat16, kDgrad, 512>(P, src, who, st) : launch_nt<__half, kDgrad, 512>(P, src, who, st);
 }
