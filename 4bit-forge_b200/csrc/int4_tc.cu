@@ -44,8 +44,14 @@ constexpr int kLinear = 0, kGated = 1, kDgrad = 2;
 constexpr int kMT = 128, kKT = 128;             // rows of a CTA tile, channels of a stage
 constexpr int kSubA = kMT * 128, kABytes = 2 * kSubA;   // K-major: two sub-tiles of 64 channels (128 bytes a row)
 constexpr int kThreads = 640;
-constexpr int kRegsSum = 160, kRegsLoad = 56, kRegsMisc = 48;
-static_assert(2 * kRegsSum + 2 * kRegsLoad + kRegsMisc <= 5 * 96, "register shares within the launch's total");
+// Registers a thread of the summing, loading and other warps, out of 5 x 96: what each form needs so that its inner loops
+// keep everything in registers.  (The 4096 x 2048 -> 7168 product took 130 us with 176 for the sums and 190 with 160; the
+// gated 8192 x 7168 -> 2048 one 371 us with 64 for the loads and 454 with 48.)
+template <int MODE> struct Regs {
+    static constexpr int kSum = MODE == kLinear ? 176 : MODE == kGated ? 160 : 152;
+    static constexpr int kLoad = MODE == kLinear ? 48 : MODE == kGated ? 64 : 72, kMisc = 32;
+    static_assert(2 * kSum + 2 * kLoad + kMisc <= 5 * 96, "register shares within the launch's total");
+};
 constexpr int kOutBytes = 32 * 128;             // a summing warp's block: 32 tokens x 32 rows, fp32
 constexpr int kRing = 196608;                   // operand stages
 constexpr int kOffOut = kRing;
@@ -345,38 +351,45 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
     const int ntiles = P.rt * P.tt;
     const int tile0 = (int)blockIdx.x / (PAIR ? 2 : P.split);
     const int tile_step = PAIR ? (int)gridDim.x / 2 : P.split > 1 ? ntiles : (int)gridDim.x;
-    const auto tile_col = [&](int tile) -> int64_t {                  // first output column of this CTA's rows
-        return PAIR ? ((int64_t)(tile % P.rt) * 2 + member) * kTileCols : (int64_t)(tile % P.rt) * kTileCols;
+    const auto tile_col = [&](int tile) -> int {                      // first output column of this CTA's rows
+        return PAIR ? ((tile % P.rt) * 2 + member) * kTileCols : (tile % P.rt) * kTileCols;
     };
 
     if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSum));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Regs<MODE>::kSum));
         const int quarter = warp & 3, half = warp >> 2;
         const uint32_t tlane = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * kCols;
         uint32_t chunk = 0;
         bool ok = true;
         for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
-            const int64_t t0 = (int64_t)(tile / P.rt) * NT, c0 = tile_col(tile);
             uint64_t acc[kCols / 2];
 #pragma unroll
             for (int i = 0; i < kCols / 2; ++i) acc[i] = 0ull;
-            const float *sp = nullptr;                                // this lane's scales
-            int64_t g = 0;
+            const float *sp = nullptr;                                // this lane's next scale
+            int left = 0;                                             // scales of the row from there on
             float s_next = 0.0f;
             if constexpr (MODE != kDgrad) {
-                int64_t row = MODE == kGated ? c0 + quarter * 16 + (lane & 15) : c0 + quarter * 32 + lane;
-                row = row < P.f.R ? row : P.f.R - 1;
-                sp = P.f.scales[MODE == kGated && lane >= 16 ? 1 : 0] + row * P.f.G;
-                g = (int64_t)st0 * kKT / CH;
-                s_next = g < P.f.G ? __ldg(sp + g) : 0.0f;
+                const int c = tile_col(tile) + (MODE == kGated ? quarter * 16 + (lane & 15) : quarter * 32 + lane);
+                const int row = c < (int)P.f.R ? c : (int)P.f.R - 1, g = st0 * (kKT / CH);
+                sp = P.f.scales[MODE == kGated && lane >= 16 ? 1 : 0] + (int64_t)row * P.f.G + g;
+                left = (int)P.f.G - g;
+                s_next = left > 0 ? __ldg(sp) : 0.0f;
+            }
+            if (MODE == kLinear && P.split == 1 && P.f.res) {         // the residual's lines, long before the epilogue reads them
+#pragma unroll
+                for (int j = 0; j < kCols / 32; ++j) {
+                    const int64_t t = (int64_t)(tile / P.rt) * NT + half * kCols + j * 32 + lane, c = tile_col(tile) + quarter * 32;
+                    if (t < P.T && c < P.N)
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"((const T *)P.f.res + t * P.f.ldres + c));
+                }
             }
             const int nch = (st1 - st0 + kStagesPer - 1) / kStagesPer * kPerStage;
             for (int ch = 0; ch < nch; ++ch, ++chunk) {
                 const uint32_t buf = chunk & 1u;
                 const float sc = s_next;
                 if constexpr (MODE != kDgrad) {
-                    ++g;
-                    s_next = g < P.f.G ? __ldg(sp + g) : 0.0f;
+                    ++sp;
+                    s_next = --left > 0 ? __ldg(sp) : 0.0f;
                 }
                 ok = wait_on(b_afull + 8 * buf, (chunk >> 1) & 1u, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
@@ -405,6 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
             }
             if (!ok) break;
             if (P.split == 1) {
+                const int64_t t0 = (int64_t)(tile / P.rt) * NT, c0 = tile_col(tile);
                 const uint32_t buf = smem_base + kOffOut + warp * kOutBytes;
                 const uint32_t wb = blk(buf, 0, lane) - buf;          // piece index without the token's bits
 #pragma unroll
@@ -439,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                     }
                     __syncwarp();
                     if constexpr (MODE == kGated) {
-#pragma unroll
+#pragma unroll 1
                         for (int k = 0; k < 2; ++k) {
                             const int tok = k * 16 + (lane >> 1), p = (lane & 1) * 8;
                             float z[8], u[8];
@@ -513,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
             __syncwarp();
         }
     } else if (warp < 16) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<MODE>::kLoad));
         const int lt = tid & 127, group = (warp >> 2) & 1;            // groups of four warps take the stages in turn
         int base = 0;                                                 // stages before this tile
         bool ok = true;
@@ -531,26 +545,24 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
             const uint32_t d0 = (uint32_t)((r0 >> 3) * 1024 + (r0 & 7) * 128), x0 = (uint32_t)(((2 * q) ^ (r0 & 7)) << 4),
                            x1 = (uint32_t)(((2 * q + 1) ^ (r0 & 7)) << 4);
             for (int tile = tile0; tile < ntiles && ok; tile += tile_step, base += st1 - st0) {
-                const int64_t c0 = tile_col(tile);
-                const uint32_t *rp[4];
-#pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    int64_t row = MODE == kGated ? c0 + p * 16 + (r0 & 15) : c0 + p * 32 + r0;
-                    row = row < P.f.R ? row : P.f.R - 1;              // rows past the matrix: computed, never stored
-                    rp[p] = P.f.packed[MODE == kGated && r0 >= 16 ? 1 : 0] + row * CP + 2 * q;
-                }
-                uint2 w[8];                                           // [sub-tile][row]
+                const int c0 = tile_col(tile) + (MODE == kGated ? r0 & 15 : r0), R = (int)P.f.R;
+                constexpr int kStep = MODE == kGated ? 16 : 32;       // matrix rows between this thread's rows
+                const uint32_t *rp = P.f.packed[MODE == kGated && r0 >= 16 ? 1 : 0] + (int64_t)c0 * CP + 2 * q;
+                uint2 w[8];                                           // [sub-tile][row]; rows past the matrix are zeros
                 const auto fetch = [&](int st) {
                     const int word = st * 16;
-                    if (P.f.vec8 && word + 16 <= CP) {
+                    if (P.f.vec8 && word + 16 <= CP && c0 + 3 * kStep < R) {
 #pragma unroll
-                        for (int p = 0; p < 8; ++p) w[p] = __ldg(reinterpret_cast<const uint2 *>(rp[p & 3] + word + (p >> 2) * 8));
+                        for (int p = 0; p < 8; ++p)
+                            w[p] = __ldg(reinterpret_cast<const uint2 *>(rp + (int64_t)(p & 3) * kStep * CP + word + (p >> 2) * 8));
                     } else {
 #pragma unroll
                         for (int p = 0; p < 8; ++p) {
                             const int j = word + (p >> 2) * 8 + 2 * q;
-                            w[p].x = j < CP ? __ldg(rp[p & 3] + word + (p >> 2) * 8) : kZeroWord;
-                            w[p].y = j + 1 < CP ? __ldg(rp[p & 3] + word + (p >> 2) * 8 + 1) : kZeroWord;
+                            const bool in = c0 + (p & 3) * kStep < R;
+                            const uint32_t *src = rp + (int64_t)(p & 3) * kStep * CP + word + (p >> 2) * 8;
+                            w[p].x = in && j < CP ? __ldg(src) : kZeroWord;
+                            w[p].y = in && j + 1 < CP ? __ldg(src + 1) : kZeroWord;
                         }
                     }
                 };
@@ -625,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
         __syncwarp();
         if (P.split > 1) cluster_sync();
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMisc));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<MODE>::kMisc));
         if (warp == 16) {
             // ------------------------------ token tile by TMA ------------------------------
             uint32_t it = 0;
