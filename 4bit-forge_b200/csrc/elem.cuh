@@ -34,6 +34,23 @@ template <typename T> __device__ __forceinline__ void load8(const T *p, float (&
         for (int i = 0; i < 8; ++i) v[i] = Elem<T>::to_f(e[i]);
     }
 }
+// the same eight elements as they are in memory, for loads that run ahead of their use
+template <typename T> struct Raw8 {
+    uint4 q[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) q[i] = reinterpret_cast<const uint4 *>(p)[i];
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) q[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        const T *e = reinterpret_cast<const T *>(q);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = Elem<T>::to_f(e[i]);
+    }
+};
 template <typename T> __device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
     if constexpr (sizeof(T) == 4) {
         reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
@@ -64,7 +81,7 @@ template <int ACT> __device__ __forceinline__ float act_bwd(float z) {
         return s * (1.0f + z * (1.0f - s));
     }
     if constexpr (ACT == FORGE_ACT_GELU)
-        return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+        return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
     return 1.0f;
 }
 __device__ __forceinline__ float act_fwd_rt(int act, float z) {

@@ -1,4 +1,4 @@
-// int4 products for few tokens (up to 32): the weights are streamed once, from global memory straight into the operand
+// int4 products for few tokens (up to 16): the weights are streamed once, from global memory straight into the operand
 // registers of warp-level m16n8k16 matrix instructions; 16 weight rows are the M side, the tokens the N side.
 //
 //   acc[r, t] = sum over groups  scale[r, g] * ( sum over the group's channels  (nibble - 8) * x[t, c] )
@@ -77,7 +77,7 @@ template <int LW> __device__ __forceinline__ void load_words(const uint32_t *row
 
 // GS: group size; NT: blocks of 8 tokens; W: warps
 template <typename T, bool GATED, int GS, int NT, int W>
-__global__ void __launch_bounds__(W * 32) decode_kernel(const Int4Fwd P) {
+__global__ void __launch_bounds__(W * 32, W == 8 && NT == 1 ? 3 : 1) decode_kernel(const Int4Fwd P) {
     constexpr int M = GATED ? 2 : 1;
     constexpr int LW = GS / 32;            // packed words of a group that one thread takes
     constexpr int NG = 128 / GS;           // groups in a block of 128 channels
@@ -97,32 +97,49 @@ __global__ void __launch_bounds__(W * 32) decode_kernel(const Int4Fwd P) {
     }
     float acc[M][NT][4] = {};
 
-    for (int kb = warp; kb < nblk; kb += W) {
-        uint32_t wra[M][NG][LW], wrb[M][NG][LW];
+    // one block of 128 channels: the words and scales of this thread's two rows, and (one token block) its channels of x;
+    // the next block's are under way while a block is multiplied
+    struct Block {
+        uint32_t a[M][NG][LW], b[M][NG][LW];
         float fa[M][NG], fb[M][NG];
+        uint4 x[NT == 1 ? 4 : 1];
+    };
+    const auto fetch_x = [&](int kb, int j, int i, int n) {
+        const int word = kb * 16 + j * (GS / 8) + q * LW + i, t = n * 8 + r8;
+        return t < (int)P.T && word < CP ? __ldg(reinterpret_cast<const uint4 *>((const T *)P.x + t * P.ldx + word * 8))
+                                         : make_uint4(0u, 0u, 0u, 0u);
+    };
+    const auto fetch = [&](int kb, Block &B) {
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
             for (int j = 0; j < NG; ++j) {
-                const int word = kb * 16 + j * (GS / 8) + q * LW;
-                load_words<LW>(wa[m], word, CP, vec, wra[m][j]);
-                load_words<LW>(wb[m], word, CP, vec, wrb[m][j]);
-                const int g = kb * NG + j;
-                fa[m][j] = g < P.G ? __ldg(sa[m] + g) : 0.0f;
-                fb[m][j] = g < P.G ? __ldg(sb[m] + g) : 0.0f;
+                const int word = kb * 16 + j * (GS / 8) + q * LW, g = kb * NG + j;
+                load_words<LW>(wa[m], word, CP, vec, B.a[m][j]);
+                load_words<LW>(wb[m], word, CP, vec, B.b[m][j]);
+                B.fa[m][j] = g < (int)P.G ? __ldg(sa[m] + g) : 0.0f;
+                B.fb[m][j] = g < (int)P.G ? __ldg(sb[m] + g) : 0.0f;
             }
+        if constexpr (NT == 1)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) B.x[k] = fetch_x(kb, k / LW, k % LW, 0);
+    };
+    Block next;
+    if (warp < nblk) fetch(warp, next);
+    for (int kb = warp; kb < nblk; kb += W) {
+        const Block B = next;
+        if (kb + W < nblk) fetch(kb + W, next);
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
             float d[M][NT][4] = {};
 #pragma unroll
             for (int i = 0; i < LW; ++i) {
-                const int word = kb * 16 + j * (GS / 8) + q * LW + i;
                 uint32_t b[NT][4];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const int64_t t = n * 8 + r8;
-                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                    if (t < P.T && word < CP) v = __ldg(reinterpret_cast<const uint4 *>((const T *)P.x + t * P.ldx + word * 8));
+                    uint4 v;
+                    if constexpr (NT == 1) v = B.x[j * LW + i];
+                    else v = fetch_x(kb, j, i, n);
                     b[n][0] = __byte_perm(v.x, v.z, 0x5410);   // channels 0, 4
                     b[n][1] = __byte_perm(v.x, v.z, 0x7632);   // 1, 5
                     b[n][2] = __byte_perm(v.y, v.w, 0x5410);   // 2, 6
@@ -131,8 +148,8 @@ __global__ void __launch_bounds__(W * 32) decode_kernel(const Int4Fwd P) {
 #pragma unroll
                 for (int m = 0; m < M; ++m) {
                     uint32_t a[4], c[4];
-                    unpack<T>(wra[m][j][i], a);
-                    unpack<T>(wrb[m][j][i], c);
+                    unpack<T>(B.a[m][j][i], a);
+                    unpack<T>(B.b[m][j][i], c);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         Mma<T>::mma(d[m][n], a[0], c[0], a[1], c[1], b[n][0], b[n][1]);
@@ -144,10 +161,10 @@ __global__ void __launch_bounds__(W * 32) decode_kernel(const Int4Fwd P) {
             for (int m = 0; m < M; ++m)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    acc[m][n][0] = fmaf(fa[m][j], d[m][n][0], acc[m][n][0]);
-                    acc[m][n][1] = fmaf(fa[m][j], d[m][n][1], acc[m][n][1]);
-                    acc[m][n][2] = fmaf(fb[m][j], d[m][n][2], acc[m][n][2]);
-                    acc[m][n][3] = fmaf(fb[m][j], d[m][n][3], acc[m][n][3]);
+                    acc[m][n][0] = fmaf(B.fa[m][j], d[m][n][0], acc[m][n][0]);
+                    acc[m][n][1] = fmaf(B.fa[m][j], d[m][n][1], acc[m][n][1]);
+                    acc[m][n][2] = fmaf(B.fb[m][j], d[m][n][2], acc[m][n][2]);
+                    acc[m][n][3] = fmaf(B.fb[m][j], d[m][n][3], acc[m][n][3]);
                 }
         }
     }
@@ -185,18 +202,21 @@ __global__ void __launch_bounds__(W * 32) decode_kernel(const Int4Fwd P) {
     }
 }
 
-template <typename T, bool GATED, int GS, int NT> int launch(const Int4Fwd &P, cudaStream_t st) {
-    constexpr int W = NT == 4 ? 8 : 16;
+template <typename T, bool GATED, int GS, int NT, int W> int launch_w(const Int4Fwd &P, cudaStream_t st) {
     constexpr int smem = W * (GATED ? 2 : 1) * NT * 8 * 17 * 4;
     static_assert(smem <= 48 * 1024, "fits the default shared memory");
     decode_kernel<T, GATED, GS, NT, W><<<(unsigned)cdiv(P.R, (int64_t)16), W * 32, smem, st>>>(P);
     FORGE_NOTE_LAUNCH();
     return check_launch(GATED ? "forge_int4_gated" : "forge_int4_linear");
 }
+// Sixteen warps share the K axis where a CTA has an SM to itself, eight where several are resident.
+template <typename T, bool GATED, int GS, int NT> int launch(const Int4Fwd &P, cudaStream_t st) {
+    if (P.R <= 148 * 16 && P.C > 1024) return launch_w<T, GATED, GS, NT, 16>(P, st);
+    return launch_w<T, GATED, GS, NT, 8>(P, st);
+}
 template <typename T, bool GATED, int GS> int launch_nt(const Int4Fwd &P, cudaStream_t st) {
     if (P.T <= 8) return launch<T, GATED, GS, 1>(P, st);
-    if (P.T <= 16) return launch<T, GATED, GS, 2>(P, st);
-    return launch<T, GATED, GS, 4>(P, st);
+    return launch<T, GATED, GS, 2>(P, st);
 }
 template <typename T, bool GATED> int launch_gs(const Int4Fwd &P, cudaStream_t st) {
     if (P.gs == 32) return launch_nt<T, GATED, 32>(P, st);

@@ -50,6 +50,11 @@ struct DzParams {
     float *unscale;
 };
 __device__ __forceinline__ float pow2_of(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
+// the largest entry of a row becomes 2^14 .. 2^15; rows of zeros and of infinities keep the factor 1
+__device__ __forceinline__ int row_exponent(float amax) {
+    const int e = (amax > 0.0f && isfinite(amax)) ? 14 - ilogbf(amax) : 0;
+    return e > 126 ? 126 : (e < -126 ? -126 : e);
+}
 
 // One CTA per token row: the row of the K operand, its power of two, and zeros up to the padded length.
 template <typename T, int ACT, bool GATED> __global__ void __launch_bounds__(256) dz_kernel(const DzParams P) {
@@ -86,14 +91,105 @@ template <typename T, int ACT, bool GATED> __global__ void __launch_bounds__(256
             amax = slot[0];
 #pragma unroll
             for (int w = 1; w < 8; ++w) amax = fmaxf(amax, slot[w]);
-            // the largest entry becomes 2^14 .. 2^15; rows of zeros and of infinities keep the factor 1
-            int e = (amax > 0.0f && isfinite(amax)) ? 14 - ilogbf(amax) : 0;
-            e = e > 126 ? 126 : (e < -126 ? -126 : e);
+            const int e = row_exponent(amax);
             scale = pow2_of(e);
             if (threadIdx.x == 0) P.unscale[t] = pow2_of(-e);
         }
     }
     for (int64_t k = P.K + threadIdx.x; k < P.ldk; k += 256) a[k] = __float2half_rn(0.0f);
+}
+
+// The same with a row in registers (R a multiple of 8, 16-byte aligned rows, R <= 8 TPR NV): dz is computed once, rows are
+// read 16 bytes at a time, and a CTA that walks several rows keeps the column sums of dz (linear form) on the way:
+// partial[blockIdx.x, R] when wanted.
+template <typename T, int ACT, bool GATED, int TPR, int NV>
+__global__ void __launch_bounds__(TPR) dz_rows_kernel(const DzParams P, float *partial) {
+    constexpr int M = GATED ? 2 : 1, W = TPR / 32;
+    __shared__ float slot[2][W];
+    const int R = (int)P.R, tid = threadIdx.x;
+    float db[NV][8];
+    if (!GATED)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) db[i][e] = 0.0f;
+    Raw8<T> rd[NV], rz[NV], ru[NV];
+    const auto fetch = [&](int64_t t) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int r = (tid + i * TPR) * 8;
+            rd[i].zero(); rz[i].zero(); ru[i].zero();
+            if (r < R && t < P.T) {
+                rd[i].load((const T *)P.dy + t * P.lddy + r);
+                if (GATED || ACT != FORGE_ACT_NONE) rz[i].load((const T *)P.z + t * P.R + r);
+                if (GATED) ru[i].load((const T *)P.u + t * P.R + r);
+            }
+        }
+    };
+    fetch(blockIdx.x);
+    int flip = 0;
+    for (int64_t t = blockIdx.x; t < P.T; t += gridDim.x, flip ^= 1) {
+        float v[M][NV][8], amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int r = (tid + i * TPR) * 8;
+            float d[8], z[8], u[8], f[8] = {};
+            rd[i].get(d);
+            rz[i].get(z);
+            ru[i].get(u);
+            if (r < R) load8(P.f + r, f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if constexpr (GATED) {
+                    v[0][i][e] = d[e] * u[e] * act_bwd<ACT>(z[e]) * f[e];
+                    v[M - 1][i][e] = d[e] * act_fwd<ACT>(z[e]);
+                } else {
+                    const float dz = d[e] * act_bwd<ACT>(z[e]);
+                    db[i][e] += dz;
+                    v[0][i][e] = dz * f[e];
+                }
+            }
+            if constexpr (GATED) {
+                if (r < R) load8(P.f + R + r, f);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[M - 1][i][e] *= f[e];
+            }
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(v[m][i][e]));
+        }
+        fetch(t + gridDim.x);                    // under way while this row is scaled
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        if ((tid & 31) == 0) slot[flip][tid >> 5] = amax;
+        __syncthreads();
+        amax = (tid & 31) < W ? slot[flip][tid & 31] : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        const int e2 = row_exponent(amax);
+        const float scale = pow2_of(e2);
+        if (tid == 0) P.unscale[t] = pow2_of(-e2);
+        __half *a = P.a + t * P.ldk;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int r = (tid + i * TPR) * 8;
+            if (r < R)
+#pragma unroll
+                for (int m = 0; m < M; ++m) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[m][i][e] *= scale;
+                    store8(a + m * R + r, v[m][i]);
+                }
+        }
+        for (int64_t k = P.K + tid; k < P.ldk; k += TPR) a[k] = __float2half_rn(0.0f);
+    }
+    if (!GATED && partial)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int r = (tid + i * TPR) * 8;
+            if (r < R) store8(partial + (int64_t)blockIdx.x * R + r, db[i]);
+        }
 }
 
 // Partial column sums of dz: CTA (column block, row share)
@@ -112,19 +208,29 @@ __global__ void __launch_bounds__(256) dbias_kernel(const T *__restrict__ dy, in
     }
     partial[(int64_t)blockIdx.y * R + r] = s;
 }
+// 32 columns x 32 strands of partial rows per CTA, joined in a fixed order
 template <typename T>
-__global__ void __launch_bounds__(256) dbias_sum_kernel(const float *__restrict__ partial, int n, int64_t R, T *out) {
-    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (r >= R) return;
+__global__ void __launch_bounds__(1024) dbias_sum_kernel(const float *__restrict__ partial, int n, int64_t R, T *out) {
+    __shared__ float sh[32][33];
+    const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
+    const int64_t r = (int64_t)blockIdx.x * 32 + lane;
     float s = 0.0f;
-    for (int k = 0; k < n; ++k) s += partial[(int64_t)k * R + r];
-    out[r] = Elem<T>::from_f(s);
+    if (r < R)
+        for (int j = k; j < n; j += 32) s += partial[(int64_t)j * R + r];
+    sh[k][lane] = s;
+    __syncthreads();
+    s = sh[lane][k];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const int64_t ro = (int64_t)blockIdx.x * 32 + k;
+    if (lane == 0 && ro < R) out[ro] = Elem<T>::from_f(s);
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------
 constexpr int64_t kMaxDim = 1ll << 24;        // rows and columns of a weight matrix
 constexpr int64_t kMaxTokens = 0x7fffffffLL;
-constexpr int kBiasParts = 64;
+constexpr int kBiasParts = 64;            // row shares of the column sums of dz, strided form
+constexpr int kRowCtas = 296;             // CTAs that walk rows in the row-in-registers form, two per SM
 
 int check_sizes(const char *who, int dtype, int64_t T, int64_t C, int64_t R, int gs, int act) {
     const char *msg = nullptr;
@@ -153,19 +259,10 @@ BwdLayout bwd_layout(int64_t T, int64_t C, int64_t R, int gs, int mats) {
     L.pairs = L.unscale + up(T * 4);
     L.f = L.pairs + up(mats * R * cdiv(C, (int64_t)gs) * 4);
     L.partial = L.f + up(mats * R * 4);
-    L.total = L.partial + up(kBiasParts * R * 4);
+    L.total = L.partial + up((T < kRowCtas ? (T < kBiasParts ? kBiasParts : T) : kRowCtas) * R * 4);
     return L;
 }
 
-template <typename T, bool GATED> void launch_dz(const DzParams &P, int act, cudaStream_t st) {
-    switch (act) {
-        case FORGE_ACT_RELU: dz_kernel<T, FORGE_ACT_RELU, GATED><<<(unsigned)P.T, 256, 0, st>>>(P); break;
-        case FORGE_ACT_SILU: dz_kernel<T, FORGE_ACT_SILU, GATED><<<(unsigned)P.T, 256, 0, st>>>(P); break;
-        case FORGE_ACT_GELU: dz_kernel<T, FORGE_ACT_GELU, GATED><<<(unsigned)P.T, 256, 0, st>>>(P); break;
-        default: dz_kernel<T, FORGE_ACT_NONE, GATED><<<(unsigned)P.T, 256, 0, st>>>(P);
-    }
-    FORGE_NOTE_LAUNCH();
-}
 template <typename T> void launch_dbias(const void *dy, int64_t lddy, const void *z, int act, int64_t n, int64_t R,
                                         float *partial, void *out, cudaStream_t st) {
     const int parts = (int)(n < kBiasParts ? (n > 0 ? n : 0) : kBiasParts);
@@ -179,7 +276,39 @@ template <typename T> void launch_dbias(const void *dy, int64_t lddy, const void
         }
         FORGE_NOTE_LAUNCH();
     }
-    dbias_sum_kernel<T><<<(unsigned)cdiv(R, (int64_t)256), 256, 0, st>>>(partial, parts, R, (T *)out); FORGE_NOTE_LAUNCH();
+    dbias_sum_kernel<T><<<(unsigned)cdiv(R, (int64_t)32), 1024, 0, st>>>(partial, parts, R, (T *)out); FORGE_NOTE_LAUNCH();
+}
+// The row-in-registers form of dz where it fits; the number of partial rows written, or 0 when the call is not for it.
+template <typename T, int ACT, bool GATED> int launch_dz_rows(const DzParams &P, float *partial, cudaStream_t st) {
+    if (P.R % 8 != 0 || P.R > 8192 || (uintptr_t)P.dy % 16 != 0 || P.lddy % 8 != 0 || (uintptr_t)P.z % 16 != 0 ||
+        (uintptr_t)P.u % 16 != 0)
+        return 0;
+    const int ctas = (int)imin64(P.T, kRowCtas);
+    if (P.R <= 2048) dz_rows_kernel<T, ACT, GATED, 256, 1><<<ctas, 256, 0, st>>>(P, partial);
+    else if (P.R <= 4096) dz_rows_kernel<T, ACT, GATED, 512, 1><<<ctas, 512, 0, st>>>(P, partial);
+    else dz_rows_kernel<T, ACT, GATED, 512, 2><<<ctas, 512, 0, st>>>(P, partial);
+    FORGE_NOTE_LAUNCH();
+    return ctas;
+}
+
+// dz into the K operand; returns the partial rows of its column sums that were written on the way (0: none)
+template <typename T, bool GATED, int ACT> int launch_dz_act(const DzParams &P, float *partial, cudaStream_t st) {
+    if (const int parts = launch_dz_rows<T, ACT, GATED>(P, partial, st)) return parts;
+    dz_kernel<T, ACT, GATED><<<(unsigned)P.T, 256, 0, st>>>(P);
+    FORGE_NOTE_LAUNCH();
+    return 0;
+}
+template <typename T, bool GATED> int launch_dz(const DzParams &P, int act, float *partial, cudaStream_t st) {
+    switch (act) {
+        case FORGE_ACT_RELU: return launch_dz_act<T, GATED, FORGE_ACT_RELU>(P, partial, st);
+        case FORGE_ACT_SILU: return launch_dz_act<T, GATED, FORGE_ACT_SILU>(P, partial, st);
+        case FORGE_ACT_GELU: return launch_dz_act<T, GATED, FORGE_ACT_GELU>(P, partial, st);
+        default: return launch_dz_act<T, GATED, FORGE_ACT_NONE>(P, partial, st);
+    }
+}
+template <typename T> void sum_dbias(const float *partial, int parts, int64_t R, void *out, cudaStream_t st) {
+    dbias_sum_kernel<T><<<(unsigned)cdiv(R, (int64_t)32), 1024, 0, st>>>(partial, parts, R, (T *)out);
+    FORGE_NOTE_LAUNCH();
 }
 
 int run_fwd(Int4Fwd &P, int dtype, bool gated, cudaStream_t st) {
@@ -231,25 +360,31 @@ static int backward(const char *who, const void *dy, int64_t lddy, int dtype, co
     const int mats = p1 ? 2 : 1;
     const BwdLayout L = bwd_layout(T, C, R, gs, mats);
     uint8_t *base = (uint8_t *)ws;
+    const bool bf16 = dtype == FORGE_DTYPE_BF16;
+    float *partial = (float *)(base + L.partial);
+    int parts = 0;
+    const int64_t G = cdiv(C, (int64_t)gs);
+    if (dx && T > 0) {
+        scale_prep_kernel<<<(unsigned)cdiv(mats * R, (int64_t)8), 256, 0, st>>>(s0, s1, R, G, (__half2 *)(base + L.pairs),
+                                                                                (float *)(base + L.f));
+        FORGE_NOTE_LAUNCH();
+        DzParams D{dy, z, u, lddy, T, R, mats * R, L.ldk, (const float *)(base + L.f), (__half *)(base + L.a),
+                   (float *)(base + L.unscale)};
+        float *pp = dbias ? partial : nullptr;
+        if (mats == 2) parts = bf16 ? launch_dz<__nv_bfloat16, true>(D, act, pp, st) : launch_dz<__half, true>(D, act, pp, st);
+        else parts = bf16 ? launch_dz<__nv_bfloat16, false>(D, act, pp, st) : launch_dz<__half, false>(D, act, pp, st);
+    }
     if (dbias) {
-        float *partial = (float *)(base + L.partial);
-        if (dtype == FORGE_DTYPE_BF16) launch_dbias<__nv_bfloat16>(dy, lddy, z, act, T, R, partial, dbias, st);
-        else launch_dbias<__half>(dy, lddy, z, act, T, R, partial, dbias, st);
+        if (parts > 0) {
+            if (bf16) sum_dbias<__nv_bfloat16>(partial, parts, R, dbias, st);
+            else sum_dbias<__half>(partial, parts, R, dbias, st);
+        } else if (bf16) {
+            launch_dbias<__nv_bfloat16>(dy, lddy, z, act, T, R, partial, dbias, st);
+        } else {
+            launch_dbias<__half>(dy, lddy, z, act, T, R, partial, dbias, st);
+        }
     }
     if (!dx || T == 0) return check_launch(who);
-    const int64_t G = cdiv(C, (int64_t)gs);
-    scale_prep_kernel<<<(unsigned)cdiv(mats * R, (int64_t)8), 256, 0, st>>>(s0, s1, R, G, (__half2 *)(base + L.pairs),
-                                                                            (float *)(base + L.f));
-    FORGE_NOTE_LAUNCH();
-    DzParams D{dy, z, u, lddy, T, R, mats * R, L.ldk, (const float *)(base + L.f), (__half *)(base + L.a),
-               (float *)(base + L.unscale)};
-    if (dtype == FORGE_DTYPE_BF16) {
-        if (mats == 2) launch_dz<__nv_bfloat16, true>(D, act, st);
-        else launch_dz<__nv_bfloat16, false>(D, act, st);
-    } else {
-        if (mats == 2) launch_dz<__half, true>(D, act, st);
-        else launch_dz<__half, false>(D, act, st);
-    }
     Int4Dgrad P{(const __half *)(base + L.a), L.ldk, (const float *)(base + L.unscale),
                 {(const uint32_t *)p0, (const uint32_t *)p1}, (const __half2 *)(base + L.pairs), gs, mats, T, C, R, G, dx, status};
     return int4_dgrad_tc(P, dtype == FORGE_DTYPE_BF16, who, st);

@@ -35,7 +35,7 @@ struct Int4Dgrad {
     int32_t *status;
 };
 
-constexpr int kDecodeTokens = 32;      // most tokens that int4_decode takes
+constexpr int kDecodeTokens = 16;      // most tokens that int4_decode takes
 // more tokens than int4_decode takes; the backward product
 int int4_fwd_tc(const Int4Fwd &P, bool bf16, bool gated, cudaStream_t st);
 int int4_dgrad_tc(const Int4Dgrad &P, bool bf16, const char *who, cudaStream_t st);

@@ -5,7 +5,8 @@
 //   n = r * rstd,  t = dy * weight,  dx = rstd * (t - n * mean(t n)) + dresidual,  dweight = sum over rows of dy * n
 //
 // Bound by HBM: a row is read once, kept in registers across the reduction, and written once.  One row belongs to 32
-// threads (up to 1024 channels), or to a whole CTA of 256 or 1024 threads; a thread holds up to four 8-element vectors.
+// threads (up to 1024 channels), or to a whole CTA of 256 to 1024 threads; a thread holds one or two 8-element vectors
+// there, so that enough rows are in flight on an SM while some wait for their reduction.
 // Rows that are longer, not a multiple of 8 channels, or not 16-byte aligned take the strided kernels below, which
 // read a row twice (the second time from cache).
 // dweight: every CTA walks rows and keeps its columns' sums in registers; one fp32 partial row per CTA, summed in a
@@ -69,10 +70,6 @@ template <int TPR> __device__ __forceinline__ float row_sum(float v, float *slot
     return v;
 }
 
-template <typename T> __device__ __forceinline__ void load_w8(const NormParams &P, int64_t c, float (&v)[8]) {
-    if (P.w_f32) load8((const float *)P.w + c, v);
-    else load8((const T *)P.w + c, v);
-}
 template <typename T> __device__ __forceinline__ float load_w(const void *w, int w_f32, int64_t c) {
     return w_f32 ? ((const float *)w)[c] : Elem<T>::to_f(((const T *)w)[c]);
 }
@@ -86,47 +83,49 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) rmsnorm_kernel(const No
     const int t = threadIdx.x % TPR;
     const int C = (int)P.C;
     const T *x = (const T *)P.x + row * P.ldx;
-    float h[NV][8], w[NV][8];
+    Raw8<T> hx[NV], hr[NV], hw[NV];
+    float h[NV][8];
     float ss = 0.0f;
+    const T *res = (const T *)P.res + row * P.ldres;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (t + i * TPR) * 8;
+        hx[i].zero(); hr[i].zero(); hw[i].zero();
         if (c < C) {
-            load8(x + c, h[i]);
-            load_w8<T>(P, c, w[i]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) h[i][e] = w[i][e] = 0.0f;
-        }
-    }
-    if (P.res) {
-        const T *res = (const T *)P.res + row * P.ldres;
-        T *r = (T *)P.r + row * P.C;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (t + i * TPR) * 8;
-            if (c < C) {
-                float v[8];
-                load8(res + c, v);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) h[i][e] += v[e];
-                store8(r + c, h[i]);
-            }
+            hx[i].load(x + c);
+            if (P.res) hr[i].load(res + c);
+            if (!P.w_f32) hw[i].load((const T *)P.w + c);
         }
     }
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+        const int c = (t + i * TPR) * 8;
+        hx[i].get(h[i]);
+        if (P.res) {
+            float v[8];
+            hr[i].get(v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[i][e] += v[e];
+            if (c < C) store8((T *)P.r + row * P.C + c, h[i]);
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = fmaf(h[i][e], h[i][e], ss);
+    }
     const float rstd = rsqrtf(row_sum<TPR>(ss, slot) / (float)C + P.eps);
+    const auto scaled_row = [&](int i, int c) {           // h[i] becomes y
+        float w[8] = {};
+        if (!P.w_f32) hw[i].get(w);
+        else if (c < C) load8((const float *)P.w + c, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[i][e] = h[i][e] * rstd * w[e];
+    };
     if (!P.scales) {
         T *y = (T *)P.y + row * P.C;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (t + i * TPR) * 8;
             if (c < C) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) h[i][e] = h[i][e] * rstd * w[i][e];
+                scaled_row(i, c);
                 store8(y + c, h[i]);
             }
         }
@@ -138,11 +137,10 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) rmsnorm_kernel(const No
     for (int i = 0; i < NV; ++i) {
         const int c = (t + i * TPR) * 8;
         float amax = kAmaxFloor;
+        scaled_row(i, c);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            h[i][e] = h[i][e] * rstd * w[i][e];
+        for (int e = 0; e < 8; ++e)
             if (c < C) amax = max_nan(amax, fabsf(h[i][e]));   // channels past the row are not part of its group
-        }
         // 16 neighbouring threads hold a group of 128 channels
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
@@ -210,8 +208,9 @@ template <typename T> __global__ void __launch_bounds__(256) rmsnorm_strided_ker
 }
 
 // Backward: every CTA (or warp, TPR = 32) walks rows; column sums of dy * n stay in registers.
+constexpr int bwd_per_sm(int tpr) { return tpr == 128 ? 6 : tpr <= 256 ? 3 : 1; }
 template <typename T, int TPR, int NV>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) rmsnorm_bwd_kernel(const NormBwdParams P) {
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, sizeof(T) == 2 ? bwd_per_sm(TPR) : 1) rmsnorm_bwd_kernel(const NormBwdParams P) {
     constexpr int kRows = TPR == 32 ? 8 : 1;
     __shared__ float slot[2][2][32];
     const int t = threadIdx.x % TPR;
@@ -229,22 +228,31 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) rmsnorm_bwd_kernel(cons
             else load8((const T *)P.w + c, w[i]);
         }
     }
+    Raw8<T> rx[NV], rg[NV], rd[NV];
+    const auto fetch = [&](int64_t row) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (t + i * TPR) * 8;
+            rx[i].zero(); rg[i].zero();
+            if (c < C && row < P.T) {
+                rx[i].load((const T *)P.x + row * P.ldx + c);
+                rg[i].load((const T *)P.dy + row * P.lddy + c);
+            }
+        }
+    };
+    fetch(unit);
     int flip = 0;
     for (int64_t row = unit; row < P.T; row += units, flip ^= 1) {
-        const T *x = (const T *)P.x + row * P.ldx, *dy = (const T *)P.dy + row * P.lddy;
         float r[NV][8], g[NV][8];
         float ss = 0.0f, dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (t + i * TPR) * 8;
-            if (c < C) {
-                load8(x + c, r[i]);
-                load8(dy + c, g[i]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) r[i][e] = g[i][e] = 0.0f;
-            }
+            rx[i].get(r[i]);
+            rg[i].get(g[i]);
+            if (P.dres && c < C) rd[i].load((const T *)P.dres + row * P.lddres + c);
         }
+        fetch(row + units);                       // under way while this row is reduced
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -261,14 +269,13 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) rmsnorm_bwd_kernel(cons
         for (int i = 0; i < NV; ++i) {
             const int c = (t + i * TPR) * 8;
             if (c < C) {
-                float o[8], d[8];
-                if (P.dres) load8((const T *)P.dres + row * P.lddres + c, d);
+                float o[8], d[8] = {};
+                if (P.dres) rd[i].get(d);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float n = r[i][e] * rstd;
                     dw[i][e] = fmaf(g[i][e], n, dw[i][e]);
-                    o[e] = rstd * (g[i][e] * w[i][e] - n * c1);
-                    if (P.dres) o[e] += d[e];
+                    o[e] = rstd * (g[i][e] * w[i][e] - n * c1) + d[e];
                 }
                 store8(dx + c, o);
             }
@@ -316,29 +323,28 @@ template <typename T> __global__ void __launch_bounds__(256) rmsnorm_dw_strided_
     P.partial[(int64_t)blockIdx.y * P.C + c] = s;
 }
 
-// out[c] = sum over n rows of partial[n, C], in a fixed order: 32 columns x 8 row strands per CTA
+// out[c] = sum over n rows of partial[n, C], in a fixed order: 32 columns x 32 row strands per CTA
 template <typename T>
-__global__ void __launch_bounds__(256) column_sum_kernel(const float *__restrict__ partial, int n, int64_t C, T *out) {
-    __shared__ float s[8][33];
+__global__ void __launch_bounds__(1024) column_sum_kernel(const float *__restrict__ partial, int n, int64_t C, T *out) {
+    __shared__ float s[32][33];
     const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
     const int k = threadIdx.x >> 5;
     float v = 0.0f;
     if (c < C)
 #pragma unroll 4
-        for (int r = k; r < n; r += 8) v += partial[(int64_t)r * C + c];
+        for (int r = k; r < n; r += 32) v += partial[(int64_t)r * C + c];
     s[k][threadIdx.x & 31] = v;
     __syncthreads();
-    if (k == 0 && c < C) {
-        v = 0.0f;
+    v = s[threadIdx.x & 31][k];              // column k of the block, strand = lane
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v += s[j][threadIdx.x];
-        out[c] = Elem<T>::from_f(v);
-    }
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    const int64_t co = (int64_t)blockIdx.x * 32 + k;
+    if ((threadIdx.x & 31) == 0 && co < C) out[co] = Elem<T>::from_f(v);
 }
 
 constexpr int64_t kMaxRows = 0x7fffffffLL;       // one CTA per row at most
-// Rows per partial sum: up to two CTAs per SM walk the rows
-constexpr int kBwdCtas = 296;
+// CTAs that walk the rows in the backward pass: as many as the SMs hold
+int bwd_cap(int tpr) { return 148 * bwd_per_sm(tpr); }
 
 bool vec_ok(const void *p, int64_t ld, size_t es) { return ((uintptr_t)p % 16 == 0) && (ld * (int64_t)es) % 16 == 0; }
 // The row-in-registers kernels: (threads per row, vectors per thread) by length; 0 = strided form.
@@ -346,10 +352,10 @@ struct RowShape { int tpr, nv; };
 RowShape row_shape(int64_t C) {
     if (C <= 256) return {32, 1};
     if (C <= 512) return {32, 2};
-    if (C <= 1024) return {32, 4};
+    if (C <= 1024) return {128, 1};
     if (C <= 2048) return {256, 1};
-    if (C <= 4096) return {256, 2};
-    if (C <= 8192) return {256, 4};
+    if (C <= 4096) return {512, 1};
+    if (C <= 8192) return {512, 2};
     if (C <= 16384) return {1024, 2};
     return {0, 0};
 }
@@ -361,15 +367,15 @@ template <typename T> void launch_fwd(const NormParams &P, RowShape s, cudaStrea
         rmsnorm_kernel<T, TPR, NV><<<(unsigned)cdiv(P.T, (int64_t)rows), TPR == 32 ? 256 : TPR, 0, st>>>(P); \
         return;                                                                                             \
     }
-    FORGE_NORM_CASE(32, 1) FORGE_NORM_CASE(32, 2) FORGE_NORM_CASE(32, 4) FORGE_NORM_CASE(256, 1)
-    FORGE_NORM_CASE(256, 2) FORGE_NORM_CASE(256, 4) FORGE_NORM_CASE(1024, 2)
+    FORGE_NORM_CASE(32, 1) FORGE_NORM_CASE(32, 2) FORGE_NORM_CASE(128, 1) FORGE_NORM_CASE(256, 1)
+    FORGE_NORM_CASE(512, 1) FORGE_NORM_CASE(512, 2) FORGE_NORM_CASE(1024, 2)
 #undef FORGE_NORM_CASE
     rmsnorm_strided_kernel<T><<<(unsigned)P.T, 256, 0, st>>>(P);
 }
 
 int bwd_ctas(int64_t T, RowShape s) {
     const int64_t rows = s.tpr == 32 ? 8 : 1;
-    return (int)imin64(cdiv(T, rows), kBwdCtas);
+    return (int)imin64(cdiv(T, rows), bwd_cap(s.tpr));
 }
 int strided_partials(int64_t T) { return (int)imin64(cdiv(T, (int64_t)16), 64); }
 
@@ -381,8 +387,8 @@ template <typename T> void launch_bwd(NormBwdParams &P, RowShape s, cudaStream_t
         rmsnorm_bwd_kernel<T, TPR, NV><<<ctas, TPR == 32 ? 256 : TPR, 0, st>>>(P); FORGE_NOTE_LAUNCH();       \
         return;                                                                                              \
     }
-    FORGE_NORM_CASE(32, 1) FORGE_NORM_CASE(32, 2) FORGE_NORM_CASE(32, 4) FORGE_NORM_CASE(256, 1)
-    FORGE_NORM_CASE(256, 2) FORGE_NORM_CASE(256, 4) FORGE_NORM_CASE(1024, 2)
+    FORGE_NORM_CASE(32, 1) FORGE_NORM_CASE(32, 2) FORGE_NORM_CASE(128, 1) FORGE_NORM_CASE(256, 1)
+    FORGE_NORM_CASE(512, 1) FORGE_NORM_CASE(512, 2) FORGE_NORM_CASE(1024, 2)
 #undef FORGE_NORM_CASE
     P.n_partial = strided_partials(P.T);
     rmsnorm_bwd_strided_kernel<T><<<(unsigned)P.T, 256, 0, st>>>(P); FORGE_NOTE_LAUNCH();
@@ -450,10 +456,10 @@ extern "C" int forge_rmsnorm_backward(const void *dy, int64_t lddy, const void *
         else launch_bwd<__half>(P, s, st);
     }
     const unsigned blocks = (unsigned)cdiv(C, (int64_t)32);
-    if (w_dtype == FORGE_DTYPE_F32) column_sum_kernel<float><<<blocks, 256, 0, st>>>(P.partial, P.n_partial, C, (float *)dweight);
+    if (w_dtype == FORGE_DTYPE_F32) column_sum_kernel<float><<<blocks, 1024, 0, st>>>(P.partial, P.n_partial, C, (float *)dweight);
     else if (w_dtype == FORGE_DTYPE_BF16)
-        column_sum_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(P.partial, P.n_partial, C, (__nv_bfloat16 *)dweight);
-    else column_sum_kernel<__half><<<blocks, 256, 0, st>>>(P.partial, P.n_partial, C, (__half *)dweight);
+        column_sum_kernel<__nv_bfloat16><<<blocks, 1024, 0, st>>>(P.partial, P.n_partial, C, (__nv_bfloat16 *)dweight);
+    else column_sum_kernel<__half><<<blocks, 1024, 0, st>>>(P.partial, P.n_partial, C, (__half *)dweight);
     FORGE_NOTE_LAUNCH();
     return check_launch("forge_rmsnorm_backward");
 }
