@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int s = 0; s < kStages; ++s) {
-            mbar_init(b_full + 8 * s, PAIR ? 1 + 8 : 1 + 4);   // the TMA issuer and four loading warps a CTA
+            mbar_init(b_full + 8 * s, 1 + 8);   // the TMA issuer and the loading warps: four of each CTA of a pair, or all eight
             mbar_init(b_empty + 8 * s, 1);
         }
         for (int a = 0; a < 2; ++a) {
@@ -503,11 +503,10 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
         if (P.split > 1) {
             cluster_sync();
             const int64_t t0 = (int64_t)(tile0 / P.rt) * NT, c0 = tile_col(tile0);
-            const int per = NT / P.split;                             // tokens of this CTA's slice
             constexpr int kGroups = kTileCols / 8;
-            for (int i = tid; i < per * kGroups && ok; i += 256) {
-                const int tok = rank * per + i / kGroups, cg = i % kGroups;
-                if (t0 + tok >= P.T) continue;
+            for (int i = rank * 256 + tid; i < NT * kGroups && ok; i += 256 * P.split) {
+                const int tok = i / kGroups, cg = i % kGroups;
+                if (t0 + tok >= P.T) break;                           // tokens only grow
                 // gated: channels cg * 8 .. are gate rows of the 32-row block cg / 2, the up rows 16 further
                 const int row = MODE == kGated ? (cg >> 1) * 32 + (cg & 1) * 8 : cg * 8;
                 float z[8] = {}, u[8] = {};
@@ -528,7 +527,10 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
         }
     } else if (warp < 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<MODE>::kLoad));
-        const int lt = tid & 127, group = (warp >> 2) & 1;            // groups of four warps take the stages in turn
+        // Two groups of four warps.  Pairs (long runs of stages): the groups take the stages in turn.  Else (few stages, where
+        // the time to the first products counts): both work on every stage, one 64-channel half each.
+        const int lt = tid & 127, group = (warp >> 2) & 1;
+        constexpr int kTurn = PAIR ? 2 : 1;
         int base = 0;                                                 // stages before this tile
         bool ok = true;
         const auto publish = [&](uint32_t s) {
@@ -548,38 +550,48 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                 const int c0 = tile_col(tile) + (MODE == kGated ? r0 & 15 : r0), R = (int)P.f.R;
                 constexpr int kStep = MODE == kGated ? 16 : 32;       // matrix rows between this thread's rows
                 const uint32_t *rp = P.f.packed[MODE == kGated && r0 >= 16 ? 1 : 0] + (int64_t)c0 * CP + 2 * q;
-                uint2 w[8];                                           // [sub-tile][row]; rows past the matrix are zeros
-                const auto fetch = [&](int st) {
-                    const int word = st * 16;
-                    if (P.f.vec8 && word + 16 <= CP && c0 + 3 * kStep < R) {
+                // [half][row] words of one stage, or [row] words of this group's half; rows past the matrix are zeros
+                constexpr int kWords = PAIR ? 8 : 4, kDeep = PAIR ? 1 : 2;
+                const int h0 = PAIR ? 0 : group;
+                uint2 w[kDeep][kWords];
+                const auto fetch = [&](int st, uint2 (&d)[kWords]) {
+                    const int word = st * 16 + h0 * 8;
+                    if (P.f.vec8 && st * 16 + 16 <= CP && c0 + 3 * kStep < R) {
 #pragma unroll
-                        for (int p = 0; p < 8; ++p)
-                            w[p] = __ldg(reinterpret_cast<const uint2 *>(rp + (int64_t)(p & 3) * kStep * CP + word + (p >> 2) * 8));
+                        for (int p = 0; p < kWords; ++p)
+                            d[p] = __ldg(reinterpret_cast<const uint2 *>(rp + (int64_t)(p & 3) * kStep * CP + word + (p >> 2) * 8));
                     } else {
 #pragma unroll
-                        for (int p = 0; p < 8; ++p) {
+                        for (int p = 0; p < kWords; ++p) {
                             const int j = word + (p >> 2) * 8 + 2 * q;
                             const bool in = c0 + (p & 3) * kStep < R;
                             const uint32_t *src = rp + (int64_t)(p & 3) * kStep * CP + word + (p >> 2) * 8;
-                            w[p].x = in && j < CP ? __ldg(src) : kZeroWord;
-                            w[p].y = in && j + 1 < CP ? __ldg(src + 1) : kZeroWord;
+                            d[p].x = in && j < CP ? __ldg(src) : kZeroWord;
+                            d[p].y = in && j + 1 < CP ? __ldg(src + 1) : kZeroWord;
                         }
                     }
                 };
-                const int first = st0 + ((group + base) & 1);
-                if (first < st1) fetch(first);
-                for (int st = first; st < st1; st += 2) {
-                    const uint32_t it = (uint32_t)(base + st - st0), s = it % kStages;
-                    ok = wait_on(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
-                    if (!ok) break;
-                    const uint32_t tileb = smem_base + s * kStageBytes + d0;
+                const int first = st0 + (PAIR ? (group + base) & 1 : 0);
 #pragma unroll
-                    for (int p = 0; p < 8; ++p) {
-                        sts128(tileb + (p >> 2) * kSubA + (p & 3) * 4096 + x0, word_to_half<kBf16>(w[p].x));
-                        sts128(tileb + (p >> 2) * kSubA + (p & 3) * 4096 + x1, word_to_half<kBf16>(w[p].y));
+                for (int a = 0; a < kDeep; ++a)
+                    if (first + a < st1) fetch(first + a, w[a]);
+                for (int stb = first; stb < st1 && ok; stb += kTurn * kDeep) {
+#pragma unroll
+                    for (int a = 0; a < kDeep; ++a) {
+                        const int st = stb + a;
+                        if (st >= st1) break;
+                        const uint32_t it = (uint32_t)(base + st - st0), s = it % kStages;
+                        ok = wait_on(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
+                        if (!ok) break;
+                        const uint32_t tileb = smem_base + s * kStageBytes + h0 * kSubA + d0;
+#pragma unroll
+                        for (int p = 0; p < kWords; ++p) {
+                            sts128(tileb + (p >> 2) * kSubA + (p & 3) * 4096 + x0, word_to_half<kBf16>(w[a][p].x));
+                            sts128(tileb + (p >> 2) * kSubA + (p & 3) * 4096 + x1, word_to_half<kBf16>(w[a][p].y));
+                        }
+                        publish(s);
+                        if (st + kTurn * kDeep < st1) fetch(st + kTurn * kDeep, w[a]);
                     }
-                    publish(s);
-                    if (st + 2 < st1) fetch(st + 2);
                 }
             }
         } else {
@@ -609,14 +621,14 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                         sc[p][1] = k < K && in1 ? __ldg(ss + so) : zero;
                     }
                 };
-                const int first = st0 + ((group + base) & 1);
-                if (first < st1) fetch(first * kKT);
-                for (int st = first; st < st1; st += 2) {
+                const int first = st0 + (PAIR ? (group + base) & 1 : 0), h0 = PAIR ? 0 : group;
+                if (first < st1) fetch(first * kKT + h0 * 64);
+                for (int st = first; st < st1; st += kTurn) {
                     const uint32_t it = (uint32_t)(base + st - st0), s = it % kStages;
                     ok = wait_on(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
                     if (!ok) break;
 #pragma unroll 1
-                    for (int h = 0; h < 2; ++h) {
+                    for (int h = h0; h < (PAIR ? 2 : h0 + 1); ++h) {
                         const uint32_t tileb = smem_base + s * kStageBytes + h * 8192 + d0;
 #pragma unroll
                         for (int p = 0; p < 4; ++p)
@@ -627,10 +639,10 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                                 sts128(tileb + i * 16384 + p * 2048,
                                        make_uint4(scaled(v.x, hi, lo), scaled(v.y, hi, lo), scaled(v.z, hi, lo), scaled(v.w, hi, lo)));
                             }
-                        if (h == 0) fetch(st * kKT + 64);
+                        if (PAIR && h == 0) fetch(st * kKT + 64);
                     }
                     publish(s);
-                    if (st + 2 < st1) fetch((st + 2) * kKT);
+                    if (st + kTurn < st1) fetch((st + kTurn) * kKT + h0 * 64);
                 }
             }
         }
@@ -789,9 +801,18 @@ int launch(TcParams &P, const TokenSource &src, const char *who, cudaStream_t st
     }
     P.rt = (int)rt;
     P.tt = (int)tt;
+    // Clusters of this size that a B200 runs at once with one such CTA per SM (cudaOccupancyMaxActiveClusters): the largest
+    // share of the K axis whose clusters all run together and that leaves a member two stages of work.
+    static const int kResident[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
     P.split = 1;
-    while (!PAIR && P.split < 8 && tiles * P.split * 2 <= sms && P.nst >= P.split * 4) P.split *= 2;
+    if (!PAIR)
+        for (int c = 8; c > 1; --c)
+            if (tiles <= kResident[c] && P.nst >= 2 * c) {
+                P.split = c;
+                break;
+            }
     P.per = (P.nst + P.split - 1) / P.split;
+    P.split = (P.nst + P.per - 1) / P.per;                             // no member without stages
     const auto kernel = int4_tc_kernel<T, MODE, CH, NT, PAIR>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
     if (e == cudaSuccess) {
