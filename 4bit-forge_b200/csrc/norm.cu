@@ -54,18 +54,16 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 
 // Sum over the threads of a row: every thread gets it.  `slot` holds one float per warp and is used once per call site
 // and row (two slots alternate where a kernel walks several rows).
-template <int TPR> __device__ __forceinline__ float row_sum(float v, float *slot) {
+template <bool CTA> __device__ __forceinline__ float row_sum(float v, float *slot) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if constexpr (TPR > 32) {
-        constexpr int W = TPR / 32;
+    if constexpr (CTA) {
         const int lane = threadIdx.x & 31;
         if (lane == 0) slot[threadIdx.x >> 5] = v;
         __syncthreads();
-        v = lane < W ? slot[lane] : 0.0f;
+        v = lane < (int)(blockDim.x >> 5) ? slot[lane] : 0.0f;
 #pragma unroll
-        for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        v = __shfl_sync(0xffffffffu, v, 0);
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     }
     return v;
 }
@@ -74,13 +72,15 @@ template <typename T> __device__ __forceinline__ float load_w(const void *w, int
     return w_f32 ? ((const float *)w)[c] : Elem<T>::to_f(((const T *)w)[c]);
 }
 
-template <typename T, int TPR, int NV>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) rmsnorm_kernel(const NormParams P) {
-    constexpr int kRows = TPR == 32 ? 8 : 1;
+// WARP: eight rows a CTA, a warp each; else one row a CTA, of as many warps as its vectors fill
+template <typename T, bool WARP, int NV>
+__global__ void __launch_bounds__(WARP ? 256 : 1024) rmsnorm_kernel(const NormParams P) {
+    constexpr int kRows = WARP ? 8 : 1;
+    const int TPR = WARP ? 32 : (int)blockDim.x;
     __shared__ float slot[32];
-    const int64_t row = (int64_t)blockIdx.x * kRows + (TPR == 32 ? threadIdx.x / 32 : 0);
-    if (TPR == 32 && row >= P.T) return;
-    const int t = threadIdx.x % TPR;
+    const int64_t row = (int64_t)blockIdx.x * kRows + (WARP ? threadIdx.x / 32 : 0);
+    if (WARP && row >= P.T) return;
+    const int t = WARP ? threadIdx.x % 32 : threadIdx.x;
     const int C = (int)P.C;
     const T *x = (const T *)P.x + row * P.ldx;
     Raw8<T> hx[NV], hr[NV], hw[NV];
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) rmsnorm_kernel(const No
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = fmaf(h[i][e], h[i][e], ss);
     }
-    const float rstd = rsqrtf(row_sum<TPR>(ss, slot) / (float)C + P.eps);
+    const float rstd = rsqrtf(row_sum<!WARP>(ss, slot) / (float)C + P.eps);
     const auto scaled_row = [&](int i, int c) {           // h[i] becomes y
         float w[8] = {};
         if (!P.w_f32) hw[i].get(w);
@@ -170,7 +170,7 @@ template <typename T> __global__ void __launch_bounds__(256) rmsnorm_strided_ker
         }
         ss = fmaf(h, h, ss);
     }
-    const float rstd = rsqrtf(row_sum<256>(ss, slot) / (float)P.C + P.eps);
+    const float rstd = rsqrtf(row_sum<true>(ss, slot) / (float)P.C + P.eps);
     if (!P.scales) {
         for (int64_t c = threadIdx.x; c < P.C; c += 256) {
             float h = Elem<T>::to_f(x[c]);
@@ -260,8 +260,8 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, sizeof(T) == 2 ? bwd_pe
                 ss = fmaf(r[i][e], r[i][e], ss);
                 dot = fmaf(g[i][e] * w[i][e], r[i][e], dot);
             }
-        ss = row_sum<TPR>(ss, slot[flip][0]);
-        dot = row_sum<TPR>(dot, slot[flip][1]);
+        ss = row_sum<(TPR > 32)>(ss, slot[flip][0]);
+        dot = row_sum<(TPR > 32)>(dot, slot[flip][1]);
         const float rstd = rsqrtf(ss / (float)C + P.eps);
         const float c1 = dot * rstd / (float)C;                 // mean(t n)
         T *dx = (T *)P.dx + row * P.C;
@@ -299,8 +299,8 @@ template <typename T> __global__ void __launch_bounds__(256) rmsnorm_bwd_strided
         ss = fmaf(r, r, ss);
         dot = fmaf(Elem<T>::to_f(dy[c]) * load_w<T>(P.w, P.w_f32, c), r, dot);
     }
-    ss = row_sum<256>(ss, slot[0]);
-    dot = row_sum<256>(dot, slot[1]);
+    ss = row_sum<true>(ss, slot[0]);
+    dot = row_sum<true>(dot, slot[1]);
     const float rstd = rsqrtf(ss / (float)P.C + P.eps), c1 = dot * rstd / (float)P.C;
     if (threadIdx.x == 0) P.stats[row] = rstd;
     for (int64_t c = threadIdx.x; c < P.C; c += 256) {
@@ -347,7 +347,7 @@ constexpr int64_t kMaxRows = 0x7fffffffLL;       // one CTA per row at most
 int bwd_cap(int tpr) { return 148 * bwd_per_sm(tpr); }
 
 bool vec_ok(const void *p, int64_t ld, size_t es) { return ((uintptr_t)p % 16 == 0) && (ld * (int64_t)es) % 16 == 0; }
-// The row-in-registers kernels: (threads per row, vectors per thread) by length; 0 = strided form.
+// The row-in-registers backward kernels: (threads per row, vectors per thread) by length; 0 = strided form.
 struct RowShape { int tpr, nv; };
 RowShape row_shape(int64_t C) {
     if (C <= 256) return {32, 1};
@@ -360,17 +360,15 @@ RowShape row_shape(int64_t C) {
     return {0, 0};
 }
 
-template <typename T> void launch_fwd(const NormParams &P, RowShape s, cudaStream_t st) {
-#define FORGE_NORM_CASE(TPR, NV)                                                                            \
-    if (s.tpr == TPR && s.nv == NV) {                                                                       \
-        const int rows = TPR == 32 ? 8 : 1;                                                                 \
-        rmsnorm_kernel<T, TPR, NV><<<(unsigned)cdiv(P.T, (int64_t)rows), TPR == 32 ? 256 : TPR, 0, st>>>(P); \
-        return;                                                                                             \
-    }
-    FORGE_NORM_CASE(32, 1) FORGE_NORM_CASE(32, 2) FORGE_NORM_CASE(128, 1) FORGE_NORM_CASE(256, 1)
-    FORGE_NORM_CASE(512, 1) FORGE_NORM_CASE(512, 2) FORGE_NORM_CASE(1024, 2)
-#undef FORGE_NORM_CASE
-    rmsnorm_strided_kernel<T><<<(unsigned)P.T, 256, 0, st>>>(P);
+template <typename T> void launch_fwd(const NormParams &P, bool vec, cudaStream_t st) {
+    const unsigned T8 = (unsigned)cdiv(P.T, (int64_t)8), T1 = (unsigned)P.T;
+    const int vecs = (int)(P.C / 8);
+    const auto warps = [](int v) { return (v + 31) / 32 * 32; };
+    if (vec && P.C <= 256) rmsnorm_kernel<T, true, 1><<<T8, 256, 0, st>>>(P);
+    else if (vec && P.C <= 512) rmsnorm_kernel<T, true, 2><<<T8, 256, 0, st>>>(P);
+    else if (vec && P.C <= 8192) rmsnorm_kernel<T, false, 1><<<T1, warps(vecs), 0, st>>>(P);
+    else if (vec && P.C <= 16384) rmsnorm_kernel<T, false, 2><<<T1, warps((vecs + 1) / 2), 0, st>>>(P);
+    else rmsnorm_strided_kernel<T><<<T1, 256, 0, st>>>(P);
 }
 
 int bwd_ctas(int64_t T, RowShape s) {
@@ -415,11 +413,10 @@ extern "C" int forge_rmsnorm(const void *x, int64_t ldx, const void *residual, i
     const size_t es = elem_size(dtype), ws = elem_size(w_dtype);
     const bool vec = C % 8 == 0 && vec_ok(x, ldx, es) && (!residual || (vec_ok(residual, ldres, es) &&
                      vec_ok(residual_out, C, es))) && vec_ok(weight, 0, ws) && (uintptr_t)y % 16 == 0;
-    const RowShape s = vec ? row_shape(C) : RowShape{0, 0};
     cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == FORGE_DTYPE_F32) launch_fwd<float>(P, s, st);
-    else if (dtype == FORGE_DTYPE_BF16) launch_fwd<__nv_bfloat16>(P, s, st);
-    else launch_fwd<__half>(P, s, st);
+    if (dtype == FORGE_DTYPE_F32) launch_fwd<float>(P, vec, st);
+    else if (dtype == FORGE_DTYPE_BF16) launch_fwd<__nv_bfloat16>(P, vec, st);
+    else launch_fwd<__half>(P, vec, st);
     FORGE_NOTE_LAUNCH();
     return check_launch("forge_rmsnorm");
 }

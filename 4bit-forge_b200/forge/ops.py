@@ -373,11 +373,12 @@ def _fail(msg):
 
 
 def _on_device(t, name):
-    """True when t lives on the current device; raises when it is not a CUDA tensor."""
-    _abi._require_cuda()
-    if not t.is_cuda:
+    """The index of t's device when that is the current one, else None; raises when t is not a CUDA tensor."""
+    dev = t.get_device()
+    if dev < 0:
+        _abi._require_cuda()
         _fail(f"{name} must be a CUDA tensor (there is no CPU path)")
-    return t.get_device() == torch.cuda.current_device()
+    return dev if dev == torch.cuda.current_device() else None
 
 
 def _rows(t, T, C, aligned: bool):
@@ -402,14 +403,14 @@ def _dense(t, name, shape, dtype, dev):
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _norm_args(x, weight):
+def _norm_args(x, weight, dev):
     if x.dim() != 2 or x.shape[1] == 0:
         _fail(f"x must be [T, C], got {list(x.shape)}")
     if x.dtype not in _ACT_DTYPES:
         _fail(f"x must be float32, bfloat16 or float16, got {x.dtype}")
     T, C = x.shape
     wt = weight.dtype
-    weight = _dense(weight, "weight", (C,), torch.float32 if wt == torch.float32 else x.dtype, x.get_device())
+    weight = _dense(weight, "weight", (C,), torch.float32 if wt == torch.float32 else x.dtype, dev)
     return T, C, weight, _ACT_DTYPES[wt], _ACT_DTYPES[x.dtype]
 
 
@@ -420,16 +421,17 @@ def rmsnorm(x, weight, eps: float = 1e-6, residual=None, quant_group: int = 0):
     Returns y, or (y, h) with a residual: h rounded to x's type is the new residual stream.  quant_group=128 returns the
     8-bit form instead of y: (q, scales) or (q, scales, h), q float8_e4m3fn [T, C], scales fp32 [T, ceil(C/128)], such that
     q * scales, group by group, is y: the layout fp8_block_dequant reads when C is a multiple of 128."""
-    if not _on_device(x, "x"):
+    dev = _on_device(x, "x")
+    if dev is None:
         with torch.cuda.device(x.device):
             return rmsnorm(x, weight, eps, residual, quant_group)
-    T, C, weight, wcode, code = _norm_args(x, weight)
+    T, C, weight, wcode, code = _norm_args(x, weight, dev)
     if quant_group not in (0, 128):
         _fail("quant_group must be 0 (no quantisation) or 128")
     x, ldx = _rows(x, T, C, False)
     h, pres, ldres, ph = None, None, 0, None
     if residual is not None:
-        _like(residual, "residual", x.shape, x.dtype, x.get_device())
+        _like(residual, "residual", x.shape, x.dtype, dev)
         residual, ldres = _rows(residual, T, C, False)
         h = torch.empty_like(x, memory_format=torch.contiguous_format)
         pres, ph = residual.data_ptr(), h.data_ptr()
@@ -439,7 +441,7 @@ def rmsnorm(x, weight, eps: float = 1e-6, residual=None, quant_group: int = 0):
     else:
         y, scales = torch.empty_like(x, memory_format=torch.contiguous_format), None
     call("forge_rmsnorm", x.data_ptr(), ldx, pres, ldres, weight.data_ptr(), wcode, code, T, C, eps, y.data_ptr(),
-         None if scales is None else scales.data_ptr(), ph, stream_ptr())
+         None if scales is None else scales.data_ptr(), ph, stream_ptr(dev))
     if scales is None:
         return y if h is None else (y, h)
     return (y, scales) if h is None else (y, scales, h)
@@ -449,22 +451,23 @@ def rmsnorm_backward(dy, x, weight, eps: float = 1e-6, dresidual=None):
     """Gradients of rmsnorm at the normed rows x (the h of the forward call when it had a residual): returns (dx, dweight),
     dx [T, C] of x's type with `dresidual` (the gradient that reaches h past the norm) added, dweight [C] of the weight's
     type (forge_rmsnorm_backward).  dx is the gradient of the forward call's x and of its residual alike."""
-    if not _on_device(x, "x"):
+    dev = _on_device(x, "x")
+    if dev is None:
         with torch.cuda.device(x.device):
             return rmsnorm_backward(dy, x, weight, eps, dresidual)
-    T, C, weight, wcode, code = _norm_args(x, weight)
-    _like(dy, "dy", x.shape, x.dtype, x.get_device())
+    T, C, weight, wcode, code = _norm_args(x, weight, dev)
+    _like(dy, "dy", x.shape, x.dtype, dev)
     (dy, lddy), (x, ldx) = _rows(dy, T, C, False), _rows(x, T, C, False)
     pres, ldres = None, 0
     if dresidual is not None:
-        _like(dresidual, "dresidual", x.shape, x.dtype, x.get_device())
+        _like(dresidual, "dresidual", x.shape, x.dtype, dev)
         dresidual, ldres = _rows(dresidual, T, C, False)
         pres = dresidual.data_ptr()
     dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     dw = torch.empty_like(weight)
     ws = torch.empty(query("forge_rmsnorm_backward_workspace_bytes", T, C), dtype=torch.uint8, device=x.device)
     call("forge_rmsnorm_backward", dy.data_ptr(), lddy, x.data_ptr(), ldx, weight.data_ptr(), wcode, code, pres, ldres, T, C,
-         eps, dx.data_ptr(), dw.data_ptr(), ws.data_ptr(), stream_ptr())
+         eps, dx.data_ptr(), dw.data_ptr(), ws.data_ptr(), stream_ptr(dev))
     return dx, dw
 
 
@@ -505,10 +508,10 @@ def int4_linear(x, packed, scales, gs: int = 128, bias=None, act: str = "none", 
     pack_int4 writes it for symmetric codes, scales [R, ceil(C/gs)], W = (nibble - 8) * scale.  x [T, C] bf16 or fp16;
     bias [R] and residual [T, R] of x's type; act "none", "relu", "silu" or "gelu" (erf form).  Returns y [T, R], or
     (y, z) with want_preact: z = x W^T + bias rounded to x's type, for int4_linear_backward."""
-    if not _on_device(x, "x"):
+    dev = _on_device(x, "x")
+    if dev is None:
         with torch.cuda.device(x.device):
             return int4_linear(x, packed, scales, gs, bias, act, residual, want_preact, status)
-    dev = x.get_device()
     packed, scales, R, C = _int4_weight(packed, scales, gs, dev, "packed")
     T, code, ac, pst = _product_args(x, "x", C, act, status)
     x, ldx = _rows(x, T, C, True)
@@ -520,10 +523,10 @@ def int4_linear(x, packed, scales, gs: int = 128, bias=None, act: str = "none", 
         _like(residual, "residual", (T, R), x.dtype, dev)
         residual, ldres = _rows(residual, T, R, False)
         pres = residual.data_ptr()
-    y = x.new_empty((T, R))
+    y = x.new_empty((T, R)) if pres is None else torch.empty_like(residual, memory_format=torch.contiguous_format)
     z = torch.empty_like(y) if want_preact else None
     call("forge_int4_linear", x.data_ptr(), ldx, code, packed.data_ptr(), scales.data_ptr(), gs, T, C, R, pb, ac, pres, ldres,
-         y.data_ptr(), None if z is None else z.data_ptr(), pst, stream_ptr())
+         y.data_ptr(), None if z is None else z.data_ptr(), pst, stream_ptr(dev))
     return y if z is None else (y, z)
 
 
@@ -532,10 +535,10 @@ def int4_linear_backward(dy, packed, scales, gs: int = 128, preact=None, act: st
     """Gradients of int4_linear for frozen weights: dz = dy * act'(preact); returns (dx, dbias), dx = dz W [T, C] and
     dbias = the column sums of dz [R], both of dy's type, None where not wanted.  preact is the z of the forward call
     (not needed with act="none"); the residual's gradient is dy itself (forge_int4_linear_backward)."""
-    if not _on_device(dy, "dy"):
+    dev = _on_device(dy, "dy")
+    if dev is None:
         with torch.cuda.device(dy.device):
             return int4_linear_backward(dy, packed, scales, gs, preact, act, want_dx, want_dbias, status)
-    dev = dy.get_device()
     packed, scales, R, C = _int4_weight(packed, scales, gs, dev, "packed")
     T, code, ac, pst = _product_args(dy, "dy", R, act, status)
     if not (want_dx or want_dbias):
@@ -551,7 +554,7 @@ def int4_linear_backward(dy, packed, scales, gs: int = 128, preact=None, act: st
     db = dy.new_empty((R,)) if want_dbias else None
     ws = torch.empty(query("forge_int4_backward_workspace_bytes", T, C, R, gs, 1), dtype=torch.uint8, device=dy.device)
     call("forge_int4_linear_backward", dy.data_ptr(), lddy, code, packed.data_ptr(), scales.data_ptr(), gs, T, C, R, pz, ac,
-         None if dx is None else dx.data_ptr(), None if db is None else db.data_ptr(), ws.data_ptr(), pst, stream_ptr())
+         None if dx is None else dx.data_ptr(), None if db is None else db.data_ptr(), ws.data_ptr(), pst, stream_ptr(dev))
     return dx, db
 
 
@@ -560,10 +563,10 @@ def int4_gated(x, gate_packed, gate_scales, up_packed, up_scales, gs: int = 128,
     """h = act(x Wg^T) * (x Wu^T) over two pack-quantized int4 matrices of one shape (see int4_linear), both projections,
     the activation and the product in one kernel (forge_int4_gated).  Returns h [T, R], or (h, g, u) with want_preact: the
     two projections rounded to x's type, for int4_gated_backward."""
-    if not _on_device(x, "x"):
+    dev = _on_device(x, "x")
+    if dev is None:
         with torch.cuda.device(x.device):
             return int4_gated(x, gate_packed, gate_scales, up_packed, up_scales, gs, act, want_preact, status)
-    dev = x.get_device()
     gate_packed, gate_scales, R, C = _int4_weight(gate_packed, gate_scales, gs, dev, "gate_packed")
     up_packed, up_scales, R2, C2 = _int4_weight(up_packed, up_scales, gs, dev, "up_packed")
     if R != R2 or C != C2:
@@ -576,7 +579,7 @@ def int4_gated(x, gate_packed, gate_scales, up_packed, up_scales, gs: int = 128,
         g, u = torch.empty_like(h), torch.empty_like(h)
         pg, pu = g.data_ptr(), u.data_ptr()
     call("forge_int4_gated", x.data_ptr(), ldx, code, gate_packed.data_ptr(), gate_scales.data_ptr(), up_packed.data_ptr(),
-         up_scales.data_ptr(), gs, T, C, R, ac, h.data_ptr(), pg, pu, pst, stream_ptr())
+         up_scales.data_ptr(), gs, T, C, R, ac, h.data_ptr(), pg, pu, pst, stream_ptr(dev))
     return (h, g, u) if want_preact else h
 
 
@@ -584,10 +587,10 @@ def int4_gated_backward(dh, g, u, gate_packed, gate_scales, up_packed, up_scales
                         status=None):
     """Gradient of int4_gated for frozen weights, at the g and u of the forward call:
     dx = (dh * u * act'(g)) Wg + (dh * act(g)) Wu, [T, C] of dh's type (forge_int4_gated_backward)."""
-    if not _on_device(dh, "dh"):
+    dev = _on_device(dh, "dh")
+    if dev is None:
         with torch.cuda.device(dh.device):
             return int4_gated_backward(dh, g, u, gate_packed, gate_scales, up_packed, up_scales, gs, act, status)
-    dev = dh.get_device()
     gate_packed, gate_scales, R, C = _int4_weight(gate_packed, gate_scales, gs, dev, "gate_packed")
     up_packed, up_scales, R2, C2 = _int4_weight(up_packed, up_scales, gs, dev, "up_packed")
     if R != R2 or C != C2:
@@ -599,5 +602,5 @@ def int4_gated_backward(dh, g, u, gate_packed, gate_scales, up_packed, up_scales
     ws = torch.empty(query("forge_int4_backward_workspace_bytes", T, C, R, gs, 2), dtype=torch.uint8, device=dh.device)
     call("forge_int4_gated_backward", dh.data_ptr(), lddh, code, g.data_ptr(), u.data_ptr(), gate_packed.data_ptr(),
          gate_scales.data_ptr(), up_packed.data_ptr(), up_scales.data_ptr(), gs, T, C, R, ac, dx.data_ptr(), ws.data_ptr(),
-         pst, stream_ptr())
+         pst, stream_ptr(dev))
     return dx
