@@ -394,7 +394,7 @@ extern "C" int forge_int4_linear_backward(const void *dy, int64_t lddy, int dtyp
                                           int gs, int64_t T, int64_t C, int64_t R, const void *preact, int act, void *dx,
                                           void *dbias, void *ws, int32_t *status, void *stream) {
     if (int rc = check_sizes(__func__, dtype, T, C, R, gs, act)) return rc;
-    FORGE_REQUIRE(dx || dbias, "nothing to compute");
+    FORGE_REQUIRE(T == 0 || dx || dbias, "nothing to compute");     // (no tokens: dx is empty and may be null)
     FORGE_REQUIRE(T == 0 || (dy && (!dx || (packed && scales)) && (act == FORGE_ACT_NONE || preact)), "null pointer");
     FORGE_REQUIRE(ws && (uintptr_t)ws % 256 == 0, "workspace must be 256-byte aligned");
     FORGE_REQUIRE(T <= 1 || lddy >= R, "dy row stride below R");

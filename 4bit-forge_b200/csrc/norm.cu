@@ -4,15 +4,15 @@
 // and its backward pass at the stored stream r:
 //   n = r * rstd,  t = dy * weight,  dx = rstd * (t - n * mean(t n)) + dresidual,  dweight = sum over rows of dy * n
 //
-// Bound by HBM: a row is read once, kept in registers across the reduction, and written once.  One row belongs to 32
-// threads (up to 1024 channels), or to a whole CTA of 256 to 1024 threads; a thread holds one or two 8-element vectors
-// there, so that enough rows are in flight on an SM while some wait for their reduction.
+// Bound by HBM: a row is read once, kept in registers across the reduction, and written once.  One row belongs to a warp
+// (up to 512 channels) or to a CTA, eight channels a thread.
 // Rows that are longer, not a multiple of 8 channels, or not 16-byte aligned take the strided kernels below, which
 // read a row twice (the second time from cache).
 // dweight: every CTA walks rows and keeps its columns' sums in registers; one fp32 partial row per CTA, summed in a
 // fixed order by a second launch, so results do not depend on scheduling.
 #include "common.cuh"
 #include "elem.cuh"
+#include "tcgen05.cuh"
 
 using namespace forge;
 
@@ -72,87 +72,109 @@ template <typename T> __device__ __forceinline__ float load_w(const void *w, int
     return w_f32 ? ((const float *)w)[c] : Elem<T>::to_f(((const T *)w)[c]);
 }
 
-// WARP: eight rows a CTA, a warp each; else one row a CTA, of as many warps as its vectors fill
+// CTAs of as many warps as a row's vectors fill walk the rows (WARP: a warp a row, eight a CTA) with the next kDeep rows on
+// their way into shared memory.  A row is a chain of load, reduction and store of about a microsecond, so what keeps HBM
+// busy is the bytes in flight beside it: 8192 x 7168 with residual to e4m3 took 87 us with one row a CTA and two CTAs an
+// SM.  A thread copies (cp.async) and reads its own vectors only, so the ring needs no barrier.
+constexpr int kDeep = 4;
+
 template <typename T, bool WARP, int NV>
 __global__ void __launch_bounds__(WARP ? 256 : 1024) rmsnorm_kernel(const NormParams P) {
-    constexpr int kRows = WARP ? 8 : 1;
-    const int TPR = WARP ? 32 : (int)blockDim.x;
-    __shared__ float slot[32];
-    const int64_t row = (int64_t)blockIdx.x * kRows + (WARP ? threadIdx.x / 32 : 0);
-    if (WARP && row >= P.T) return;
-    const int t = WARP ? threadIdx.x % 32 : threadIdx.x;
-    const int C = (int)P.C;
-    const T *x = (const T *)P.x + row * P.ldx;
-    Raw8<T> hx[NV], hr[NV], hw[NV];
-    float h[NV][8];
-    float ss = 0.0f;
-    const T *res = (const T *)P.res + row * P.ldres;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (t + i * TPR) * 8;
-        hx[i].zero(); hr[i].zero(); hw[i].zero();
-        if (c < C) {
-            hx[i].load(x + c);
-            if (P.res) hr[i].load(res + c);
-            if (!P.w_f32) hw[i].load((const T *)P.w + c);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (t + i * TPR) * 8;
-        hx[i].get(h[i]);
-        if (P.res) {
-            float v[8];
-            hr[i].get(v);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) h[i][e] += v[e];
-            if (c < C) store8((T *)P.r + row * P.C + c, h[i]);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(h[i][e], h[i][e], ss);
-    }
-    const float rstd = rsqrtf(row_sum<!WARP>(ss, slot) / (float)C + P.eps);
-    const auto scaled_row = [&](int i, int c) {           // h[i] becomes y
-        float w[8] = {};
-        if (!P.w_f32) hw[i].get(w);
-        else if (c < C) load8((const float *)P.w + c, w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) h[i][e] = h[i][e] * rstd * w[e];
+    constexpr int kQ = sizeof(T) / 2;                     // 16-byte pieces of a vector
+    extern __shared__ uint4 ring[];                       // [kDeep][x, residual][NV][kQ][threads]
+    __shared__ float slot[2][32];
+    const int TPR = WARP ? 32 : (int)blockDim.x, t = WARP ? threadIdx.x % 32 : threadIdx.x, C = (int)P.C;
+    const int64_t step = WARP ? (int64_t)gridDim.x * 8 : gridDim.x;
+    const int64_t row0 = WARP ? (int64_t)blockIdx.x * 8 + threadIdx.x / 32 : blockIdx.x;
+    const int arrays = P.res ? 2 : 1;
+    const auto place = [&](int s, int a, int i, int k) -> uint4 * {
+        return ring + ((((s * arrays + a) * NV + i) * kQ + k) * (int)blockDim.x + (int)threadIdx.x);
     };
-    if (!P.scales) {
-        T *y = (T *)P.y + row * P.C;
+    const auto fetch = [&](int64_t row, int s) {
+        if (row < P.T)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (t + i * TPR) * 8;
+                if (c < C)
+#pragma unroll
+                    for (int k = 0; k < kQ; ++k) {
+                        tc::cp_async16_zfill(tc::smem_u32(place(s, 0, i, k)),
+                                             reinterpret_cast<const uint4 *>((const T *)P.x + row * P.ldx + c) + k, true);
+                        if (P.res)
+                            tc::cp_async16_zfill(tc::smem_u32(place(s, 1, i, k)),
+                                                 reinterpret_cast<const uint4 *>((const T *)P.res + row * P.ldres + c) + k, true);
+                    }
+            }
+        tc::cp_async_commit();
+    };
+    const auto take = [&](int s, int a, int i, float (&v)[8]) {
+        Raw8<T> r;
+        if ((t + i * TPR) * 8 < C)
+#pragma unroll
+            for (int k = 0; k < kQ; ++k) r.q[k] = *place(s, a, i, k);
+        else
+            r.zero();
+        r.get(v);
+    };
+    Raw8<T> hw[NV];
+#pragma unroll
+    for (int a = 0; a < kDeep; ++a) fetch(row0 + a * step, a);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (t + i * TPR) * 8;
+        hw[i].zero();
+        if (c < C && !P.w_f32) hw[i].load((const T *)P.w + c);
+    }
+    int flip = 0, s = 0;
+    for (int64_t row = row0; row < P.T; row += step, s = (s + 1) % kDeep) {
+        tc::cp_async_wait<kDeep - 1>();
+        float h[NV][8], ss = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (t + i * TPR) * 8;
+            take(s, 0, i, h[i]);
+            if (P.res) {
+                float v[8];
+                take(s, 1, i, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) h[i][e] += v[e];
+                if (c < C) store8((T *)P.r + row * P.C + c, h[i]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss = fmaf(h[i][e], h[i][e], ss);
+        }
+        fetch(row + kDeep * step, s);
+        const float rstd = rsqrtf(row_sum<!WARP>(ss, slot[flip]) / (float)C + P.eps);
+        flip ^= 1;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (t + i * TPR) * 8;
+            float w[8] = {}, amax = kAmaxFloor;
+            if (!P.w_f32) hw[i].get(w);
+            else if (c < C) load8((const float *)P.w + c, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                h[i][e] = h[i][e] * rstd * w[e];
+                if (c < C) amax = max_nan(amax, fabsf(h[i][e]));   // channels past the row are not part of its group
+            }
+            if (!P.scales) {
+                if (c < C) store8((T *)P.y + row * P.C + c, h[i]);
+                continue;
+            }
+            // 16 neighbouring threads hold a group of 128 channels
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            const float sc = amax / kF8Max, inv = 1.0f / sc;
             if (c < C) {
-                scaled_row(i, c);
-                store8(y + c, h[i]);
+                uint2 out;
+                out.x = e4m3x4(h[i][0] * inv, h[i][1] * inv, h[i][2] * inv, h[i][3] * inv);
+                out.y = e4m3x4(h[i][4] * inv, h[i][5] * inv, h[i][6] * inv, h[i][7] * inv);
+                *reinterpret_cast<uint2 *>((uint8_t *)P.y + row * P.C + c) = out;
+                if ((t & 15) == 0) P.scales[row * cdiv(P.C, (int64_t)kQGroup) + c / kQGroup] = sc;
             }
         }
-        return;
     }
-    uint8_t *q = (uint8_t *)P.y + row * P.C;
-    float *srow = P.scales + row * cdiv(P.C, (int64_t)kQGroup);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (t + i * TPR) * 8;
-        float amax = kAmaxFloor;
-        scaled_row(i, c);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (c < C) amax = max_nan(amax, fabsf(h[i][e]));   // channels past the row are not part of its group
-        // 16 neighbouring threads hold a group of 128 channels
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        const float s = amax / kF8Max, inv = 1.0f / s;
-        if (c < C) {
-            uint2 out;
-            out.x = e4m3x4(h[i][0] * inv, h[i][1] * inv, h[i][2] * inv, h[i][3] * inv);
-            out.y = e4m3x4(h[i][4] * inv, h[i][5] * inv, h[i][6] * inv, h[i][7] * inv);
-            *reinterpret_cast<uint2 *>(q + c) = out;
-            if ((t & 15) == 0) srow[c / kQGroup] = s;
-        }
-    }
+    tc::cp_async_wait<0>();
 }
 
 // Any length, stride and alignment: the row is read twice.
@@ -360,15 +382,29 @@ RowShape row_shape(int64_t C) {
     return {0, 0};
 }
 
-template <typename T> void launch_fwd(const NormParams &P, bool vec, cudaStream_t st) {
-    const unsigned T8 = (unsigned)cdiv(P.T, (int64_t)8), T1 = (unsigned)P.T;
+template <typename T, bool WARP, int NV> int launch_rows(const NormParams &P, int threads, cudaStream_t st) {
+    const int smem = kDeep * (P.res ? 2 : 1) * NV * (int)sizeof(T) / 2 * threads * 16;
+    const auto kernel = rmsnorm_kernel<T, WARP, NV>;
+    if (smem > 40 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) {
+            set_error("forge_rmsnorm: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+            return FORGE_ERR_LAUNCH;
+        }
+    }
+    const int64_t per_sm = 1024 / threads;                 // CTAs on an SM: 1024 threads, 128 KB of ring at most
+    const int64_t rows = WARP ? cdiv(P.T, (int64_t)8) : P.T;
+    kernel<<<(unsigned)imin64(rows, 148 * per_sm), threads, smem, st>>>(P);
+    return FORGE_OK;
+}
+template <typename T> int launch_fwd(const NormParams &P, bool vec, cudaStream_t st) {
     const int vecs = (int)(P.C / 8);
     const auto warps = [](int v) { return (v + 31) / 32 * 32; };
-    if (vec && P.C <= 256) rmsnorm_kernel<T, true, 1><<<T8, 256, 0, st>>>(P);
-    else if (vec && P.C <= 512) rmsnorm_kernel<T, true, 2><<<T8, 256, 0, st>>>(P);
-    else if (vec && P.C <= 8192) rmsnorm_kernel<T, false, 1><<<T1, warps(vecs), 0, st>>>(P);
-    else if (vec && P.C <= 16384) rmsnorm_kernel<T, false, 2><<<T1, warps((vecs + 1) / 2), 0, st>>>(P);
-    else rmsnorm_strided_kernel<T><<<T1, 256, 0, st>>>(P);
+    if (vec && P.C <= 256) return launch_rows<T, true, 1>(P, 256, st);
+    if (vec && P.C <= 512) return launch_rows<T, true, 2>(P, 256, st);
+    if (vec && P.C <= (sizeof(T) == 2 ? 8192 : 4096)) return launch_rows<T, false, 1>(P, warps(vecs), st);
+    rmsnorm_strided_kernel<T><<<(unsigned)P.T, 256, 0, st>>>(P);
+    return FORGE_OK;
 }
 
 int bwd_ctas(int64_t T, RowShape s) {
@@ -414,9 +450,10 @@ extern "C" int forge_rmsnorm(const void *x, int64_t ldx, const void *residual, i
     const bool vec = C % 8 == 0 && vec_ok(x, ldx, es) && (!residual || (vec_ok(residual, ldres, es) &&
                      vec_ok(residual_out, C, es))) && vec_ok(weight, 0, ws) && (uintptr_t)y % 16 == 0;
     cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == FORGE_DTYPE_F32) launch_fwd<float>(P, vec, st);
-    else if (dtype == FORGE_DTYPE_BF16) launch_fwd<__nv_bfloat16>(P, vec, st);
-    else launch_fwd<__half>(P, vec, st);
+    const int rc = dtype == FORGE_DTYPE_F32    ? launch_fwd<float>(P, vec, st)
+                   : dtype == FORGE_DTYPE_BF16 ? launch_fwd<__nv_bfloat16>(P, vec, st)
+                                               : launch_fwd<__half>(P, vec, st);
+    if (rc != FORGE_OK) return rc;
     FORGE_NOTE_LAUNCH();
     return check_launch("forge_rmsnorm");
 }

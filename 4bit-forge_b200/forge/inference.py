@@ -143,6 +143,15 @@ class Int4FeedForward(torch.nn.Module):
             raise RuntimeError("gate and up must be [I, H/8] and down [H, I/8] packed words")
         self.norm_weight = None if norm_weight is None else torch.nn.Parameter(norm_weight.detach().clone())
 
+    def _apply(self, fn, recurse=True):
+        """Module.to(dtype), .half() and the like move the scales but leave them in fp32: they are part of the codes."""
+        kept = {name: getattr(self, name) for name in ("gate_scales", "up_scales", "down_scales")}
+        super()._apply(fn, recurse)
+        for name, scales in kept.items():
+            if getattr(self, name).dtype != torch.float32:
+                setattr(self, name, scales.to(getattr(self, name).device))
+        return self
+
     @classmethod
     def from_quantized(cls, out, index, group_size=128, **kw):
         """Matrix `index` of every family of MoELayerQuantizer.quantize_experts(...) (cfg.pack, symmetric, "gptq"): routed

@@ -274,6 +274,54 @@ def test_gated_backward(T, C, R, gs, dt, act):
     close(dx, want, grad_tol(dg, Wg, dt, want) + grad_tol(du, Wu, dt, want * 0), "dx")
 
 
+# enough tiles that two CTAs share each (more than 37 tiles of 256 rows x 256 tokens), with ragged edges in every direction
+LARGE = [(1100, 264, 2501, 32, torch.bfloat16, "gelu"), (2049, 520, 1300, 64, torch.float16, "none"),
+         (2600, 1032, 1025, 128, torch.bfloat16, "silu"), (257, 136, 5000, 128, torch.float16, "relu"),
+         (3000, 8, 1000, 32, torch.bfloat16, "none")]
+
+
+@pytest.mark.parametrize("T,C,R,gs,dt,act", LARGE)
+def test_large_tiles(T, C, R, gs, dt, act):
+    g = gen(T + C)
+    packed, scales, W, x = check_linear(T, C, R, gs, dt, act, g)
+    check_linear(T, C, R, gs, dt, "none", g, bias=False, residual=True)
+    y = ops().int4_linear(x, packed, scales, gs)
+    Z = x.double() @ W.T
+    close(y, Z, HALF[dt] * Z.abs() + sum_tol(x.double(), W, scales.shape[1]) + 2.0 ** -25, "plain product")
+    test_gated(T, C, R // 2 + 1, gs, dt, act)
+    # the backward product has C on the side of the rows
+    test_linear_backward(T, 8 * (R // 8), max(C, 33), gs, dt, act)
+    test_gated_backward(T, 8 * (R // 8), max(C // 2 + 1, 33), gs, dt, act)
+
+
+@pytest.mark.parametrize("T,C,R", [(5, 16384, 40), (20, 16384, 40), (40, 20000, 70), (130, 16384, 300), (700, 8200, 64)])
+def test_long_sums_over_few_rows(T, C, R):
+    """The K axis is shared by the warps or the CTAs of a cluster, unevenly."""
+    test_linear(T, C, R, 128, torch.bfloat16, "none")
+    test_gated(T, C, R, 64, torch.float16, "silu")
+    test_linear_backward(T, 8 * R, C // 4, 32, torch.bfloat16, "gelu")
+
+
+@pytest.mark.parametrize("T", [3, 20, 100])
+def test_words_that_start_off_16_bytes(T):
+    """Packed matrices that are views into one buffer: rows start on 4 or 8 bytes only."""
+    g = gen(T + 1)
+    C, R, gs = 256, 48, 128
+    packed, scales, W = weight(R, C, gs, g)
+    x = torch.randn(T, C, generator=g, device=DEV).half()
+    want = ops().int4_linear(x, packed, scales, gs)
+    want_g = ops().int4_gated(x, packed, scales, packed, scales, gs)
+    dy = torch.randn(T, R, generator=g, device=DEV).half()
+    want_d = ops().int4_linear_backward(dy, packed, scales, gs)[0]
+    for off in (1, 2, 3, 4):
+        buf = torch.zeros(packed.numel() + off, dtype=torch.int32, device=DEV)
+        view = buf[off:].view(R, C // 8)
+        view.copy_(packed)
+        assert torch.equal(ops().int4_linear(x, view, scales, gs), want)
+        assert torch.equal(ops().int4_gated(x, view, scales, packed, scales, gs), want_g)
+        assert torch.equal(ops().int4_linear_backward(dy, view, scales, gs)[0], want_d)
+
+
 def test_gated_backward_against_differences():
     g = gen(77)
     T, C, R, gs = 3, 128, 96, 32
@@ -525,3 +573,75 @@ def test_rows_past_two_to_the_31_elements():
     want = norm64(y[tail].double(), w.double())
     close(n[tail], want, (2.0 ** -8 + 2.0 ** -18) * want.abs(), "norm tail")
     assert _abi.query("forge_launch_count") > 0
+
+
+def test_captured_training_step():
+    """Forward and backward of the block in one graph, replayed with other inputs, against the eager step."""
+    from forge.inference import Int4FeedForward
+    parts, x, res, w = block_parts(300, 256, 192, 64, torch.bfloat16, 11)
+    blk = Int4FeedForward(*[p[:2] for p in parts], group_size=64, norm_weight=w)
+    dout = torch.randn(300, 256, generator=gen(2), device=DEV).to(torch.bfloat16)
+
+    def step(a, b):
+        out = blk(a, residual=b)
+        return (out, *torch.autograd.grad(out, (a, b, blk.norm_weight), dout))
+    sx, sr = torch.zeros_like(x).requires_grad_(), torch.zeros_like(res).requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(sx, sr)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(sx, sr)
+    for a, b in ((x, res), (res, x)):
+        with torch.no_grad():
+            sx.copy_(a)
+            sr.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(a.clone().requires_grad_(), b.clone().requires_grad_())
+        for g1, g2 in zip(got, want):
+            assert torch.equal(g1, g2)
+
+
+def test_block_without_norm_and_without_tokens():
+    from forge.inference import Int4FeedForward
+    parts, x, res, w = block_parts(9, 128, 64, 32, torch.float16, 3)
+    bare = Int4FeedForward(*[p[:2] for p in parts], group_size=32)
+    X = x.double()
+    a = act64(X @ parts[0][2].T, "silu") * (X @ parts[1][2].T)
+    want = a @ parts[2][2].T
+    mag = ((X.abs() @ parts[0][2].abs().T) * (X.abs() @ parts[1][2].abs().T)) @ parts[2][2].abs().T
+    close(bare(x), want, 2.0 ** -11 * want.abs() + 2.0 ** -11 * 1.01 * (a.abs() @ parts[2][2].abs().T) + 2.0 ** -14 * mag + 2.0 ** -24, "bare")
+    normed = Int4FeedForward(*[p[:2] for p in parts], group_size=32, norm_weight=w)
+    for blk in (bare, normed):
+        assert blk(x[:0]).shape == (0, 128)
+        e = x[:0].clone().requires_grad_()
+        blk(e).sum().backward()
+        assert e.grad.shape == (0, 128)
+    assert not bool(normed.norm_weight.grad.any())
+
+
+def test_calls_from_two_threads():
+    import threading
+    g = gen(4)
+    packed, scales, _ = weight(264, 2048, 128, g)
+    xs = [torch.randn(T, 2048, generator=g, device=DEV).half() for T in (1, 12, 60, 400)]
+    want = [ops().int4_linear(x, packed, scales, 128) for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                k = (i + _) % len(xs)
+                y = ops().int4_linear(xs[k], packed, scales, 128)
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(y, want[k]):
+                    bad.append(k)
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert not bad

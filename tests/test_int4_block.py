@@ -105,6 +105,10 @@ def test_feed_forward_block_checks_its_matrices():
     blk = Int4FeedForward(gate, up, down, group_size=32)
     assert sorted(n for n, _ in blk.named_buffers()) == ["down_packed", "down_scales", "gate_packed", "gate_scales",
                                                          "up_packed", "up_scales"]
+    third = up[1] / 3
+    blk.up_scales.copy_(third)
+    blk = blk.to(torch.bfloat16).half()              # the scales stay as they are
+    assert blk.up_scales.dtype == torch.float32 and torch.equal(blk.up_scales, third)
     with pytest.raises(RuntimeError):
         Int4FeedForward(gate, gate, gate, group_size=32)
     with pytest.raises(RuntimeError):
