@@ -386,7 +386,8 @@ static int backward(const char *who, const void *dy, int64_t lddy, int dtype, co
     }
     if (!dx || T == 0) return check_launch(who);
     Int4Dgrad P{(const __half *)(base + L.a), L.ldk, (const float *)(base + L.unscale),
-                {(const uint32_t *)p0, (const uint32_t *)p1}, (const __half2 *)(base + L.pairs), gs, mats, T, C, R, G, dx, status};
+                {(const uint32_t *)p0, (const uint32_t *)p1}, (const __half2 *)(base + L.pairs), gs, mats, T, C, R, G, dx, status,
+                C % 16 == 0 && ((uintptr_t)p0 | (uintptr_t)p1) % 8 == 0};
     return int4_dgrad_tc(P, dtype == FORGE_DTYPE_BF16, who, st);
 }
 

@@ -33,6 +33,7 @@ struct Int4Dgrad {
     int64_t T, C, R, G;
     void *dx;                    // [T, C]
     int32_t *status;
+    bool vec8;                   // rows of packed words start on 8 bytes
 };
 
 constexpr int kDecodeTokens = 16;      // most tokens that int4_decode takes

@@ -11,8 +11,7 @@
 //
 // Backward (dx = dz W): M is the channels, read along the rows of W (an MN-major operand), K the weight rows.  A chunk has
 // many scales there, so they have to be in the operand: W' = fp16((nibble - 8) * s'), s' the scale without its row's power
-// of two (which dz carries exactly), from an fp16 pair (hi, lo) so that W' is rounded once.  Chunks of 512 weight rows are
-// added up in registers.
+// of two (which dz carries exactly), kept as an fp16 pair (hi, lo).  Chunks of 512 weight rows are added up in registers.
 //
 // A CTA (one per SM, 640 threads): warps 0-7 add finished chunks to the sums and run the epilogue, warps 8-11 and 12-15
 // turn packed words into 16-bit operand tiles, one stage each in turn (words read ahead into registers, tiles written with
@@ -191,9 +190,11 @@ template <bool BF16> __device__ __forceinline__ uint4 word_to_half(uint32_t w) {
     }
     return make_uint4(p[0], p[1], p[2], p[3]);
 }
-__device__ __forceinline__ uint32_t scaled(uint32_t v, __half2 hi, __half2 lo) {
+// W' of the backward form.  fp16 gradients: from the scale's pair, rounded once (2^-11).  bf16 gradients, rounded to 2^-8
+// themselves: from the scale's high part alone, 2^-11 more and one operation in three less for the loading warps.
+template <typename T> __device__ __forceinline__ uint32_t scaled(uint32_t v, __half2 hi, __half2 lo) {
     const __half2 q = *reinterpret_cast<const __half2 *>(&v);
-    const __half2 r = __hfma2(q, hi, __hmul2(q, lo));
+    const __half2 r = std::is_same<T, __half>::value ? __hfma2(q, hi, __hmul2(q, lo)) : __hmul2(q, hi);
     return *reinterpret_cast<const uint32_t *>(&r);
 }
 
@@ -595,54 +596,81 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                 }
             }
         } else {
-            // words l8 + 8 i of K rows k0 + 16 p (p < 8, four at a time): eight lanes read 32 bytes of a row, the 64 channels
-            // of block i
+            // Eight lanes read the 16 words (128 channels) of a K row, two each; K rows k0 + 16 p of a 64-row half.  The upper
+            // four lanes, whose words lie in the second 64-channel block, store their two pieces in the other order: eight
+            // lanes then write eight different pieces of 16 bytes.
             const int CP = (int)(P.d.C / 8), l8 = lt & 7, k0 = lt >> 3, K = (int)(P.d.mats * P.d.R), R = (int)P.d.R;
             const int G = (int)P.d.G, sh = P.d.gs == 32 ? 5 : P.d.gs == 64 ? 6 : 7;
-            const uint32_t d0 = (uint32_t)((k0 >> 3) * 1024 + (k0 & 7) * 128 + ((l8 ^ (k0 & 7)) << 4));
+            const bool swap = l8 >= 4;
+            const uint32_t d0 = (uint32_t)((l8 >> 2) * 16384 + (k0 >> 3) * 1024 + (k0 & 7) * 128);
+            const uint32_t xa = (uint32_t)((((2 * l8 + (swap ? 1 : 0)) & 7) ^ (k0 & 7)) << 4),
+                           xb = (uint32_t)((((2 * l8 + (swap ? 0 : 1)) & 7) ^ (k0 & 7)) << 4);
+            struct Half {
+                uint2 w[4];
+                __half2 s[4];
+            };
             for (int tile = tile0; tile < ntiles && ok; tile += tile_step, base += st1 - st0) {
-                const int c = (int)tile_col(tile) + l8 * 8;           // this lane's channels: c + 64 i
-                const bool in0 = c < (int)P.d.C, in1 = c + 64 < (int)P.d.C;
-                const uint32_t *w0 = P.d.packed[0] + c / 8, *w1 = P.d.mats == 2 ? P.d.packed[1] + c / 8 : w0;
-                const __half2 *sp = P.d.pairs + (c >> sh);
-                const int so = ((c + 64) >> sh) - (c >> sh);
-                uint32_t w[4][2];
-                __half2 sc[4][2];
-                const auto fetch = [&](int k1) {
+                const int c = tile_col(tile) + l8 * 16, word = c / 8;
+                const bool in0 = word < CP, in1 = word + 1 < CP;
+                const uint32_t *w0 = P.d.packed[0] + word, *w1 = P.d.mats == 2 ? P.d.packed[1] + word : w0;
+                const __half2 *sp = P.d.pairs + (c >> sh);            // 16 channels lie in one group
+                const auto fetch = [&](int st, int h, Half &H) {
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
-                        const int k = k1 + k0 + 16 * p;
+                        const int k = st * kKT + h * 64 + k0 + 16 * p;
                         const uint32_t *src = (k < R ? w0 : w1) + (int64_t)(k < R ? k : k - R) * CP;
-                        const __half2 *ss = sp + (int64_t)k * G;
-                        const __half2 zero = __half2(__ushort_as_half(0), __ushort_as_half(0));
-                        w[p][0] = k < K && in0 ? __ldg(src) : kZeroWord;
-                        w[p][1] = k < K && in1 ? __ldg(src + 8) : kZeroWord;
-                        sc[p][0] = k < K && in0 ? __ldg(ss) : zero;
-                        sc[p][1] = k < K && in1 ? __ldg(ss + so) : zero;
+                        uint2 v = make_uint2(kZeroWord, kZeroWord);
+                        if (P.d.vec8) {
+                            if (k < K && in0) v = __ldg(reinterpret_cast<const uint2 *>(src));
+                        } else {
+                            if (k < K && in0) v.x = __ldg(src);
+                            if (k < K && in1) v.y = __ldg(src + 1);
+                        }
+                        H.w[p] = v;
+                        H.s[p] = k < K && in0 ? __ldg(sp + (int64_t)k * G) : __half2(__ushort_as_half(0), __ushort_as_half(0));
                     }
                 };
-                const int first = st0 + (PAIR ? (group + base) & 1 : 0), h0 = PAIR ? 0 : group;
-                if (first < st1) fetch(first * kKT + h0 * 64);
-                for (int st = first; st < st1; st += kTurn) {
-                    const uint32_t it = (uint32_t)(base + st - st0), s = it % kStages;
-                    ok = wait_on(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
-                    if (!ok) break;
-#pragma unroll 1
-                    for (int h = h0; h < (PAIR ? 2 : h0 + 1); ++h) {
-                        const uint32_t tileb = smem_base + s * kStageBytes + h * 8192 + d0;
+                const auto unpack = [&](uint32_t at, const Half &H) {
 #pragma unroll
-                        for (int p = 0; p < 4; ++p)
+                    for (int p = 0; p < 4; ++p) {
+                        const __half2 hi = __low2half2(H.s[p]), lo = __high2half2(H.s[p]);
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const uint4 v = word_to_half<false>(w[p][i]);
-                                const __half2 hi = __low2half2(sc[p][i]), lo = __high2half2(sc[p][i]);
-                                sts128(tileb + i * 16384 + p * 2048,
-                                       make_uint4(scaled(v.x, hi, lo), scaled(v.y, hi, lo), scaled(v.z, hi, lo), scaled(v.w, hi, lo)));
-                            }
-                        if (PAIR && h == 0) fetch(st * kKT + 64);
+                        for (int e = 0; e < 2; ++e) {
+                            uint4 v = word_to_half<false>((e == 0) != swap ? H.w[p].x : H.w[p].y);
+                            v = make_uint4(scaled<T>(v.x, hi, lo), scaled<T>(v.y, hi, lo), scaled<T>(v.z, hi, lo), scaled<T>(v.w, hi, lo));
+                            sts128(at + p * 2048 + (e == 0 ? xa : xb), v);
+                        }
                     }
-                    publish(s);
-                    if (st + kTurn < st1) fetch((st + kTurn) * kKT + h0 * 64);
+                };
+                const int first = st0 + (PAIR ? (group + base) & 1 : 0);
+                Half b[2];                                            // both halves of a stage, or one of two stages
+                if (first < st1) fetch(first, PAIR ? 0 : group, b[0]);
+                if (PAIR ? first < st1 : first + 1 < st1) fetch(PAIR ? first : first + 1, PAIR ? 1 : group, b[1]);
+                for (int stb = first; stb < st1 && ok; stb += 2) {
+#pragma unroll
+                    for (int a = 0; a < (PAIR ? 1 : 2); ++a) {
+                        const int st = stb + a;
+                        if (st >= st1) break;
+                        const uint32_t it = (uint32_t)(base + st - st0), s = it % kStages;
+                        ok = wait_on(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
+                        if (!ok) break;
+                        const uint32_t at = smem_base + s * kStageBytes + d0;
+                        if constexpr (PAIR) {
+                            unpack(at, b[0]);
+                            unpack(at + 8192, b[1]);
+                        } else {
+                            unpack(at + group * 8192, b[a]);
+                        }
+                        publish(s);
+                        if (st + 2 < st1) {
+                            if constexpr (PAIR) {
+                                fetch(st + 2, 0, b[0]);
+                                fetch(st + 2, 1, b[1]);
+                            } else {
+                                fetch(st + 2, group, b[a]);
+                            }
+                        }
+                    }
                 }
             }
         }
