@@ -558,9 +558,12 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                 const auto fetch = [&](int st, uint2 (&d)[kWords]) {
                     const int word = st * 16 + h0 * 8;
                     if (P.f.vec8 && st * 16 + 16 <= CP && c0 + 3 * kStep < R) {
+                        const uint32_t *src = rp + word;
 #pragma unroll
-                        for (int p = 0; p < kWords; ++p)
-                            d[p] = __ldg(reinterpret_cast<const uint2 *>(rp + (int64_t)(p & 3) * kStep * CP + word + (p >> 2) * 8));
+                        for (int p = 0; p < 4; ++p, src += kStep * CP) {
+                            d[p] = __ldg(reinterpret_cast<const uint2 *>(src));
+                            if (PAIR) d[kWords - 4 + p] = __ldg(reinterpret_cast<const uint2 *>(src + 8));
+                        }
                     } else {
 #pragma unroll
                         for (int p = 0; p < kWords; ++p) {
@@ -614,10 +617,23 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                 const bool in0 = word < CP, in1 = word + 1 < CP;
                 const uint32_t *w0 = P.d.packed[0] + word, *w1 = P.d.mats == 2 ? P.d.packed[1] + word : w0;
                 const __half2 *sp = P.d.pairs + (c >> sh);            // 16 channels lie in one group
+                // whole halves inside one matrix, and a tile inside its columns: no test and little address work per load
+                const bool whole = P.d.vec8 && tile_col(tile) + kMT <= (int)P.d.C;
                 const auto fetch = [&](int st, int h, Half &H) {
+                    const int kb = st * kKT + h * 64;
+                    if (whole && kb + 64 <= K && (kb + 64 <= R || kb >= R)) {
+                        const uint32_t *src = (kb >= R ? w1 : w0) + (int64_t)((kb >= R ? kb - R : kb) + k0) * CP;
+                        const __half2 *ss = sp + (int64_t)(kb + k0) * G;
+#pragma unroll
+                        for (int p = 0; p < 4; ++p, src += 16 * CP, ss += 16 * G) {
+                            H.w[p] = __ldg(reinterpret_cast<const uint2 *>(src));
+                            H.s[p] = __ldg(ss);
+                        }
+                        return;
+                    }
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
-                        const int k = st * kKT + h * 64 + k0 + 16 * p;
+                        const int k = kb + k0 + 16 * p;
                         const uint32_t *src = (k < R ? w0 : w1) + (int64_t)(k < R ? k : k - R) * CP;
                         uint2 v = make_uint2(kZeroWord, kZeroWord);
                         if (P.d.vec8) {
