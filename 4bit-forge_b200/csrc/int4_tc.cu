@@ -22,6 +22,12 @@
 // half of the tokens, the even one issues the MMAs for both.  One CTA alone moves 192 KB through its shared memory per
 // 128-channel step (operands written and read), 1.5 times what the 1024 cycles of the MMAs allow; a pair's CTA moves 128.
 //
+// Measured (burst clocks): gated 8192 x 7168 -> 2048 348 us (1.38 PFLOP/s, 0.85 of the measured cuBLAS burst rate; 418 us,
+// 1.15 PFLOP/s, when the power limit holds the clock down), 4096 x 2048 -> 7168 with residual 128 us (0.94 PFLOP/s), dx of
+// gated 4096 x 2048 -> 7168 200 us (1.20 PFLOP/s).  ncu on the gated kernel at 4096 tokens: tensor pipe 72 % active (84 % on
+// the SMs that have four tiles), shared memory 84 %: what bounds it is the shared-memory port, which carries both operands
+// in and out.  The smaller products end on a partly filled round of tiles (448 tiles on 74 pairs).
+//
 // With fewer tiles than SMs the K axis is shared by the CTAs of a cluster: each leaves its sums in its shared memory and
 // every CTA adds up a slice of the tokens from all of them, in rank order, over distributed shared memory.
 #include <cuda.h>
