@@ -645,3 +645,43 @@ def test_calls_from_two_threads():
     [t.start() for t in ts]
     [t.join() for t in ts]
     assert not bad
+
+
+def test_few_tokens_and_many_rows():
+    """More row tiles than SMs for one token tile: a CTA walks several tiles alone."""
+    test_linear(40, 264, 20001, 64, torch.bfloat16, "gelu")
+    test_gated(50, 136, 10300, 128, torch.float16, "silu")
+    test_linear_backward(33, 20008, 70, 32, torch.bfloat16, "relu")
+    test_gated_backward(60, 20008, 33, 128, torch.float16, "gelu")
+    test_linear(9, 64, 40003, 32, torch.float16, "none")
+
+
+@pytest.mark.parametrize("T", [2, 30, 700])
+def test_plain_gate_half_scales_and_status(T):
+    """No activation on the gate; scales kept in 16 bits; the status word stays clear."""
+    g = gen(T + 5)
+    C, R, gs = 512, 1300, 128
+    wg, sg, Wg = weight(R, C, gs, g)
+    wu, su, Wu = weight(R, C, gs, g)
+    sg, su = sg.half(), su.half()                       # as a checkpoint keeps them (weights off by 2^-11)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    x = torch.randn(T, C, generator=g, device=DEV).half()
+    h, gg, uu = ops().int4_gated(x, wg, sg, wu, su, gs, act="none", want_preact=True, status=status)
+    a, b = (ops().int4_linear(x, w, s.float(), gs, status=status) for w, s in ((wg, sg), (wu, su)))
+    # the two entry points may share the K axis among different numbers of CTAs, so their fp32 sums differ by the sums'
+    # tolerance each, and each is then rounded to fp16: half a step (2^-11) either side
+    for p, q, W in ((gg, a, Wg), (uu, b, Wu)):
+        close(p, q.double(), 2 * 2.0 ** -11 * 1.01 * q.double().abs() + 2 * 1.01 * sum_tol(x.double(), W, C // gs) + 2.0 ** -24)
+    prod = gg.double() * uu.double()
+    # g, u and h rounded: half a step relative (2^-11) each, but never less than 2^-25, half of fp16's smallest step, which g
+    # passes on times u and u times g
+    close(h, prod, 3.1 * 2.0 ** -11 * prod.abs() + 1.01 * 2.0 ** -25 * (1 + gg.double().abs() + uu.double().abs()))
+    dh = torch.randn(T, R, generator=g, device=DEV).half()
+    dx = ops().int4_gated_backward(dh, gg, uu, wg, sg, wu, su, gs, act="none", status=status)
+    dz = (dh.double() * uu.double(), dh.double() * gg.double())
+    d1, _ = ops().int4_linear_backward(dz[0].half(), wg, sg, gs, status=status)
+    d2, _ = ops().int4_linear_backward(dz[1].half(), wu, su, gs, status=status)
+    mag = sum(d.abs() @ ops().int4_packed_dequant(w ^ -0x77777778, s, (R, C), dtype=torch.float32).double().abs()
+              for d, w, s in ((dz[0], wg, sg), (dz[1], wu, su)))
+    close(dx, d1.double() + d2.double(), 5 * 2.0 ** -11 * mag + 2.0 ** -23)
+    assert int(status) == 0
