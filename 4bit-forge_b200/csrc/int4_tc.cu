@@ -196,11 +196,10 @@ template <bool BF16> __device__ __forceinline__ uint4 word_to_half(uint32_t w) {
     }
     return make_uint4(p[0], p[1], p[2], p[3]);
 }
-// W' of the backward form.  fp16 gradients: from the scale's pair, rounded once (2^-11).  bf16 gradients, rounded to 2^-8
-// themselves: from the scale's high part alone, 2^-11 more and one operation in three less for the loading warps.
-template <typename T> __device__ __forceinline__ uint32_t scaled(uint32_t v, __half2 hi, __half2 lo) {
+// W' of the backward form, from both halves of the scale and rounded once (2^-11).
+__device__ __forceinline__ uint32_t scaled(uint32_t v, __half2 hi, __half2 lo) {
     const __half2 q = *reinterpret_cast<const __half2 *>(&v);
-    const __half2 r = std::is_same<T, __half>::value ? __hfma2(q, hi, __hmul2(q, lo)) : __hmul2(q, hi);
+    const __half2 r = __hfma2(q, hi, __hmul2(q, lo));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
 
@@ -659,7 +658,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             uint4 v = word_to_half<false>((e == 0) != swap ? H.w[p].x : H.w[p].y);
-                            v = make_uint4(scaled<T>(v.x, hi, lo), scaled<T>(v.y, hi, lo), scaled<T>(v.z, hi, lo), scaled<T>(v.w, hi, lo));
+                            v = make_uint4(scaled(v.x, hi, lo), scaled(v.y, hi, lo), scaled(v.z, hi, lo), scaled(v.w, hi, lo));
                             sts128(at + p * 2048 + (e == 0 ? xa : xb), v);
                         }
                     }
