@@ -8,7 +8,9 @@
 // Backward operand: dz is the K operand of the second product and has to be a 16-bit matrix.  It is written as fp16
 // (11 bits, against bf16's 8) times a power of two per token row that puts the row's largest entry just below 2^15;
 // the product is multiplied by the inverse power at the end, so nothing but the 2^-12 relative rounding remains.  The
-// weights' scales are split the same way: a power of two per weight row goes into dz (exactly), the rest is at most 2.
+// weights' scales are split the same way, see scale_prep_kernel.
+#include <cooperative_groups.h>
+#include <utility>
 #include "common.cuh"
 #include "elem.cuh"
 #include "int4_mm.cuh"
@@ -19,27 +21,83 @@ namespace {
 
 // ---- backward preparation ------------------------------------------------------------------------------------------
 
-// Per weight row r: the power of two f[r] = 2^floor(log2 max_g |s|) and the normalised scales s / f as an fp16 pair
-// (hi, lo), hi + lo = s / f to 22 bits.  One warp per row.
-__global__ void __launch_bounds__(256) scale_prep_kernel(const float *__restrict__ s0, const float *__restrict__ s1,
-                                                         int64_t R, int64_t G, __half2 *__restrict__ pairs,
-                                                         float *__restrict__ f) {
-    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int64_t rows = s1 ? 2 * R : R;
-    if (row >= rows) return;
-    const int lane = threadIdx.x & 31;
-    const float *s = (row < R ? s0 + row * G : s1 + (row - R) * G);
-    float m = 0.0f;
-    for (int64_t g = lane; g < G; g += 32) m = fmaxf(m, fabsf(s[g]));
+// Scales of the backward operand.  K is the weight rows (gate and up one after the other), in blocks of kKBlock.
+//   f[k]     = 2^floor(log2 max_g |s[k, g]|)                            a row's power, moved into dz
+//   e        = floor(log2 max over the block's k of |s[k, g]| / f[k])   a channel group's, one per block of rows
+//   s'[k, g] = s[k, g] / f[k] 2^(11 - e) <= 2^12                        as an fp16 pair (hi, lo)
+//   group[block, g] = 2^(e - 11)                                        undone where the block's sums are added up
+// Both are powers of two, so they cost no bits.  With 2^12 at the top a product (nibble - 8) s' stays below 2^15, and it is a
+// normal fp16 number down to 2^-25 of its block's largest scale: only a scale that far below its row's AND below its block's
+// group loses bits.  A cluster takes a block, a CTA of it 64 rows and a warp four: the rows' powers stay in the warp, the
+// groups' maxima meet in shared memory.  Nothing but latency: 2048 rows of 32 groups take 4.7 us (one CTA per block: 20 us; without the
+// groups' powers, a warp a row: 2.2 us), 2 x 2048 rows of 56 groups 6.3 us.
+constexpr int kPrepCtas = 8, kPrepRows = 4, kPrepGroups = 1024;      // a cluster's CTAs, a warp's rows, groups at a time
+static_assert(kPrepCtas * 16 * kPrepRows == kKBlock, "a cluster of 16 warps a CTA covers a block");
+__device__ __forceinline__ int exponent_of(float v) { return (int)((__float_as_uint(v) >> 23) & 255u) - 127; }
+__device__ __forceinline__ float finite_abs(float v) { return isfinite(v) ? fabsf(v) : 0.0f; }
+
+__global__ void __cluster_dims__(kPrepCtas) __launch_bounds__(512)
+scale_prep_kernel(const float *__restrict__ s0, const float *__restrict__ s1, int64_t R, int64_t K, int64_t G,
+                  __half2 *__restrict__ pairs, float *__restrict__ f, float *__restrict__ group) {
+    __shared__ int top[kPrepGroups];          // largest s / f, as the bits of a float that is not negative
+    __shared__ float power[kPrepGroups];      // 2^(11 - e)
+    const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t k0 = (int64_t)blockIdx.x * (16 * kPrepRows) + warp * kPrepRows, block = blockIdx.x / kPrepCtas;
+    const float *row[kPrepRows];
+    float m[kPrepRows], inv[kPrepRows];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const int e = (m > 0.0f && isfinite(m)) ? ilogbf(m) : 0;
-    for (int64_t g = lane; g < G; g += 32) {
-        const float v = scalbnf(s[g], -e);
-        const __half hi = __float2half_rn(v);
-        pairs[row * G + g] = __halves2half2(hi, __float2half_rn(v - __half2float(hi)));
+    for (int i = 0; i < kPrepRows; ++i) {
+        const int64_t k = k0 + i < K ? k0 + i : K - 1;
+        row[i] = k < R ? s0 + k * G : s1 + (k - R) * G;
+        m[i] = 0.0f;
     }
-    if (lane == 0) f[row] = scalbnf(1.0f, e);
+#pragma unroll 2
+    for (int64_t g = lane; g < G; g += 32)
+#pragma unroll
+        for (int i = 0; i < kPrepRows; ++i) m[i] = fmaxf(m[i], finite_abs(row[i][g]));
+#pragma unroll
+    for (int i = 0; i < kPrepRows; ++i) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], o));
+        const int e = m[i] > 0.0f ? exponent_of(m[i]) : 0;
+        inv[i] = scalbnf(1.0f, -e);
+        if (lane == 0 && k0 + i < K) f[k0 + i] = scalbnf(1.0f, e);
+    }
+    for (int64_t g0 = 0; g0 < G; g0 += kPrepGroups) {
+        const int n = (int)imin64(G - g0, kPrepGroups);
+        for (int g = threadIdx.x; g < n; g += 512) top[g] = 0;
+        __syncthreads();
+#pragma unroll 2
+        for (int g = lane; g < n; g += 32) {
+            float t = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kPrepRows; ++i)
+                if (k0 + i < K) t = fmaxf(t, finite_abs(row[i][g0 + g]) * inv[i]);
+            atomicMax(top + g, __float_as_int(t));
+        }
+        cluster.sync();
+        for (int g = threadIdx.x; g < n; g += 512) {
+            int t = 0;
+#pragma unroll
+            for (int r = 0; r < kPrepCtas; ++r) t = max(t, *cluster.map_shared_rank(top + g, r));
+            const int e = t == 0 ? 0 : max(exponent_of(__int_as_float(t)), -100);      // (2^(e - 11) stays a normal number)
+            power[g] = scalbnf(1.0f, 11 - e);
+            if (cluster.block_rank() == 0) group[block * G + g0 + g] = scalbnf(1.0f, e - 11);
+        }
+        auto read = cluster.barrier_arrive();
+        __syncthreads();
+#pragma unroll 2
+        for (int g = lane; g < n; g += 32)
+#pragma unroll
+            for (int i = 0; i < kPrepRows; ++i)
+                if (k0 + i < K) {
+                    const float v = row[i][g0 + g] * inv[i] * power[g];
+                    const __half hi = __float2half_rn(v);
+                    pairs[(k0 + i) * G + g0 + g] = __halves2half2(hi, __float2half_rn(v - __half2float(hi)));
+                }
+        cluster.barrier_wait(std::move(read));        // nobody clears or leaves its maxima while they are read
+    }
 }
 
 struct DzParams {
@@ -248,7 +306,7 @@ bool rows_ok(const void *p, int64_t ld, int64_t n, int64_t T) {
 }
 
 struct BwdLayout {       // byte offsets into the workspace of a backward pass
-    int64_t ldk, a, unscale, pairs, f, partial, total;
+    int64_t ldk, a, unscale, pairs, f, group, partial, total;
 };
 BwdLayout bwd_layout(int64_t T, int64_t C, int64_t R, int gs, int mats) {
     BwdLayout L{};
@@ -258,7 +316,8 @@ BwdLayout bwd_layout(int64_t T, int64_t C, int64_t R, int gs, int mats) {
     L.unscale = up(T * L.ldk * 2);
     L.pairs = L.unscale + up(T * 4);
     L.f = L.pairs + up(mats * R * cdiv(C, (int64_t)gs) * 4);
-    L.partial = L.f + up(mats * R * 4);
+    L.group = L.f + up(mats * R * 4);
+    L.partial = L.group + up(cdiv(mats * R, (int64_t)kKBlock) * cdiv(C, (int64_t)gs) * 4);
     L.total = L.partial + up((T < kRowCtas ? (T < kBiasParts ? kBiasParts : T) : kRowCtas) * R * 4);
     return L;
 }
@@ -365,8 +424,8 @@ static int backward(const char *who, const void *dy, int64_t lddy, int dtype, co
     int parts = 0;
     const int64_t G = cdiv(C, (int64_t)gs);
     if (dx && T > 0) {
-        scale_prep_kernel<<<(unsigned)cdiv(mats * R, (int64_t)8), 256, 0, st>>>(s0, s1, R, G, (__half2 *)(base + L.pairs),
-                                                                                (float *)(base + L.f));
+        scale_prep_kernel<<<(unsigned)cdiv(mats * R, (int64_t)kKBlock) * kPrepCtas, 512, 0, st>>>(
+            s0, s1, R, mats * R, G, (__half2 *)(base + L.pairs), (float *)(base + L.f), (float *)(base + L.group));
         FORGE_NOTE_LAUNCH();
         DzParams D{dy, z, u, lddy, T, R, mats * R, L.ldk, (const float *)(base + L.f), (__half *)(base + L.a),
                    (float *)(base + L.unscale)};
@@ -386,7 +445,8 @@ static int backward(const char *who, const void *dy, int64_t lddy, int dtype, co
     }
     if (!dx || T == 0) return check_launch(who);
     Int4Dgrad P{(const __half *)(base + L.a), L.ldk, (const float *)(base + L.unscale),
-                {(const uint32_t *)p0, (const uint32_t *)p1}, (const __half2 *)(base + L.pairs), gs, mats, T, C, R, G, dx, status,
+                {(const uint32_t *)p0, (const uint32_t *)p1}, (const __half2 *)(base + L.pairs), (const float *)(base + L.group),
+                gs, mats, T, C, R, G, dx, status,
                 C % 16 == 0 && ((uintptr_t)p0 | (uintptr_t)p1) % 8 == 0};
     return int4_dgrad_tc(P, dtype == FORGE_DTYPE_BF16, who, st);
 }

@@ -29,6 +29,7 @@ struct Int4Dgrad {
     const float *unscale;        // [T]
     const uint32_t *packed[2];
     const __half2 *pairs;        // [mats * R, G]: normalised scales, hi and lo part
+    const float *group;          // [ceil(mats * R / kKBlock), G]: powers of two that the sums of a block of rows take
     int gs, mats;
     int64_t T, C, R, G;
     void *dx;                    // [T, C]
@@ -36,6 +37,7 @@ struct Int4Dgrad {
     bool vec8;                   // rows of packed words start on 8 bytes
 };
 
+constexpr int kKBlock = 512;           // weight rows whose products are summed up before they enter dx
 constexpr int kDecodeTokens = 16;      // most tokens that int4_decode takes
 // more tokens than int4_decode takes; the backward product
 int int4_fwd_tc(const Int4Fwd &P, bool bf16, bool gated, cudaStream_t st);

@@ -11,7 +11,8 @@
 //
 // Backward (dx = dz W): M is the channels, read along the rows of W (an MN-major operand), K the weight rows.  A chunk has
 // many scales there, so they have to be in the operand: W' = fp16((nibble - 8) * s'), s' the scale without its row's power
-// of two (which dz carries exactly), kept as an fp16 pair (hi, lo).  Chunks of 512 weight rows are added up in registers.
+// of two (which dz carries exactly) and without that of its channel group in the chunk, kept as an fp16 pair (hi, lo).  Chunks
+// of 512 weight rows are added up in registers, times the group's power: again one factor for a thread, which has one channel.
 //
 // A CTA (one per SM, 640 threads): warps 0-7 add finished chunks to the sums and run the epilogue, warps 8-11 and 12-15
 // turn packed words into 16-bit operand tiles, one stage each in turn (words read ahead into registers, tiles written with
@@ -138,11 +139,6 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     uint64_t d;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
 __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
@@ -299,7 +295,7 @@ __device__ __forceinline__ void rows8(uint32_t buf, int token, int row, float (&
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
 
-// T: output type; MODE; CH: channels per chunk (forward: the group size; backward: 512 weight rows); NT: tokens per tile;
+// T: output type; MODE; CH: channels per chunk (forward: the group size; backward: kKBlock weight rows); NT: tokens per tile;
 // PAIR: two CTAs per tile
 template <typename T, int MODE, int CH, int NT, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_constant__ TcParams P,
@@ -380,6 +376,10 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                 sp = P.f.scales[MODE == kGated && lane >= 16 ? 1 : 0] + (int64_t)row * P.f.G + g;
                 left = (int)P.f.G - g;
                 s_next = left > 0 ? __ldg(sp) : 0.0f;
+            } else {
+                const int c = min(tile_col(tile) + quarter * 32 + lane, (int)P.d.C - 1);
+                sp = P.d.group + (int64_t)(st0 / kStagesPer) * P.d.G + c / P.d.gs;
+                s_next = __ldg(sp);
             }
             if (MODE == kLinear && P.split == 1 && P.f.res) {         // the residual's lines, long before the epilogue reads them
 #pragma unroll
@@ -389,13 +389,17 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                         asm volatile("prefetch.global.L2 [%0];" ::"l"((const T *)P.f.res + t * P.f.ldres + c));
                 }
             }
-            const int nch = (st1 - st0 + kStagesPer - 1) / kStagesPer * kPerStage;
+            // chunks end at multiples of kStagesPer stages, wherever this CTA's share of them begins
+            const int nch = st1 > st0 ? ((st1 - 1) / kStagesPer - st0 / kStagesPer + 1) * kPerStage : 0;
             for (int ch = 0; ch < nch; ++ch, ++chunk) {
                 const uint32_t buf = chunk & 1u;
                 const float sc = s_next;
                 if constexpr (MODE != kDgrad) {
                     ++sp;
                     s_next = --left > 0 ? __ldg(sp) : 0.0f;
+                } else if (ch + 1 < nch) {
+                    sp += P.d.G;
+                    s_next = __ldg(sp);
                 }
                 ok = wait_on(b_afull + 8 * buf, (chunk >> 1) & 1u, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
@@ -416,10 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                         }
                     }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        if constexpr (MODE == kDgrad) acc[j * 8 + i] = add2(acc[j * 8 + i], pack2(v[2 * i], v[2 * i + 1]));
-                        else acc[j * 8 + i] = fma2(pack2(v[2 * i], v[2 * i + 1]), sc2, acc[j * 8 + i]);
-                    }
+                    for (int i = 0; i < 8; ++i) acc[j * 8 + i] = fma2(pack2(v[2 * i], v[2 * i + 1]), sc2, acc[j * 8 + i]);
                 }
             }
             if (!ok) break;
@@ -737,8 +738,8 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after();
-                    const bool first_stage = (st - st0) % kStagesPer == 0;
-                    const bool last_stage = (st - st0) % kStagesPer == kStagesPer - 1 || st + 1 == st1;
+                    const bool first_stage = st % kStagesPer == 0 || st == st0;
+                    const bool last_stage = st % kStagesPer == kStagesPer - 1 || st + 1 == st1;
                     const uint64_t ad = ad0 + (uint64_t)(s * (kStageBytes >> 4)), bd = bd0 + (uint64_t)(s * (kStageBytes >> 4));
 #pragma unroll
                     for (int e = 0; e < kPerStage; ++e) {
@@ -921,7 +922,7 @@ int int4_dgrad_tc(const Int4Dgrad &D, bool bf16, const char *who, cudaStream_t s
     P.d = D; P.T = D.T; P.N = D.C; P.status = D.status;
     P.nst = (int)cdiv(D.ldk, (int64_t)kKT);
     const TokenSource src{D.a, false, D.T, D.ldk, D.ldk};
-    return bf16 ? launch_nt<__nv_bfloat16, kDgrad, 512>(P, src, who, st) : launch_nt<__half, kDgrad, 512>(P, src, who, st);
+    return bf16 ? launch_nt<__nv_bfloat16, kDgrad, kKBlock>(P, src, who, st) : launch_nt<__half, kDgrad, kKBlock>(P, src, who, st);
 }
 
 }  // namespace forge

@@ -534,7 +534,8 @@ def int4_linear_backward(dy, packed, scales, gs: int = 128, preact=None, act: st
                          want_dbias: bool = False, status=None):
     """Gradients of int4_linear for frozen weights: dz = dy * act'(preact); returns (dx, dbias), dx = dz W [T, C] and
     dbias = the column sums of dz [R], both of dy's type, None where not wanted.  preact is the z of the forward call
-    (not needed with act="none"); the residual's gradient is dy itself (forge_int4_linear_backward)."""
+    (not needed with act="none"); the residual's gradient is dy itself (forge_int4_linear_backward).  dz and W are rounded to
+    fp16 (2^-11 each) after powers of two are taken out of dz's rows and of W's rows and channel groups; sums in fp32."""
     dev = _on_device(dy, "dy")
     if dev is None:
         with torch.cuda.device(dy.device):
@@ -586,7 +587,8 @@ def int4_gated(x, gate_packed, gate_scales, up_packed, up_scales, gs: int = 128,
 def int4_gated_backward(dh, g, u, gate_packed, gate_scales, up_packed, up_scales, gs: int = 128, act: str = "silu",
                         status=None):
     """Gradient of int4_gated for frozen weights, at the g and u of the forward call:
-    dx = (dh * u * act'(g)) Wg + (dh * act(g)) Wu, [T, C] of dh's type (forge_int4_gated_backward)."""
+    dx = (dh * u * act'(g)) Wg + (dh * act(g)) Wu, [T, C] of dh's type (forge_int4_gated_backward).  Rounded on the way like
+    int4_linear_backward."""
     dev = _on_device(dh, "dh")
     if dev is None:
         with torch.cuda.device(dh.device):

@@ -47,3 +47,59 @@ def test_both_halves_of_the_scale_reach_the_gradient(T, dt):
         assert bool((dx == 386).all()), dx.unique()
     else:
         assert bool(((dx.double() - want).abs() <= 2.0 ** -11 * want).all()), dx.unique()
+
+
+def spread_scales(R, C, gs, g, ratio, where):
+    """Scales of one size, but for the channels of the first group: in every row, in one block of 512 rows and in the rows
+    behind it, or in every row by another power of two, they are `ratio` of the others."""
+    s = torch.rand(R, C // gs, generator=g, device=DEV) + 0.5
+    if where == "group":
+        s[:, 0] *= ratio
+    elif where == "block":
+        s[512:, 0] *= ratio
+        s[:512, 0] = 0                       # (their products would hide the small ones)
+    else:
+        s[:, 0] *= ratio
+        s *= 2.0 ** torch.randint(-20, 21, (R, 1), generator=g, device=DEV)
+    return s
+
+
+@pytest.mark.parametrize("T", [3, 70, 1500])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("where", ["group", "block", "rows"])
+@pytest.mark.parametrize("power", [-13, -16, -20, -26, -40])
+def test_groups_of_small_scales_keep_their_gradient(T, dt, where, power):
+    """The channels whose scales are far below those of the rest of their rows, judged by themselves.  fp16 gradients are
+    scaled so that the small group's are of ordinary size (the others may overflow)."""
+    R, C, gs = 1100, 2560, 128
+    g = torch.Generator(device=DEV).manual_seed(1000 * T - power)
+    lift = 2.0 ** -power if dt == torch.float16 else 1.0
+
+    def matrix():
+        codes = torch.randint(0, 16, (R, C), generator=g, device=DEV)
+        s = spread_scales(R, C, gs, g, 2.0 ** power, where) * lift
+        return words(codes), s, (codes[:, :gs].double() - 8) * s[:, :1].double()
+    (p0, s0, W0), (p1, s1, W1) = matrix(), matrix()
+    dy = torch.randn(T, R, generator=g, device=DEV).to(dt)
+    if where == "rows":                      # terms of one size, as the powers of the rows meet those of the gradient
+        dy = (dy.double() * 2.0 ** -14).to(dt)
+    dx = ops().int4_linear_backward(dy, p0, s0, gs)[0][:, :gs].double()
+    want = dy.double() @ W0
+    assert float((dx - want).norm() / want.norm()) <= norm_bound(dt)
+    gate, up = (torch.randn(T, R, generator=g, device=DEV).to(dt) for _ in range(2))
+    dx = ops().int4_gated_backward(dy, gate, up, p0, s0, p1, s1, gs, act="relu")[:, :gs].double()
+    on = (gate > 0).double()
+    want = (dy.double() * up.double() * on) @ W0 + (dy.double() * gate.double() * on) @ W1
+    assert float((dx - want).norm() / want.norm()) <= norm_bound(dt)
+
+
+def test_scales_of_more_groups_than_fit_at_a_time():
+    R, C, gs, T = 700, 40000, 32, 5
+    g = torch.Generator(device=DEV).manual_seed(9)
+    codes = torch.randint(0, 16, (R, C), generator=g, device=DEV)
+    s = (torch.rand(R, C // gs, generator=g, device=DEV) + 0.5) * 2.0 ** (-30 * torch.rand(1, C // gs, generator=g, device=DEV))
+    dy = torch.randn(T, R, generator=g, device=DEV).to(torch.bfloat16)
+    dx = ops().int4_linear_backward(dy, words(codes), s, gs)[0].double().view(T, -1, gs)
+    want = (dy.double() @ ((codes.double() - 8) * s.double().repeat_interleave(gs, 1))).view(T, -1, gs)
+    # group by group: 160 entries each, so the ratio of two norms spreads by a tenth more
+    assert float(((dx - want).norm(dim=(0, 2)) / want.norm(dim=(0, 2))).max()) <= 1.5 * norm_bound(torch.bfloat16)
