@@ -126,7 +126,8 @@ class Int4FeedForward(torch.nn.Module):
         forward(hidden)            -> down(act(gate(x)) * up(x)) [+ hidden],   x = norm(hidden)
         forward(hidden, residual)  -> the same with hidden + residual in hidden's place
 
-    gate, up [I, H/8] and down [H, I/8] are (weight_packed, scales) pairs.  With norm_weight [H] the block starts with a
+    gate, up [I, H/8] and down [H, I/8] are (weight_packed, scales) pairs, kept as they are given where they are contiguous
+    (and the scales fp32).  With norm_weight [H] the block starts with a
     root-mean-square norm and its result is added to the residual stream (four kernels less one: norm, gated product,
     product with the residual in its epilogue); without one it is the bare block and takes no residual.  The int4 weights
     are frozen; gradients reach hidden, residual and the norm's gain (tuning through the quantised block).  The reference
@@ -155,11 +156,11 @@ class Int4FeedForward(torch.nn.Module):
     @classmethod
     def from_quantized(cls, out, index, group_size=128, **kw):
         """Matrix `index` of every family of MoELayerQuantizer.quantize_experts(...) (cfg.pack, symmetric, "gptq"): routed
-        experts first, then the shared ones."""
+        experts first, then the shared ones.  The block copies its matrices out of the batch."""
         pairs = []
         for fam in ("gate", "up", "down"):
-            packed = out[fam]["weight_packed"][index]
-            pairs.append((packed, out[fam]["scales"][index].view(packed.shape[0], -1)))
+            packed = out[fam]["weight_packed"][index].clone()
+            pairs.append((packed, out[fam]["scales"][index].reshape(packed.shape[0], -1).to(torch.float32, copy=True)))
         return cls(*pairs, group_size=group_size, **kw)
 
     def forward(self, hidden, residual=None):
