@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import torch
 
-from . import ops
+from . import _abi, ops
 
 
 class Sparse14MoERuntime:
@@ -136,12 +136,22 @@ class Int4FeedForward(torch.nn.Module):
     def __init__(self, gate, up, down, group_size=128, act="silu", norm_weight=None, eps=1e-6):
         super().__init__()
         self.group_size, self.act, self.eps = int(group_size), act, float(eps)
+        gs = self.group_size
+        if gs not in (32, 64, 128) or act not in _abi.ACTS:
+            raise RuntimeError(f"group size must be 32, 64 or 128 and act one of {', '.join(_abi.ACTS)}")
         for name, (packed, scales) in (("gate", gate), ("up", up), ("down", down)):
+            if packed.dim() != 2 or packed.dtype != torch.int32:
+                raise RuntimeError(f"{name} must be packed words, int32 [R, C/8], got {packed.dtype} {list(packed.shape)}")
+            want = (packed.shape[0], -(-packed.shape[1] * 8 // gs))
+            if scales.shape != want:
+                raise RuntimeError(f"the scales of {name} must be [R, ceil(C/{gs})] = {list(want)}, got {list(scales.shape)}")
             self.register_buffer(name + "_packed", packed.contiguous())
             self.register_buffer(name + "_scales", scales.to(torch.float32).contiguous())
         I, H8 = self.gate_packed.shape
         if self.up_packed.shape != (I, H8) or self.down_packed.shape != (H8 * 8, I // 8) or I % 8:
             raise RuntimeError("gate and up must be [I, H/8] and down [H, I/8] packed words")
+        if norm_weight is not None and norm_weight.shape != (H8 * 8,):
+            raise RuntimeError(f"norm_weight must be [{H8 * 8}], got {list(norm_weight.shape)}")
         self.norm_weight = None if norm_weight is None else torch.nn.Parameter(norm_weight.detach().clone())
 
     def _apply(self, fn, recurse=True):
@@ -156,12 +166,35 @@ class Int4FeedForward(torch.nn.Module):
     @classmethod
     def from_quantized(cls, out, index, group_size=128, **kw):
         """Matrix `index` of every family of MoELayerQuantizer.quantize_experts(...) (cfg.pack, symmetric, "gptq"): routed
-        experts first, then the shared ones.  The block copies its matrices out of the batch."""
+        experts first, then the shared ones.  The block copies its matrices out of the batch.  Codes that the packed words
+        do not hold (asymmetric ones, more than 4 bits) are refused."""
         pairs = []
         for fam in ("gate", "up", "down"):
-            packed = out[fam]["weight_packed"][index].clone()
-            pairs.append((packed, out[fam]["scales"][index].reshape(packed.shape[0], -1).to(torch.float32, copy=True)))
-        return cls(*pairs, group_size=group_size, **kw)
+            r = out[fam]
+            if "weight_packed" not in r:
+                raise RuntimeError(f"{fam} holds no packed int4 words: quantise with pack=True and algorithm 'gptq'")
+            packed = r["weight_packed"][index].clone()
+            scales = r["scales"][index].reshape(packed.shape[0], -1).to(torch.float32, copy=True)
+            pairs.append((packed, scales))
+        block = cls(*pairs, group_size=group_size, **kw)
+        for fam in ("gate", "up", "down"):
+            if not cls._nibbles_hold(out[fam], index, block.group_size):
+                raise RuntimeError(f"the codes of {fam} cannot be read back from its packed words: they are not symmetric "
+                                   "codes of 4 bits or fewer")
+        return block
+
+    @staticmethod
+    def _nibbles_hold(result, index, group_size):
+        """Whether every code of the matrix is within -8 .. 7 of its zero point, so that its nibble is the code's own: from
+        the codes where the result keeps them, else for zero points that are all those of symmetric codes of 2, 3 or 4
+        bits.  One read by the host."""
+        z, q = result["qzeros"][index], result.get("qweight")
+        if q is None:
+            return any(torch.stack([(z == v).all() for v in (2, 4, 8)]).tolist())
+        q = q[index]
+        z = z.reshape(q.shape[0], -1).to(torch.int16).repeat_interleave(group_size, 1)[:, :q.shape[1]]
+        d = q.to(torch.int16) - z
+        return bool(((d >= -8) & (d <= 7)).all())
 
     def forward(self, hidden, residual=None):
         if residual is not None and self.norm_weight is None:

@@ -44,3 +44,46 @@ def test_a_block_of_a_batch_owns_its_matrices():
     for n, b in blk.named_buffers():
         assert torch.equal(b, want[n]), n
     assert torch.equal(blk.gate_scales, quantised()["gate"]["scales"][2])
+
+
+def test_codes_that_a_nibble_does_not_hold_are_refused():
+    for keep in (True, False):
+        with pytest.raises(RuntimeError, match="symmetric"):
+            block(quantised(symmetric=False, keep_codes=keep))
+        with pytest.raises(RuntimeError, match="symmetric"):
+            block(quantised(bits=8, keep_codes=keep))
+        for bits in (2, 3, 4):
+            block(quantised(bits=bits, keep_codes=keep))
+    # one zero point of one matrix, and only for the expert that has it
+    for fam in ("gate", "up", "down"):
+        out = quantised(keep_codes=False)
+        out[fam]["qzeros"][2, 5, 1] = 7
+        block(out, 1)
+        with pytest.raises(RuntimeError, match=fam):
+            block(out, 2)
+    # an asymmetric matrix whose codes all lie within a nibble of their zero point reads back exactly
+    out = quantised()
+    out["up"]["qzeros"][2, 0, 0] = 5
+    out["up"]["qweight"][2, 0, :GS] = 9
+    block(out)
+    # a sparse result, or one that was not packed
+    out = quantised()
+    del out["down"]["weight_packed"]
+    with pytest.raises(RuntimeError, match="pack"):
+        block(out)
+
+
+def test_sizes_that_do_not_fit_are_refused_at_construction():
+    from forge.inference import Int4FeedForward
+    out = quantised()
+    for kw in (dict(group_size=64), dict(group_size=128), dict(group_size=16), dict(group_size=0), dict(act="tanh"),
+               dict(norm_weight=torch.ones(H + 1)), dict(norm_weight=torch.ones(1, H))):
+        with pytest.raises(RuntimeError):
+            block(out, **kw)
+    parts = [(out[f]["weight_packed"][0], out[f]["scales"][0]) for f in ("gate", "up", "down")]
+    Int4FeedForward(*parts, group_size=GS)
+    for k in range(3):
+        for bad in ((parts[k][0], parts[k][1][:, :-1]), (parts[k][0], parts[k][1].t()), (parts[k][0].long(), parts[k][1]),
+                    (parts[k][0][0], parts[k][1])):
+            with pytest.raises(RuntimeError):
+                Int4FeedForward(*[bad if i == k else p for i, p in enumerate(parts)], group_size=GS)
