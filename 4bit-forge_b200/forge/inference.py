@@ -80,12 +80,13 @@ class _RMSNorm(torch.autograd.Function):
 
 class _Int4Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, bias, residual, packed, scales, gs, act):
+    def forward(ctx, x, bias, residual, packed, scales, gs, act, status):
         want = act != "none"
-        out = ops.int4_linear(x, packed, scales, gs, bias=bias, act=act, residual=residual, want_preact=want)
+        out = ops.int4_linear(x, packed, scales, gs, bias=bias, act=act, residual=residual, want_preact=want,
+                              status=status)
         y, z = out if want else (out, None)
         ctx.save_for_backward(z, packed, scales)
-        ctx.gs, ctx.act = gs, act
+        ctx.gs, ctx.act, ctx.status = gs, act, status
         return y
 
     @staticmethod
@@ -96,23 +97,24 @@ class _Int4Linear(torch.autograd.Function):
         dx = db = None
         if need_x or need_b:
             dx, db = ops.int4_linear_backward(dy, packed, scales, ctx.gs, preact=z, act=ctx.act, want_dx=need_x,
-                                              want_dbias=need_b)
-        return dx, db, dy if need_r else None, None, None, None, None
+                                              want_dbias=need_b, status=ctx.status)
+        return dx, db, dy if need_r else None, None, None, None, None, None
 
 
 class _Int4Gated(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, wg, sg, wu, su, gs, act):
-        h, g, u = ops.int4_gated(x, wg, sg, wu, su, gs, act=act, want_preact=True)
+    def forward(ctx, x, wg, sg, wu, su, gs, act, status):
+        h, g, u = ops.int4_gated(x, wg, sg, wu, su, gs, act=act, want_preact=True, status=status)
         ctx.save_for_backward(g, u, wg, sg, wu, su)
-        ctx.gs, ctx.act = gs, act
+        ctx.gs, ctx.act, ctx.status = gs, act, status
         return h
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
         g, u, wg, sg, wu, su = ctx.saved_tensors
-        return ops.int4_gated_backward(dh, g, u, wg, sg, wu, su, ctx.gs, act=ctx.act), None, None, None, None, None, None
+        dx = ops.int4_gated_backward(dh, g, u, wg, sg, wu, su, ctx.gs, act=ctx.act, status=ctx.status)
+        return dx, None, None, None, None, None, None, None
 
 
 def _grad_wanted(*tensors):
@@ -130,7 +132,8 @@ class Int4FeedForward(torch.nn.Module):
     (and the scales fp32).  With norm_weight [H] the block starts with a
     root-mean-square norm and its result is added to the residual stream (four kernels less one: norm, gated product,
     product with the residual in its epilogue); without one it is the bare block and takes no residual.  The int4 weights
-    are frozen; gradients reach hidden, residual and the norm's gain (tuning through the quantised block).  The reference
+    are frozen; gradients reach hidden, residual and the norm's gain (tuning through the quantised block).  `status` (int32,
+    on the block's device, not part of the state dict) collects what the kernels report; check() reads it.  The reference
     runs its packed dense experts through vLLM and has no such block of its own."""
 
     def __init__(self, gate, up, down, group_size=128, act="silu", norm_weight=None, eps=1e-6):
@@ -153,14 +156,31 @@ class Int4FeedForward(torch.nn.Module):
         if norm_weight is not None and norm_weight.shape != (H8 * 8,):
             raise RuntimeError(f"norm_weight must be [{H8 * 8}], got {list(norm_weight.shape)}")
         self.norm_weight = None if norm_weight is None else torch.nn.Parameter(norm_weight.detach().clone())
+        self.status = torch.zeros(1, dtype=torch.int32, device=self.gate_packed.device)
+
+    def check(self):
+        """Raises when a kernel of an earlier call of this block, forward or backward, reported a failure (a bounded wait
+        that ran out): what that call returned is not valid.  Reads one word from the device, so it waits for the calls
+        on the current stream; it is left to the caller, once a step or once a request, and cannot be captured."""
+        code = int(self.status)
+        if code != 0:
+            self.status.zero_()
+            raise RuntimeError("forge.inference: " + ("a bounded device-side wait ran out (FORGE_ERR_TIMEOUT)"
+                               if code == _abi.ERR_TIMEOUT else f"a kernel reported status {code}")
+                               + "; results of this block since the last check are not valid")
 
     def _apply(self, fn, recurse=True):
-        """Module.to(dtype), .half() and the like move the scales but leave them in fp32: they are part of the codes."""
+        """Module.to(dtype), .half() and the like move the scales but leave them in fp32: they are part of the codes.  The
+        status word goes with them to another device and stays where it is otherwise (captured graphs write to it)."""
+        status, dev = self.status, self.gate_packed.device
         kept = {name: getattr(self, name) for name in ("gate_scales", "up_scales", "down_scales")}
         super()._apply(fn, recurse)
         for name, scales in kept.items():
             if getattr(self, name).dtype != torch.float32:
                 setattr(self, name, scales.to(getattr(self, name).device))
+        if self.gate_packed.device != dev:
+            new = self.gate_packed.device
+            self.status = torch.zeros(1, dtype=torch.int32, device=new) if dev.type == "meta" else status.to(new)
         return self
 
     @classmethod
@@ -202,7 +222,7 @@ class Int4FeedForward(torch.nn.Module):
         shape = hidden.shape
         x = hidden.reshape(-1, shape[-1])
         res = None if residual is None else residual.reshape(-1, shape[-1])
-        w, gs, act = self.norm_weight, self.group_size, self.act
+        w, gs, act, status = self.norm_weight, self.group_size, self.act, self.status
         gate = (self.gate_packed, self.gate_scales, self.up_packed, self.up_scales, gs)
         down = (self.down_packed, self.down_scales, gs)
         if _grad_wanted(x, res, w):
@@ -211,8 +231,8 @@ class Int4FeedForward(torch.nn.Module):
             else:
                 y, h = _RMSNorm.apply(x, w, res, self.eps)
                 h = x if h is None else h
-            a = _Int4Gated.apply(y, *gate, act)
-            out = _Int4Linear.apply(a, None, h, *down, "none")
+            a = _Int4Gated.apply(y, *gate, act, status)
+            out = _Int4Linear.apply(a, None, h, *down, "none", status)
         else:
             if w is None:
                 y, h = x, None
@@ -220,5 +240,5 @@ class Int4FeedForward(torch.nn.Module):
                 y, h = ops.rmsnorm(x, w, self.eps), x
             else:
                 y, h = ops.rmsnorm(x, w, self.eps, residual=res)
-            out = ops.int4_linear(ops.int4_gated(y, *gate, act=act), *down, residual=h)
+            out = ops.int4_linear(ops.int4_gated(y, *gate, act=act, status=status), *down, residual=h, status=status)
         return out.view(shape)

@@ -87,3 +87,76 @@ def test_sizes_that_do_not_fit_are_refused_at_construction():
                     (parts[k][0][0], parts[k][1])):
             with pytest.raises(RuntimeError):
                 Int4FeedForward(*[bad if i == k else p for i, p in enumerate(parts)], group_size=GS)
+
+
+class FakeOps:
+    """Shapes of the operators, and the status word that each call was given."""
+
+    def __init__(self):
+        self.calls = []
+
+    def rmsnorm(self, x, w, eps, residual=None):
+        return x.clone() if residual is None else (x.clone(), x + residual)
+
+    def rmsnorm_backward(self, dy, x, w, eps, dresidual=None):
+        return dy.clone(), torch.zeros_like(w)
+
+    def int4_linear(self, x, packed, scales, gs, bias=None, act="none", residual=None, want_preact=False, status=None):
+        self.calls.append(("linear", status))
+        return x.new_zeros(x.shape[0], packed.shape[0])
+
+    def int4_gated(self, x, wg, sg, wu, su, gs, act="silu", want_preact=False, status=None):
+        self.calls.append(("gated", status))
+        h = x.new_zeros(x.shape[0], wg.shape[0])
+        return (h, h.clone(), h.clone()) if want_preact else h
+
+    def int4_linear_backward(self, dy, packed, scales, gs, preact=None, act="none", want_dx=True, want_dbias=False, status=None):
+        self.calls.append(("linear backward", status))
+        return dy.new_zeros(dy.shape[0], packed.shape[1] * 8), None
+
+    def int4_gated_backward(self, dh, g, u, wg, sg, wu, su, gs, act="silu", status=None):
+        self.calls.append(("gated backward", status))
+        return dh.new_zeros(dh.shape[0], wg.shape[1] * 8)
+
+
+def test_every_product_reports_to_the_status_word(monkeypatch):
+    from forge import inference
+    fake = FakeOps()
+    monkeypatch.setattr(inference, "ops", fake)
+    for kw in ({}, {"norm_weight": torch.ones(H)}):
+        blk = block(quantised(), **kw)
+        for grad in (False, True):
+            fake.calls.clear()
+            x = torch.zeros(3, H, requires_grad=grad)
+            y = blk(x, residual=torch.zeros(3, H)) if kw else blk(x)
+            want = {"linear", "gated"}
+            if grad:
+                y.sum().backward()
+                want |= {"linear backward", "gated backward"}
+            elif kw:
+                assert y.requires_grad           # (through the gain)
+            assert {name for name, _ in fake.calls} == want
+            assert all(s is blk.status for _, s in fake.calls)
+        blk.check()
+        blk.status.fill_(3)                      # as a kernel leaves it
+        with pytest.raises(RuntimeError, match="FORGE_ERR_TIMEOUT"):
+            blk.check()
+        blk.check()                              # reported once
+        blk.status.fill_(2)
+        with pytest.raises(RuntimeError, match="status 2"):
+            blk.check()
+
+
+def test_the_status_word_moves_with_the_block():
+    import copy
+    blk = block(quantised(), norm_weight=torch.ones(H))
+    assert "status" not in blk.state_dict() and blk.status.dtype == torch.int32
+    word = blk.status
+    blk.half().to(torch.bfloat16).double()
+    assert blk.status is word
+    other = copy.deepcopy(blk)
+    other.status.fill_(3)
+    blk.check()
+    meta = copy.deepcopy(blk).to("meta")
+    assert meta.status.device.type == "meta"
+    assert int(meta.to_empty(device="cpu").status) == 0
