@@ -68,10 +68,28 @@ template <typename T> __device__ __forceinline__ void store8(T *p, const float (
 // rounding), against the 2^-9 or 2^-12 of the 16-bit result; 0 where the exact value is below 2^-126.
 __device__ __forceinline__ float sigmoid_fast(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
 
+// Phi(z), given e = exp(-z^2 / 2):  Phi(-x) = e t p(t) for x >= 0, t = 1 / (1 + 0.3 x), p the polynomial of degree 7 whose
+// largest relative error over x in [0, 14] is least (weighted least squares, fitted for this file: 2^-22.7; 2^-21.1 when it is
+// evaluated in fp32, 2^-16.5 with the exponential's own error at x = 8).  1 + erf(z / sqrt 2) loses its bits where z is
+// negative, all of them at -5.5.  2048 x 2048 values of dz take 10.0 us (15.0 with erfcf, 11.4 with erff).
+__device__ __forceinline__ float normal_cdf(float z, float e) {
+    const float t = __fdividef(1.0f, fmaf(0.3f, fabsf(z), 1.0f));
+    float p = 0.03567478805780411f;
+    p = fmaf(p, t, -0.1572030484676361f);
+    p = fmaf(p, t, 0.2063533067703247f);
+    p = fmaf(p, t, -0.05368337780237198f);
+    p = fmaf(p, t, 0.12856145203113556f);
+    p = fmaf(p, t, 0.09991355985403061f);
+    p = fmaf(p, t, 0.1207539513707161f);
+    p = fmaf(p, t, 0.11962930113077164f);
+    const float q = e * (t * p);
+    return z < 0.0f ? q : 1.0f - q;
+}
+
 template <int ACT> __device__ __forceinline__ float act_fwd(float z) {
     if constexpr (ACT == FORGE_ACT_RELU) return z < 0.0f ? 0.0f : z;      // NaN passes through
     if constexpr (ACT == FORGE_ACT_SILU) return z * sigmoid_fast(z);
-    if constexpr (ACT == FORGE_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    if constexpr (ACT == FORGE_ACT_GELU) return z * normal_cdf(z, __expf(-0.5f * z * z));
     return z;
 }
 template <int ACT> __device__ __forceinline__ float act_bwd(float z) {
@@ -80,8 +98,10 @@ template <int ACT> __device__ __forceinline__ float act_bwd(float z) {
         const float s = sigmoid_fast(z);
         return s * (1.0f + z * (1.0f - s));
     }
-    if constexpr (ACT == FORGE_ACT_GELU)
-        return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+    if constexpr (ACT == FORGE_ACT_GELU) {
+        const float e = __expf(-0.5f * z * z);
+        return normal_cdf(z, e) + z * e * 0.39894228040143268f;
+    }
     return 1.0f;
 }
 __device__ __forceinline__ float act_fwd_rt(int act, float z) {
