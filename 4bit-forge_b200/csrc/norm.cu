@@ -384,14 +384,14 @@ RowShape row_shape(int64_t C) {
 }
 
 template <typename T, bool WARP, int NV> int launch_rows(const NormParams &P, int threads, cudaStream_t st) {
+    constexpr int kRing = 128 * 1024;                      // largest ring of a CTA
     const int smem = kDeep * (P.res ? 2 : 1) * NV * (int)sizeof(T) / 2 * threads * 16;
     const auto kernel = rmsnorm_kernel<T, WARP, NV>;
-    if (smem > 40 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) {
-            set_error("forge_rmsnorm: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-            return FORGE_ERR_LAUNCH;
-        }
+    // one limit for every launch of the kernel: another thread's call may set it between this one's two steps
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing);
+    if (e != cudaSuccess || smem > kRing) {
+        set_error("forge_rmsnorm: %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
+        return FORGE_ERR_LAUNCH;
     }
     const int64_t per_sm = 1024 / threads;                 // CTAs on an SM: 1024 threads, 128 KB of ring at most
     const int64_t rows = WARP ? cdiv(P.T, (int64_t)8) : P.T;
