@@ -5,9 +5,9 @@
 //   n = r * rstd,  t = dy * weight,  dx = rstd * (t - n * mean(t n)) + dresidual,  dweight = sum over rows of dy * n
 //
 // Bound by HBM: a row is read once, kept in registers across the reduction, and written once.  One row belongs to a warp
-// (up to 512 channels) or to a CTA, eight channels a thread.
-// Rows that are longer, not a multiple of 8 channels, or not 16-byte aligned take the strided kernels below, which
-// read a row twice (the second time from cache).
+// (up to 512 channels) or to a CTA, eight or sixteen channels a thread.
+// Rows of more than 16384 channels, not of a multiple of 8 of them, or not 16-byte aligned take the strided kernels below,
+// which read a row twice (the second time from cache); so do some rows of fp32 (launch_fwd).
 // Backward: 5003 x 2048 with dresidual (82 MB) 17 us, and 4 us for the column sums.
 // dweight: every CTA walks rows and keeps its columns' sums in registers; one fp32 partial row per CTA, summed in a
 // fixed order by a second launch, so results do not depend on scheduling.
@@ -73,15 +73,21 @@ template <typename T> __device__ __forceinline__ float load_w(const void *w, int
     return w_f32 ? ((const float *)w)[c] : Elem<T>::to_f(((const T *)w)[c]);
 }
 
-// CTAs of as many warps as a row's vectors fill walk the rows (WARP: a warp a row, eight a CTA) with the next kDeep rows on
+// CTAs of as many warps as a row's vectors fill walk the rows (WARP: a warp a row, eight a CTA) with the next four rows on
 // their way into shared memory.  A row is a chain of load, reduction and store of about a microsecond, so what keeps HBM
 // busy is the bytes in flight beside it: 8192 x 7168 with residual to e4m3 (413 MB) took 87 us with one row a CTA and
-// two CTAs an SM, and takes 78 us this way (5.3 TB/s, 0.81 of the measured copy rate).  A thread copies (cp.async) and reads its own vectors only, so the ring needs no barrier.
-constexpr int kDeep = 4;
+// two CTAs an SM, and takes 77 us this way (5.4 TB/s, 0.82 of the measured copy rate).  A thread copies (cp.async) and reads
+// its own vectors only, so the ring needs no barrier.
+// A thread takes two vectors of rows that are longer than a CTA of 1024 threads of one (512 in fp32); those rows are large
+// enough to keep HBM busy with three under way, and 128 KB of fp32 with one.
+constexpr int ring_depth(int es, bool warp, int nv, int threads) { return warp || nv == 1 ? 4 : es * threads <= 2048 ? 3 : 1; }
+constexpr int ring_bytes(int es, int nv, int threads, int deep, int arrays) { return deep * arrays * nv * es / 2 * threads * 16; }
 
-template <typename T, bool WARP, int NV>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) rmsnorm_kernel(const NormParams P) {
+// TMAX: most threads of a CTA
+template <typename T, bool WARP, int NV, int TMAX>
+__global__ void __launch_bounds__(TMAX) rmsnorm_kernel(const NormParams P) {
     constexpr int kQ = sizeof(T) / 2;                     // 16-byte pieces of a vector
+    constexpr int kDeep = ring_depth(sizeof(T), WARP, NV, TMAX);
     extern __shared__ uint4 ring[];                       // [kDeep][x, residual][NV][kQ][threads]
     __shared__ float slot[2][32];
     const int TPR = WARP ? 32 : (int)blockDim.x, t = WARP ? threadIdx.x % 32 : threadIdx.x, C = (int)P.C;
@@ -383,27 +389,36 @@ RowShape row_shape(int64_t C) {
     return {0, 0};
 }
 
-template <typename T, bool WARP, int NV> int launch_rows(const NormParams &P, int threads, cudaStream_t st) {
-    constexpr int kRing = 128 * 1024;                      // largest ring of a CTA
-    const int smem = kDeep * (P.res ? 2 : 1) * NV * (int)sizeof(T) / 2 * threads * 16;
-    const auto kernel = rmsnorm_kernel<T, WARP, NV>;
+template <typename T, bool WARP, int NV, int TMAX> int launch_rows(const NormParams &P, int threads, cudaStream_t st) {
+    constexpr int kDeep = ring_depth(sizeof(T), WARP, NV, TMAX), kMost = ring_bytes(sizeof(T), NV, TMAX, kDeep, 2);
+    static_assert(kMost <= 192 * 1024, "the ring fits an SM");
+    const int smem = ring_bytes(sizeof(T), NV, threads, kDeep, P.res ? 2 : 1);
+    const auto kernel = rmsnorm_kernel<T, WARP, NV, TMAX>;
     // one limit for every launch of the kernel: another thread's call may set it between this one's two steps
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing);
-    if (e != cudaSuccess || smem > kRing) {
-        set_error("forge_rmsnorm: %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    if (e != cudaSuccess) {
+        set_error("forge_rmsnorm: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
         return FORGE_ERR_LAUNCH;
     }
-    const int64_t per_sm = 1024 / threads;                 // CTAs on an SM: 1024 threads, 128 KB of ring at most
+    const int64_t per_sm = 1024 / threads;                 // CTAs on an SM: 1024 threads, 192 KB of ring at most
     const int64_t rows = WARP ? cdiv(P.T, (int64_t)8) : P.T;
     kernel<<<(unsigned)imin64(rows, 148 * per_sm), threads, smem, st>>>(P);
     return FORGE_OK;
 }
 template <typename T> int launch_fwd(const NormParams &P, bool vec, cudaStream_t st) {
-    const int vecs = (int)(P.C / 8);
-    const auto warps = [](int v) { return (v + 31) / 32 * 32; };
-    if (vec && P.C <= 256) return launch_rows<T, true, 1>(P, 256, st);
-    if (vec && P.C <= 512) return launch_rows<T, true, 2>(P, 256, st);
-    if (vec && P.C <= (sizeof(T) == 2 ? 8192 : 4096)) return launch_rows<T, false, 1>(P, warps(vecs), st);
+    constexpr int kRow = sizeof(T) == 2 ? 1024 : 512;      // threads of a row of one vector each
+    const int64_t vecs = P.C / 8;
+    const auto warps = [](int64_t v) { return (int)((v + 31) / 32 * 32); };
+    if (vec && P.C <= 256) return launch_rows<T, true, 1, 256>(P, 256, st);
+    if (vec && P.C <= 512) return launch_rows<T, true, 2, 256>(P, 256, st);
+    if (vec && vecs <= kRow) return launch_rows<T, false, 1, kRow>(P, warps(vecs), st);
+    // Two vectors a thread.  4096 rows of 16-bit elements, ring against rows read twice: 8200 channels 37 against 48 us, with
+    // residual 53 against 138; 16384 channels 53 against 97, 99 against 321.  fp32: with residual 7168 channels 115 against
+    // 144 us, 16384 channels 272 against 411, but 4608 channels 95 against 89; without one 8192 channels 73 against 63.
+    if (vec && (sizeof(T) == 2 || (P.res && P.C >= 5120))) {
+        if (vecs <= 2 * kRow) return launch_rows<T, false, 2, kRow>(P, warps((vecs + 1) / 2), st);
+        if (vecs <= 2 * 1024) return launch_rows<T, false, 2, 1024>(P, warps((vecs + 1) / 2), st);
+    }
     rmsnorm_strided_kernel<T><<<(unsigned)P.T, 256, 0, st>>>(P);
     return FORGE_OK;
 }

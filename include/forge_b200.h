@@ -337,7 +337,8 @@ int forge_sparse14_moe_w2(const uint64_t *w2, const void *X2_bf16, int64_t ldx, 
  *   scales[t, g] = max(max |y|, 1e-12) / 448,   y8 = e4m3(y / scales[t, g]):
  * scales [T, ceil(C/128)] fp32, the layout that forge_fp8_block_dequant reads when C is a multiple of 128.  Row strides ldx, ldres in elements;
  * y, scales and residual_out are dense and alias no input.  Any C, stride and alignment (16-byte aligned rows of a
- * multiple of 8 channels up to 8192, 4096 in fp32, are read once, others twice). */
+ * multiple of 8 channels up to 16384 are read once, others twice; fp32 rows of more than 4096 channels are read once only
+ * with a residual and from 5120 on). */
 int forge_rmsnorm(const void *x, int64_t ldx, const void *residual, int64_t ldres, const void *weight, int w_dtype,
                   int dtype, int64_t T, int64_t C, float eps, void *y, float *scales, void *residual_out, void *stream);
 /* Gradients at the normed rows x (the residual_out of the forward call where there was a residual):

@@ -58,3 +58,38 @@ def test_threads_whose_rows_need_different_shared_memory():
     for x, w, r, y, _, h in cases:
         got = ops().rmsnorm(x, w, EPS, residual=r)
         assert torch.equal(got if r is None else got[0], y) and (r is None or torch.equal(got[1], h))
+
+
+@pytest.mark.parametrize("T,C", [(3, 8200), (400, 8200), (301, 12288), (2, 16376), (333, 16384), (310, 4104), (299, 8192)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("residual", [False, True])
+def test_long_rows(T, C, dt, residual):
+    """Two vectors of a row per thread, several rows per CTA, against float64; the 8-bit form against the formula at its own
+    scales; a row of NaN and a row of zeros spoil nothing beside them."""
+    g = gen(T + C)
+    x, w = torch.randn(T, C, generator=g, device=DEV).to(dt), torch.randn(C, generator=g, device=DEV).to(dt)
+    res = torch.randn(T, C, generator=g, device=DEV).to(dt) if residual else None
+    x[T // 2, 3] = float("nan")
+    x[0] = 0
+    if residual:
+        res[0] = 0
+    h = x.double() + (res.double() if residual else 0)
+    want = h / torch.sqrt(h.square().mean(1, keepdim=True) + EPS) * w.double()
+    good = torch.arange(T, device=DEV) != T // 2
+    got = ops().rmsnorm(x, w, EPS, residual=res)
+    y, r = got if residual else (got, None)
+    # with a residual h is an fp32 sum: 2^-24 of it more
+    tol = (HALF[dt] + STAT + 2.0 ** -23) * want.abs() + 1e-7 * (dt == torch.float16)
+    assert bool(((y.double() - want).abs() <= tol)[good].all()) and bool(y[T // 2].isnan().all())
+    assert not bool(y[0].any())
+    if residual:
+        assert bool(((r.double() - h).abs() <= (HALF[dt] + 2.0 ** -23) * h.abs() + 1e-7 * (dt == torch.float16))[good].all())
+    if dt == torch.float32:
+        return
+    q, s, *rest = ops().rmsnorm(x, w, EPS, residual=res, quant_group=128)
+    assert not residual or torch.equal(rest[0][good], r[good])
+    step = s.double().repeat_interleave(128, 1)[:, :C]
+    groups = torch.nn.functional.pad(want, (0, -C % 128)).view(T, -1, 128).abs().amax(2).clamp_min(1e-12) / 448
+    assert bool(((s.double() - groups).abs() <= 2.0 ** -18 * groups)[good].all())
+    # half a step of e4m3 (2^-4 relative, 2^-10 of the scale among its subnormals) and the fp32 roundings before it
+    assert bool(((q.double() * step - want).abs() <= (2.0 ** -4 + 2.0 ** -17) * want.abs() + 2.0 ** -10 * step)[good].all())
