@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(TMAX) rmsnorm_kernel(const NormParams P) {
             // 16 neighbouring threads hold a group of 128 channels
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-            const float sc = amax / kF8Max, inv = 1.0f / sc;
+            const float sc = amax / kF8Max, inv = 1.0f / sc;       // (a division a value: 100 us in place of 77)
             if (c < C) {
                 uint2 out;
                 out.x = e4m3x4(h[i][0] * inv, h[i][1] * inv, h[i][2] * inv, h[i][3] * inv);

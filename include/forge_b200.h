@@ -334,9 +334,10 @@ int forge_sparse14_moe_w2(const uint64_t *w2, const void *X2_bf16, int64_t ldx, 
  *   h = x (+ residual);   y = h / sqrt(mean(h^2) + eps) * weight;   residual_out = h   (with residual only)
  * x, residual, residual_out and y have the type `dtype` (fp32, bf16, fp16); weight [C] that type or fp32.  With scales
  * given, y is e4m3 bytes and, per 128 consecutive channels of a row (the last group may be shorter),
- *   scales[t, g] = max(max |y|, 1e-12) / 448,   y8 = e4m3(y / scales[t, g]):
- * scales [T, ceil(C/128)] fp32, the layout that forge_fp8_block_dequant reads when C is a multiple of 128.  Row strides ldx, ldres in elements;
- * y, scales and residual_out are dense and alias no input.  Any C, stride and alignment (16-byte aligned rows of a
+ *   scales[t, g] = max(max |y|, 1e-12) / 448,   y8 = e4m3(y / scales[t, g])
+ * (a product with the rounded reciprocal, within 3 2^-24 of the quotient before it is rounded to e4m3):
+ * scales [T, ceil(C/128)] fp32, the layout that forge_fp8_block_dequant reads when C is a multiple of 128.  Row strides
+ * ldx, ldres in elements; y, scales and residual_out are dense and alias no input.  Any C, stride and alignment (16-byte aligned rows of a
  * multiple of 8 channels up to 16384 are read once, others twice; fp32 rows of more than 4096 channels are read once only
  * with a residual and from 5120 on). */
 int forge_rmsnorm(const void *x, int64_t ldx, const void *residual, int64_t ldres, const void *weight, int w_dtype,

@@ -93,3 +93,24 @@ def test_long_rows(T, C, dt, residual):
     assert bool(((s.double() - groups).abs() <= 2.0 ** -18 * groups)[good].all())
     # half a step of e4m3 (2^-4 relative, 2^-10 of the scale among its subnormals) and the fp32 roundings before it
     assert bool(((q.double() * step - want).abs() <= (2.0 ** -4 + 2.0 ** -17) * want.abs() + 2.0 ** -10 * step)[good].all())
+
+
+@pytest.mark.parametrize("T,C", [(300, 64), (300, 384), (200, 1000), (40, 4096), (40, 4100), (20, 9000), (20, 9001)])
+def test_eight_bits_are_the_rounded_quotient(T, C):
+    """scale = max |y| / 448 bit for bit, and q = e4m3(y / scale) from the y that the same rows give in fp32.  The kernel
+    multiplies by the scale's rounded reciprocal: the product is within 3 2^-24 of the quotient, so rounding keeps it between
+    the codes of the quotient times 1 -+ 2^-22.  (The oracle divides in float64, since torch divides an fp32 tensor by a
+    number as a product with the rounded inverse.)"""
+    g = gen(C)
+    x, w = torch.randn(T, C, generator=g, device=DEV), torch.randn(C, generator=g, device=DEV)
+    y = ops().rmsnorm(x, w, EPS)
+    q, s = ops().rmsnorm(x, w, EPS, quant_group=128)
+    groups = torch.nn.functional.pad(y, (0, -C % 128)).view(T, -1, 128)
+    want_s = (groups.abs().amax(2).clamp_min(1e-12).double() / 448).float()
+    assert torch.equal(s, want_s)
+    quot = groups.double() / want_s.double().unsqueeze(2)
+    code = lambda v: v.float().to(torch.float8_e4m3fn).float().view(T, -1)[:, :C]
+    lo, hi = code(quot * (1 - 2.0 ** -22)), code(quot * (1 + 2.0 ** -22))
+    got = q.float()
+    assert bool(((got >= torch.minimum(lo, hi)) & (got <= torch.maximum(lo, hi))).all())
+    assert float((lo != hi).float().mean()) < 1e-4
