@@ -63,18 +63,21 @@ class Sparse14MoERuntime:
 
 # ---- dense feed-forward block on pack-quantized int4 weights ---------------------------------------------------------
 class _RMSNorm(torch.autograd.Function):
+    """(y, h): h is the stream behind the norm, x + residual, or x itself.  x comes back as an output so that the gradient
+    that reaches it past the norm is added to the norm's own before that is rounded."""
+
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
         y, h = (ops.rmsnorm(x, weight, eps), x) if residual is None else ops.rmsnorm(x, weight, eps, residual=residual)
         ctx.save_for_backward(h, weight)
         ctx.eps, ctx.has_residual = eps, residual is not None
-        return (y, h) if residual is not None else (y, None)
+        return y, h
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dh):
         h, weight = ctx.saved_tensors
-        dx, dw = ops.rmsnorm_backward(dy, h, weight, ctx.eps, dresidual=dh if ctx.has_residual else None)
+        dx, dw = ops.rmsnorm_backward(dy, h, weight, ctx.eps, dresidual=dh)
         return dx, dw, dx if ctx.has_residual else None, None
 
 
@@ -230,7 +233,6 @@ class Int4FeedForward(torch.nn.Module):
                 y, h = x, None
             else:
                 y, h = _RMSNorm.apply(x, w, res, self.eps)
-                h = x if h is None else h
             a = _Int4Gated.apply(y, *gate, act, status)
             out = _Int4Linear.apply(a, None, h, *down, "none", status)
         else:
