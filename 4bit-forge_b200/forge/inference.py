@@ -223,6 +223,8 @@ class Int4FeedForward(torch.nn.Module):
         if residual is not None and self.norm_weight is None:
             raise RuntimeError("a block without a norm takes no residual")
         shape = hidden.shape
+        if residual is not None and residual.shape != shape:
+            raise RuntimeError(f"residual must have hidden's shape {list(shape)}, got {list(residual.shape)}")
         x = hidden.reshape(-1, shape[-1])
         res = None if residual is None else residual.reshape(-1, shape[-1])
         w, gs, act, status = self.norm_weight, self.group_size, self.act, self.status

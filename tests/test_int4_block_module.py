@@ -160,3 +160,15 @@ def test_the_status_word_moves_with_the_block():
     meta = copy.deepcopy(blk).to("meta")
     assert meta.status.device.type == "meta"
     assert int(meta.to_empty(device="cpu").status) == 0
+
+
+def test_a_residual_of_another_shape_is_refused(monkeypatch):
+    """Also one of as many elements, whose rows would meet those of hidden in an order that its shape does not say."""
+    from forge import inference
+    monkeypatch.setattr(inference, "ops", FakeOps())
+    blk = block(quantised(), norm_weight=torch.ones(H))
+    x = torch.zeros(2, 3, H)
+    assert blk(x, residual=torch.zeros(2, 3, H)).shape == x.shape
+    for shape in ((3, 2, H), (6, H), (2, 6, H // 2), (1, 3, H), (H,)):
+        with pytest.raises(RuntimeError, match="shape"):
+            blk(x, residual=torch.zeros(shape))
