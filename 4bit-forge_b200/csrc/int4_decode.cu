@@ -78,9 +78,14 @@ template <int LW> __device__ __forceinline__ void load_words(const uint32_t *row
     }
 }
 
+// CTAs of eight warps on an SM: three where 80 registers hold two blocks of words, scales and tokens, two for gate and up and
+// for groups of 32.  Held to three, those spilled up to 364 bytes a thread: gated, 1 token, 7168 -> 18432 took 64 us at groups
+// of 128 and 149 us at groups of 32, and takes 49 and 80; linear at groups of 32 43 and 40.
+constexpr int ctas_per_sm(bool gated, int gs, int nt, int warps) { return warps == 8 && nt == 1 ? (gated || gs == 32 ? 2 : 3) : 1; }
+
 // GS: group size; NT: blocks of 8 tokens; W: warps
 template <typename T, bool GATED, int GS, int NT, int W>
-__global__ void __launch_bounds__(W * 32, W == 8 && NT == 1 ? 3 : 1) decode_kernel(const Int4Fwd P) {
+__global__ void __launch_bounds__(W * 32, ctas_per_sm(GATED, GS, NT, W)) decode_kernel(const Int4Fwd P) {
     constexpr int M = GATED ? 2 : 1;
     constexpr int LW = GS / 32;            // packed words of a group that one thread takes
     constexpr int NG = 128 / GS;           // groups in a block of 128 channels

@@ -50,9 +50,10 @@ constexpr int kLinear = 0, kGated = 1, kDgrad = 2;
 constexpr int kMT = 128, kKT = 128;             // rows of a CTA tile, channels of a stage
 constexpr int kSubA = kMT * 128, kABytes = 2 * kSubA;   // K-major: two sub-tiles of 64 channels (128 bytes a row)
 constexpr int kThreads = 640;
-// Registers a thread of the summing, loading and other warps, out of 5 x 96: what each form needs so that its inner loops
-// keep everything in registers.  (The 4096 x 2048 -> 7168 product took 130 us with 176 for the sums and 190 with 160; the
-// gated 8192 x 7168 -> 2048 one 371 us with 64 for the loads and 454 with 48.)
+// Registers a thread of the summing, loading and other warps, out of 5 x 96, as measured for each form; ptxas still spills 28
+// to 40 bytes in the linear form of a single CTA and 188 in the paired backward one, nothing in the others.  (The 4096 x 2048
+// -> 7168 product took 130 us with 176 for the sums and 190 with 160; the gated 8192 x 7168 -> 2048 one 371 us with 64 for the
+// loads and 454 with 48.)
 template <int MODE> struct Regs {
     static constexpr int kSum = MODE == kLinear ? 176 : MODE == kGated ? 160 : 152;
     static constexpr int kLoad = MODE == kLinear ? 48 : MODE == kGated ? 64 : 72, kMisc = 32;

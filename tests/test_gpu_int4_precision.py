@@ -103,3 +103,28 @@ def test_scales_of_more_groups_than_fit_at_a_time():
     want = (dy.double() @ ((codes.double() - 8) * s.double().repeat_interleave(gs, 1))).view(T, -1, gs)
     # group by group: 160 entries each, so the ratio of two norms spreads by a tenth more
     assert float(((dx - want).norm(dim=(0, 2)) / want.norm(dim=(0, 2))).max()) <= 1.5 * norm_bound(torch.bfloat16)
+
+
+@pytest.mark.parametrize("T", [1, 8, 13])
+@pytest.mark.parametrize("C,R,gs", [(1024, 200, 32), (776, 3000, 32), (2048, 5001, 64), (4104, 2500, 128), (7168, 2400, 32)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_few_tokens_and_wide_matrices(T, C, R, gs, dt):
+    """The few-token form with eight warps (few channels or many rows), norm-wise: the products are exact but for fp32 sums, so
+    one rounding of the result is all, h / sqrt(3) of it and a tenth; the gated result passes act and a product in fp32."""
+    g = torch.Generator(device=DEV).manual_seed(T * C + R)
+    mats = []
+    for _ in range(2):
+        codes = torch.randint(0, 16, (R, C), generator=g, device=DEV)
+        s = (torch.rand(R, -(-C // gs), generator=g, device=DEV) + 0.5) / (5 * math.sqrt(C))
+        mats.append((words(codes), s, (codes.double() - 8) * s.double().repeat_interleave(gs, 1)[:, :C]))
+    (p0, s0, W0), (p1, s1, W1) = mats
+    x = torch.randn(T, C, generator=g, device=DEV).to(dt)
+    X = x.double()
+    bound = 1.1 * HALF[dt] / math.sqrt(3) + 2.0 ** -18
+    y, want = ops().int4_linear(x, p0, s0, gs).double(), X @ W0.T
+    assert float((y - want).norm() / want.norm()) <= bound
+    h, u, v = ops().int4_gated(x, p0, s0, p1, s1, gs, want_preact=True)
+    a = X @ W0.T
+    want = a * torch.sigmoid(a) * (X @ W1.T)
+    assert float((h.double() - want).norm() / want.norm()) <= bound
+    assert torch.equal(u, ops().int4_linear(x, p0, s0, gs)) and float((v.double() - X @ W1.T).norm() / (X @ W1.T).norm()) <= bound
