@@ -6,8 +6,8 @@
 //
 // Bound by HBM: a row is read once, kept in registers across the reduction, and written once.  One row belongs to a warp
 // (up to 512 channels) or to a CTA, eight or sixteen channels a thread.
-// Rows of more than 16384 channels, not of a multiple of 8 of them, or not 16-byte aligned take the strided kernels below,
-// which read a row twice (the second time from cache); so do some rows of fp32 (launch_fwd).
+// Rows of more than 16384 channels, not of a multiple of 8 of them, or not 16-byte aligned take the strided
+// kernels below, which read a row twice (the second time from cache); so do some rows of fp32 (launch_fwd).
 // Backward: 5003 x 2048 with dresidual (82 MB) 17 us, and 4 us for the column sums.
 // dweight: every CTA walks rows and keeps its columns' sums in registers; one fp32 partial row per CTA, summed in a
 // fixed order by a second launch, so results do not depend on scheduling.
@@ -237,9 +237,12 @@ template <typename T> __global__ void __launch_bounds__(256) rmsnorm_strided_ker
 }
 
 // Backward: every CTA (or warp, TPR = 32) walks rows; column sums of dy * n stay in registers.
-constexpr int bwd_per_sm(int tpr) { return tpr == 128 ? 6 : tpr <= 256 ? 3 : 1; }
+// CTAs on an SM, as many as the registers hold (16-bit rows of 257 to 512 channels, two vectors a lane: 64000 x 512 take 48 us
+// with two and took 106 with three, which spilled 370 bytes a thread)
+constexpr int bwd_per_sm(int tpr, int nv) { return tpr == 128 ? 6 : tpr == 32 && nv == 2 ? 2 : tpr <= 256 ? 3 : 1; }
 template <typename T, int TPR, int NV>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, sizeof(T) == 2 ? bwd_per_sm(TPR) : 1) rmsnorm_bwd_kernel(const NormBwdParams P) {
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, sizeof(T) == 2 ? bwd_per_sm(TPR, NV) : 1)
+rmsnorm_bwd_kernel(const NormBwdParams P) {
     constexpr int kRows = TPR == 32 ? 8 : 1;
     __shared__ float slot[2][2][32];
     const int t = threadIdx.x % TPR;
@@ -373,7 +376,7 @@ __global__ void __launch_bounds__(1024) column_sum_kernel(const float *__restric
 
 constexpr int64_t kMaxRows = 0x7fffffffLL;       // one CTA per row at most
 // CTAs that walk the rows in the backward pass: as many as the SMs hold
-int bwd_cap(int tpr) { return 148 * bwd_per_sm(tpr); }
+int bwd_cap(int tpr, int nv) { return 148 * bwd_per_sm(tpr, nv); }
 
 bool vec_ok(const void *p, int64_t ld, size_t es) { return ((uintptr_t)p % 16 == 0) && (ld * (int64_t)es) % 16 == 0; }
 // The row-in-registers backward kernels: (threads per row, vectors per thread) by length; 0 = strided form.
@@ -425,7 +428,7 @@ template <typename T> int launch_fwd(const NormParams &P, bool vec, cudaStream_t
 
 int bwd_ctas(int64_t T, RowShape s) {
     const int64_t rows = s.tpr == 32 ? 8 : 1;
-    return (int)imin64(cdiv(T, rows), bwd_cap(s.tpr));
+    return (int)imin64(cdiv(T, rows), bwd_cap(s.tpr, s.nv));
 }
 int strided_partials(int64_t T) { return (int)imin64(cdiv(T, (int64_t)16), 64); }
 

@@ -114,3 +114,25 @@ def test_eight_bits_are_the_rounded_quotient(T, C):
     got = q.float()
     assert bool(((got >= torch.minimum(lo, hi)) & (got <= torch.maximum(lo, hi))).all())
     assert float((lo != hi).float().mean()) < 1e-4
+
+
+@pytest.mark.parametrize("T,C", [(6000, 264), (3001, 384), (5000, 512), (900, 8192), (700, 8200), (65, 16384)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+def test_backward_of_many_rows(T, C, dt):
+    """More rows than warps or CTAs walk at once, norm-wise against float64: one rounding of dx and of dweight (h / sqrt(3) of
+    the norm and a tenth), fp32 sums over a row (2^-18) and over T rows (2^-24 each at most, of magnitudes that are
+    sqrt(T) times the sum's)."""
+    g = gen(T)
+    x, dy, dres = (torch.randn(T, C, generator=g, device=DEV).to(dt) for _ in range(3))
+    w = (1 + 0.3 * torch.randn(C, generator=g, device=DEV)).to(dt)
+    X, t = x.double(), dy.double() * w.double()
+    rstd = 1 / torch.sqrt(X.square().mean(1, keepdim=True) + EPS)
+    n = X * rstd
+    dx64 = rstd * (t - n * (t * n).mean(1, keepdim=True))
+    dw64 = (dy.double() * n).sum(0)
+    one = 1.1 * HALF[dt] / 3 ** 0.5
+    off = lambda a, b: float((a.double() - b).norm() / b.norm())
+    dx, dw = ops().rmsnorm_backward(dy, x, w, EPS)
+    assert off(dx, dx64) <= one + 2.0 ** -18 and off(dw, dw64) <= one + T ** 0.5 * 2.0 ** -21
+    dx, dw2 = ops().rmsnorm_backward(dy, x, w, EPS, dresidual=dres)
+    assert off(dx, dx64 + dres.double()) <= one + 2.0 ** -18 and torch.equal(dw, dw2)
