@@ -6,7 +6,7 @@
 //
 // Bound by HBM: a row is read once, kept in registers across the reduction, and written once.  One row belongs to a warp
 // (up to 512 channels) or to a CTA, eight or sixteen channels a thread.
-// Rows of more than 16384 channels, not of a multiple of 8 of them, or not 16-byte aligned take the strided
+// Rows of more than 16384 channels (backward: 8192), not of a multiple of 8 of them, or not 16-byte aligned take the strided
 // kernels below, which read a row twice (the second time from cache); so do some rows of fp32 (launch_fwd).
 // Backward: 5003 x 2048 with dresidual (82 MB) 17 us, and 4 us for the column sums.
 // dweight: every CTA walks rows and keeps its columns' sums in registers; one fp32 partial row per CTA, summed in a
@@ -379,7 +379,9 @@ constexpr int64_t kMaxRows = 0x7fffffffLL;       // one CTA per row at most
 int bwd_cap(int tpr, int nv) { return 148 * bwd_per_sm(tpr, nv); }
 
 bool vec_ok(const void *p, int64_t ld, size_t es) { return ((uintptr_t)p % 16 == 0) && (ld * (int64_t)es) % 16 == 0; }
-// The row-in-registers backward kernels: (threads per row, vectors per thread) by length; 0 = strided form.
+// The row-in-registers backward kernels: (threads per row, vectors per thread) by length; 0 = strided form.  1024 threads of two
+// vectors have no room for a longer row: 2048 x 8200 took 127 us so (fp32 189) and takes 58 (89) in the strided form, 16384
+// channels 155 against 137 (268 against 200); 8192 channels take 27 us in registers and 57 strided.
 struct RowShape { int tpr, nv; };
 RowShape row_shape(int64_t C) {
     if (C <= 256) return {32, 1};
@@ -388,7 +390,6 @@ RowShape row_shape(int64_t C) {
     if (C <= 2048) return {256, 1};
     if (C <= 4096) return {512, 1};
     if (C <= 8192) return {512, 2};
-    if (C <= 16384) return {1024, 2};
     return {0, 0};
 }
 
@@ -441,7 +442,7 @@ template <typename T> void launch_bwd(NormBwdParams &P, RowShape s, cudaStream_t
         return;                                                                                              \
     }
     FORGE_NORM_CASE(32, 1) FORGE_NORM_CASE(32, 2) FORGE_NORM_CASE(128, 1) FORGE_NORM_CASE(256, 1)
-    FORGE_NORM_CASE(512, 1) FORGE_NORM_CASE(512, 2) FORGE_NORM_CASE(1024, 2)
+    FORGE_NORM_CASE(512, 1) FORGE_NORM_CASE(512, 2)
 #undef FORGE_NORM_CASE
     P.n_partial = strided_partials(P.T);
     rmsnorm_bwd_strided_kernel<T><<<(unsigned)P.T, 256, 0, st>>>(P); FORGE_NOTE_LAUNCH();
