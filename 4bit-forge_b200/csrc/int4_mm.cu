@@ -11,6 +11,7 @@
 // weights' scales are split the same way, see scale_prep_kernel.
 #include <cooperative_groups.h>
 #include <utility>
+#include "column_sum.cuh"
 #include "common.cuh"
 #include "elem.cuh"
 #include "int4_mm.cuh"
@@ -266,24 +267,6 @@ __global__ void __launch_bounds__(256) dbias_kernel(const T *__restrict__ dy, in
     }
     partial[(int64_t)blockIdx.y * R + r] = s;
 }
-// 32 columns x 32 strands of partial rows per CTA, joined in a fixed order
-template <typename T>
-__global__ void __launch_bounds__(1024) dbias_sum_kernel(const float *__restrict__ partial, int n, int64_t R, T *out) {
-    __shared__ float sh[32][33];
-    const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
-    const int64_t r = (int64_t)blockIdx.x * 32 + lane;
-    float s = 0.0f;
-    if (r < R)
-        for (int j = k; j < n; j += 32) s += partial[(int64_t)j * R + r];
-    sh[k][lane] = s;
-    __syncthreads();
-    s = sh[lane][k];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const int64_t ro = (int64_t)blockIdx.x * 32 + k;
-    if (lane == 0 && ro < R) out[ro] = Elem<T>::from_f(s);
-}
-
 // ---- host side -------------------------------------------------------------------------------------------------------
 constexpr int64_t kMaxDim = 1ll << 24;        // rows and columns of a weight matrix
 constexpr int64_t kMaxTokens = 0x7fffffffLL;
@@ -322,20 +305,20 @@ BwdLayout bwd_layout(int64_t T, int64_t C, int64_t R, int gs, int mats) {
     return L;
 }
 
-template <typename T> void launch_dbias(const void *dy, int64_t lddy, const void *z, int act, int64_t n, int64_t R,
-                                        float *partial, void *out, cudaStream_t st) {
-    const int parts = (int)(n < kBiasParts ? (n > 0 ? n : 0) : kBiasParts);
-    if (parts > 0) {
-        const dim3 grid((unsigned)cdiv(R, (int64_t)256), parts);
-        switch (act) {
-            case FORGE_ACT_RELU: dbias_kernel<T, FORGE_ACT_RELU><<<grid, 256, 0, st>>>((const T *)dy, lddy, (const T *)z, n, R, partial); break;
-            case FORGE_ACT_SILU: dbias_kernel<T, FORGE_ACT_SILU><<<grid, 256, 0, st>>>((const T *)dy, lddy, (const T *)z, n, R, partial); break;
-            case FORGE_ACT_GELU: dbias_kernel<T, FORGE_ACT_GELU><<<grid, 256, 0, st>>>((const T *)dy, lddy, (const T *)z, n, R, partial); break;
-            default: dbias_kernel<T, FORGE_ACT_NONE><<<grid, 256, 0, st>>>((const T *)dy, lddy, (const T *)z, n, R, partial);
-        }
-        FORGE_NOTE_LAUNCH();
+// Partial column sums of dz where the pass that writes dz did not leave them; returns their number of rows
+template <typename T> int launch_dbias(const void *dy, int64_t lddy, const void *z, int act, int64_t n, int64_t R, float *partial,
+                                       cudaStream_t st) {
+    const int parts = (int)imin64(n, kBiasParts);
+    if (parts == 0) return 0;
+    const dim3 grid((unsigned)cdiv(R, (int64_t)256), parts);
+    switch (act) {
+        case FORGE_ACT_RELU: dbias_kernel<T, FORGE_ACT_RELU><<<grid, 256, 0, st>>>((const T *)dy, lddy, (const T *)z, n, R, partial); break;
+        case FORGE_ACT_SILU: dbias_kernel<T, FORGE_ACT_SILU><<<grid, 256, 0, st>>>((const T *)dy, lddy, (const T *)z, n, R, partial); break;
+        case FORGE_ACT_GELU: dbias_kernel<T, FORGE_ACT_GELU><<<grid, 256, 0, st>>>((const T *)dy, lddy, (const T *)z, n, R, partial); break;
+        default: dbias_kernel<T, FORGE_ACT_NONE><<<grid, 256, 0, st>>>((const T *)dy, lddy, (const T *)z, n, R, partial);
     }
-    dbias_sum_kernel<T><<<(unsigned)cdiv(R, (int64_t)32), 1024, 0, st>>>(partial, parts, R, (T *)out); FORGE_NOTE_LAUNCH();
+    FORGE_NOTE_LAUNCH();
+    return parts;
 }
 // The row-in-registers form of dz where it fits; the number of partial rows written, or 0 when the call is not for it.
 template <typename T, int ACT, bool GATED> int launch_dz_rows(const DzParams &P, float *partial, cudaStream_t st) {
@@ -365,11 +348,6 @@ template <typename T, bool GATED> int launch_dz(const DzParams &P, int act, floa
         default: return launch_dz_act<T, GATED, FORGE_ACT_NONE>(P, partial, st);
     }
 }
-template <typename T> void sum_dbias(const float *partial, int parts, int64_t R, void *out, cudaStream_t st) {
-    dbias_sum_kernel<T><<<(unsigned)cdiv(R, (int64_t)32), 1024, 0, st>>>(partial, parts, R, (T *)out);
-    FORGE_NOTE_LAUNCH();
-}
-
 int run_fwd(Int4Fwd &P, int dtype, bool gated, cudaStream_t st) {
     const uintptr_t a = (uintptr_t)P.packed[0] | (uintptr_t)P.packed[1];
     P.vec8 = P.C % 16 == 0 && a % 8 == 0;
@@ -434,14 +412,10 @@ static int backward(const char *who, const void *dy, int64_t lddy, int dtype, co
         else parts = bf16 ? launch_dz<__nv_bfloat16, false>(D, act, pp, st) : launch_dz<__half, false>(D, act, pp, st);
     }
     if (dbias) {
-        if (parts > 0) {
-            if (bf16) sum_dbias<__nv_bfloat16>(partial, parts, R, dbias, st);
-            else sum_dbias<__half>(partial, parts, R, dbias, st);
-        } else if (bf16) {
-            launch_dbias<__nv_bfloat16>(dy, lddy, z, act, T, R, partial, dbias, st);
-        } else {
-            launch_dbias<__half>(dy, lddy, z, act, T, R, partial, dbias, st);
-        }
+        if (parts == 0)
+            parts = bf16 ? launch_dbias<__nv_bfloat16>(dy, lddy, z, act, T, R, partial, st)
+                         : launch_dbias<__half>(dy, lddy, z, act, T, R, partial, st);
+        launch_column_sum(partial, parts, R, dbias, dtype, st);
     }
     if (!dx || T == 0) return check_launch(who);
     Int4Dgrad P{(const __half *)(base + L.a), L.ldk, (const float *)(base + L.unscale),

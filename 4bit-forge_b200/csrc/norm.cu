@@ -12,6 +12,7 @@
 // dweight: every CTA walks rows and keeps its columns' sums in registers; one fp32 partial row per CTA, summed in a
 // fixed order by a second launch, so results do not depend on scheduling.
 #include "common.cuh"
+#include "column_sum.cuh"
 #include "elem.cuh"
 #include "tcgen05.cuh"
 
@@ -355,25 +356,6 @@ template <typename T> __global__ void __launch_bounds__(256) rmsnorm_dw_strided_
     P.partial[(int64_t)blockIdx.y * P.C + c] = s;
 }
 
-// out[c] = sum over n rows of partial[n, C], in a fixed order: 32 columns x 32 row strands per CTA
-template <typename T>
-__global__ void __launch_bounds__(1024) column_sum_kernel(const float *__restrict__ partial, int n, int64_t C, T *out) {
-    __shared__ float s[32][33];
-    const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
-    const int k = threadIdx.x >> 5;
-    float v = 0.0f;
-    if (c < C)
-#pragma unroll 4
-        for (int r = k; r < n; r += 32) v += partial[(int64_t)r * C + c];
-    s[k][threadIdx.x & 31] = v;
-    __syncthreads();
-    v = s[threadIdx.x & 31][k];              // column k of the block, strand = lane
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    const int64_t co = (int64_t)blockIdx.x * 32 + k;
-    if ((threadIdx.x & 31) == 0 && co < C) out[co] = Elem<T>::from_f(v);
-}
-
 constexpr int64_t kMaxRows = 0x7fffffffLL;       // one CTA per row at most
 // CTAs that walk the rows in the backward pass: as many as the SMs hold
 int bwd_cap(int tpr, int nv) { return 148 * bwd_per_sm(tpr, nv); }
@@ -509,11 +491,6 @@ extern "C" int forge_rmsnorm_backward(const void *dy, int64_t lddy, const void *
         else if (dtype == FORGE_DTYPE_BF16) launch_bwd<__nv_bfloat16>(P, s, st);
         else launch_bwd<__half>(P, s, st);
     }
-    const unsigned blocks = (unsigned)cdiv(C, (int64_t)32);
-    if (w_dtype == FORGE_DTYPE_F32) column_sum_kernel<float><<<blocks, 1024, 0, st>>>(P.partial, P.n_partial, C, (float *)dweight);
-    else if (w_dtype == FORGE_DTYPE_BF16)
-        column_sum_kernel<__nv_bfloat16><<<blocks, 1024, 0, st>>>(P.partial, P.n_partial, C, (__nv_bfloat16 *)dweight);
-    else column_sum_kernel<__half><<<blocks, 1024, 0, st>>>(P.partial, P.n_partial, C, (__half *)dweight);
-    FORGE_NOTE_LAUNCH();
+    launch_column_sum(P.partial, P.n_partial, C, dweight, w_dtype, st);
     return check_launch("forge_rmsnorm_backward");
 }
