@@ -128,3 +128,61 @@ def test_few_tokens_and_wide_matrices(T, C, R, gs, dt):
     want = a * torch.sigmoid(a) * (X @ W1.T)
     assert float((h.double() - want).norm() / want.norm()) <= bound
     assert torch.equal(u, ops().int4_linear(x, p0, s0, gs)) and float((v.double() - X @ W1.T).norm() / (X @ W1.T).norm()) <= bound
+
+
+def matrix(R, C, gs, g):
+    codes = torch.randint(0, 16, (R, C), generator=g, device=DEV)
+    s = torch.exp(torch.randn(R, -(-C // gs), generator=g, device=DEV)) / (5 * math.sqrt(C))
+    return words(codes), s, (codes.double() - 8) * s.double().repeat_interleave(gs, 1)[:, :C]
+
+
+def off(got, want):
+    return float((got.double() - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("T,C,R,gs", [(24, 2048, 776, 128), (64, 776, 1001, 32), (130, 1032, 520, 64), (333, 776, 1001, 32),
+                                      (1500, 2048, 2000, 128), (2100, 1000, 1800, 64)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_every_form_norm_wise(T, C, R, gs, dt):
+    """Forward: one rounding of the result, the fp32 sums 2^-18 of its norm at most (256 truncating additions of terms whose
+    signs are independent).  Backward: the bound above, with dz from the stored values."""
+    g = torch.Generator(device=DEV).manual_seed(T + C)
+    (p0, s0, W0), (p1, s1, W1) = matrix(R, C, gs, g), matrix(R, C, gs, g)
+    x = torch.randn(T, C, generator=g, device=DEV).to(dt)
+    fwd = 1.1 * HALF[dt] / math.sqrt(3) + 2.0 ** -17
+    z = x.double() @ W0.T
+    y, saved = ops().int4_linear(x, p0, s0, gs, act="gelu", want_preact=True)
+    assert off(y, z * torch.special.ndtr(z)) <= fwd and off(saved, z) <= fwd
+    assert off(ops().int4_linear(x, p0, s0, gs), z) <= fwd
+    h, u, v = ops().int4_gated(x, p0, s0, p1, s1, gs, want_preact=True)
+    assert off(h, z * torch.sigmoid(z) * (x.double() @ W1.T)) <= fwd and off(v, x.double() @ W1.T) <= fwd
+    dy = torch.randn(T, R, generator=g, device=DEV).to(dt)
+    Z = saved.double()
+    dz = dy.double() * (torch.special.ndtr(Z) + Z * torch.exp(-Z * Z / 2) / math.sqrt(2 * math.pi))
+    dx, db = ops().int4_linear_backward(dy, p0, s0, gs, preact=saved, act="gelu", want_dbias=True)
+    assert off(dx, dz @ W0) <= norm_bound(dt) and off(db, dz.sum(0)) <= fwd
+    U, V = u.double(), v.double()
+    sig = torch.sigmoid(U)
+    want = (dy.double() * V * sig * (1 + U * (1 - sig))) @ W0 + (dy.double() * U * sig) @ W1
+    assert off(ops().int4_gated_backward(dy, u, v, p0, s0, p1, s1, gs), want) <= norm_bound(dt)
+
+
+@pytest.mark.parametrize("T", [1, 20, 150, 700])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_block_norm_wise(T, dt):
+    """Roundings of half a step on the way through the block, each h / sqrt(3) norm-wise: the norm's result, which reaches both
+    projections (an elasticity of silu of 1.5 and one of 1: 1.8), the gated product, the stream, the result: 2.5 together."""
+    from forge.inference import Int4FeedForward
+    H, I, gs = 1024, 776, 64
+    g = torch.Generator(device=DEV).manual_seed(T)
+    mats = [matrix(I, H, gs, g), matrix(I, H, gs, g), matrix(H, I, gs, g)]
+    x, res = (torch.randn(T, H, generator=g, device=DEV).to(dt) for _ in range(2))
+    w = (1 + 0.2 * torch.randn(H, generator=g, device=DEV)).to(dt)
+    blk = Int4FeedForward(*[m[:2] for m in mats], group_size=gs, norm_weight=w)
+    h = x.double() + res.double()
+    n = h / torch.sqrt(h.square().mean(1, keepdim=True) + 1e-6) * w.double()
+    a = n @ mats[0][2].T
+    want = (a * torch.sigmoid(a) * (n @ mats[1][2].T)) @ mats[2][2].T + h
+    with torch.no_grad():
+        assert off(blk(x, residual=res), want) <= 1.1 * 2.5 * HALF[dt] / math.sqrt(3)
+    blk.check()
