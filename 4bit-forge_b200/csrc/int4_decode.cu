@@ -12,8 +12,9 @@
 // latency.  A CTA owns 16 rows; its warps share the K axis in blocks of 128 channels and join through shared memory in a
 // fixed order, so there is one launch and no second pass.  One token, 2048 -> 7168: 5.5 us (7.8 MB); one token through
 // gate and up, 7168 -> 2048: 7.5 us (15.7 MB, 2.1 TB/s).  Both are chains of a launch, two to four loads and a join; the
-// next block's loads are under way while a block is multiplied.  24 tokens took 16.9 us here (7168 -> 2048: each CTA reads
-// all of x) against 14.5 us in the tensor-memory kernel, which therefore takes over above 16.
+// next block's loads are under way while a block is multiplied.  Wide matrices, one token, 7168 -> 18432: 27.4 us (2.6 TB/s),
+// gate and up 48.6 us (2.9 TB/s).  Above kDecodeTokens, where every CTA's reading all of x weighs, the tensor-memory kernel is
+// the faster one.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "common.cuh"

@@ -38,7 +38,10 @@ struct Int4Dgrad {
 };
 
 constexpr int kKBlock = 512;           // weight rows whose products are summed up before they enter dx
-constexpr int kDecodeTokens = 16;      // most tokens that int4_decode takes
+// Most tokens that int4_decode takes.  16 tokens there and in the tensor-memory kernel, groups of 128: 7168 -> 2048 9.6 and
+// 15.4 us, 2048 -> 7168 10.4 and 11.8, 2048 -> 768 3.9 and 8.5, 7168 -> 18432 50.0 and 49.7 (gated 99.6 and 88.9, but 96.8 and
+// 107.5 at 9 tokens); groups of 32: 7168 -> 18432 58.5 and 92.8.  24 tokens, 7168 -> 2048: 16.9 and 14.5.
+constexpr int kDecodeTokens = 16;
 // more tokens than int4_decode takes; the backward product
 int int4_fwd_tc(const Int4Fwd &P, bool bf16, bool gated, cudaStream_t st);
 int int4_dgrad_tc(const Int4Dgrad &P, bool bf16, const char *who, cudaStream_t st);

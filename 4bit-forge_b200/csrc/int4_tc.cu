@@ -23,11 +23,12 @@
 // half of the tokens, the even one issues the MMAs for both.  One CTA alone moves 192 KB through its shared memory per
 // 128-channel step (operands written and read), 1.5 times what the 1024 cycles of the MMAs allow; a pair's CTA moves 128.
 //
-// Measured (burst clocks): gated 8192 x 7168 -> 2048 348 us (1.38 PFLOP/s, 0.85 of the measured cuBLAS burst rate; 418 us,
-// 1.15 PFLOP/s, when the power limit holds the clock down), 4096 x 2048 -> 7168 with residual 128 us (0.94 PFLOP/s), dx of
-// gated 4096 x 2048 -> 7168 200 us (1.20 PFLOP/s).  ncu on the gated kernel at 4096 tokens: tensor pipe 72 % active (84 % on
-// the SMs that have four tiles), shared memory 84 %: what bounds it is the shared-memory port, which carries both operands
-// in and out.  The smaller products end on a partly filled round of tiles (448 tiles on 74 pairs).
+// Measured (burst clocks): gated 8192 x 7168 -> 2048 352 us (1.37 PFLOP/s, 0.84 of the measured cuBLAS burst rate; 416 us,
+// 1.16 PFLOP/s, when the power limit holds the clock down), 4096 x 2048 -> 7168 with residual 124 us (0.97 PFLOP/s), dx of
+// 4096 x 7168 <- 2 x 2048 (gated) 198 us (1.21 PFLOP/s), without the 18 us of dz and the 6 us of the scales.  ncu on the
+// gated kernel at 4096 tokens: tensor pipe 72 % active (84 % on the SMs that have four tiles), shared memory 84 %: what bounds
+// it is the shared-memory port, which carries both operands in and out.  The smaller products end on a partly filled round of
+// tiles (448 tiles on 74 pairs).
 //
 // With fewer tiles than SMs the K axis is shared by the CTAs of a cluster: each leaves its sums in its shared memory and
 // every CTA adds up a slice of the tokens from all of them, in rank order, over distributed shared memory.
@@ -50,13 +51,12 @@ constexpr int kLinear = 0, kGated = 1, kDgrad = 2;
 constexpr int kMT = 128, kKT = 128;             // rows of a CTA tile, channels of a stage
 constexpr int kSubA = kMT * 128, kABytes = 2 * kSubA;   // K-major: two sub-tiles of 64 channels (128 bytes a row)
 constexpr int kThreads = 640;
-// Registers a thread of the summing, loading and other warps, out of 5 x 96, as measured for each form; ptxas still spills 28
-// to 40 bytes in the linear form of a single CTA and 188 in the paired backward one, nothing in the others.  (The 4096 x 2048
-// -> 7168 product took 130 us with 176 for the sums and 190 with 160; the gated 8192 x 7168 -> 2048 one 371 us with 64 for the
-// loads and 454 with 48.)
+// Registers a thread of the summing, loading and other warps, out of 5 x 96, as measured for each form (4096 x 2048 -> 7168:
+// 130 us with 176 for the sums, 190 with 160; gated 8192 x 7168 -> 2048: 371 us with 64 for the loads, 454 with 48; dx of 4096 x
+// 7168 <- 2 x 2048: 198 us with 160 and 64, 204 with 152 and 72).  ptxas still spills 112 bytes in the paired backward form, 16
+// to 40 in the linear and the backward form of a single CTA, nothing in the others.
 template <int MODE> struct Regs {
-    static constexpr int kSum = MODE == kLinear ? 176 : MODE == kGated ? 160 : 152;
-    static constexpr int kLoad = MODE == kLinear ? 48 : MODE == kGated ? 64 : 72, kMisc = 32;
+    static constexpr int kSum = MODE == kLinear ? 176 : 160, kLoad = MODE == kLinear ? 48 : 64, kMisc = 32;
     static_assert(2 * kSum + 2 * kLoad + kMisc <= 5 * 96, "register shares within the launch's total");
 };
 constexpr int kOutBytes = 32 * 128;             // a summing warp's block: 32 tokens x 32 rows, fp32
