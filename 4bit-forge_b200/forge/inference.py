@@ -132,12 +132,12 @@ class Int4FeedForward(torch.nn.Module):
         forward(hidden, residual)  -> the same with hidden + residual in hidden's place
 
     gate, up [I, H/8] and down [H, I/8] are (weight_packed, scales) pairs, kept as they are given where they are contiguous
-    (and the scales fp32).  With norm_weight [H] the block starts with a
-    root-mean-square norm and its result is added to the residual stream (four kernels less one: norm, gated product,
-    product with the residual in its epilogue); without one it is the bare block and takes no residual.  The int4 weights
-    are frozen; gradients reach hidden, residual and the norm's gain (tuning through the quantised block).  `status` (int32,
-    on the block's device, not part of the state dict) collects what the kernels report; check() reads it.  The reference
-    runs its packed dense experts through vLLM and has no such block of its own."""
+    (and the scales fp32).  With norm_weight [H] the block starts with a root-mean-square norm and its result is added to the
+    residual stream (three kernels: norm, gated product, product with the residual in its epilogue); without one it is the
+    bare block and takes no residual.  The int4 weights are frozen; gradients reach hidden, residual and the norm's gain
+    (tuning through the quantised block).  `status` (int32, on the block's device, not part of the state dict) collects what
+    the kernels report; check() reads it.  The reference runs its packed dense experts through vLLM and has no such block of
+    its own."""
 
     def __init__(self, gate, up, down, group_size=128, act="silu", norm_weight=None, eps=1e-6):
         super().__init__()
