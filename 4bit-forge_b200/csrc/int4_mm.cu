@@ -7,7 +7,7 @@
 //
 // Backward operand: dz is the K operand of the second product and has to be a 16-bit matrix.  It is written as fp16
 // (11 bits, against bf16's 8) times a power of two per token row that puts the row's largest entry just below 2^15;
-// the product is multiplied by the inverse power at the end, so nothing but the 2^-12 relative rounding remains.  The
+// the product is multiplied by the inverse power at the end, so nothing but the rounding (2^-11 relative, half a step) remains.  The
 // weights' scales are split the same way, see scale_prep_kernel.
 #include <cooperative_groups.h>
 #include <utility>
@@ -30,8 +30,8 @@ namespace {
 // Both are powers of two, so they cost no bits.  With 2^12 at the top a product (nibble - 8) s' stays below 2^15, and it is a
 // normal fp16 number down to 2^-25 of its block's largest scale: only a scale that far below its row's AND below its block's
 // group loses bits.  A cluster takes a block, a CTA of it 64 rows and a warp four: the rows' powers stay in the warp, the
-// groups' maxima meet in shared memory.  Nothing but latency: 2048 rows of 32 groups take 4.7 us (one CTA per block: 20 us; without the
-// groups' powers, a warp a row: 2.2 us), 2 x 2048 rows of 56 groups 6.3 us.
+// groups' maxima meet in shared memory.  Nothing but latency: 2048 rows of 32 groups take 4.7 us, 2 x 2048 rows of 56 groups
+// 6.3 us (one CTA per block: 20 and 22 us; without the groups' powers, a warp a row: 2.2 and 3.2 us).
 constexpr int kPrepCtas = 8, kPrepRows = 4, kPrepGroups = 1024;      // a cluster's CTAs, a warp's rows, groups at a time
 static_assert(kPrepCtas * 16 * kPrepRows == kKBlock, "a cluster of 16 warps a CTA covers a block");
 __device__ __forceinline__ int exponent_of(float v) { return (int)((__float_as_uint(v) >> 23) & 255u) - 127; }

@@ -172,3 +172,12 @@ def test_a_residual_of_another_shape_is_refused(monkeypatch):
     for shape in ((3, 2, H), (6, H), (2, 6, H // 2), (1, 3, H), (H,)):
         with pytest.raises(RuntimeError, match="shape"):
             blk(x, residual=torch.zeros(shape))
+
+
+def test_the_backward_workspace_holds_the_powers_of_every_block_of_rows():
+    from forge import _abi
+    lib = _abi.load_library()
+    for T, C, R, gs, mats in ((1, 8, 1, 32, 1), (5, 776, 513, 32, 2), (4096, 7168, 2048, 128, 2), (3, 40000, 700, 32, 1)):
+        K, G = mats * R, -(-C // gs)
+        n = lib.forge_int4_backward_workspace_bytes(T, C, R, gs, mats)
+        assert n >= T * (-(-K // 64) * 64) * 2 + T * 4 + K * G * 4 + K * 4 + -(-K // 512) * G * 4 + 64 * R * 4
