@@ -7,9 +7,12 @@
 //
 // Backward operand: dz is the K operand of the second product and has to be a 16-bit matrix.  It is written as fp16
 // (11 bits, against bf16's 8) times a power of two per token row that puts the row's largest entry just below 2^15;
-// the product is multiplied by the inverse power at the end, so nothing but the rounding (2^-11 relative, half a step) remains.  The
-// weights' scales are split the same way, see scale_prep_kernel.
+// the product is multiplied by the inverse power at the end, so nothing but the rounding (2^-11 relative, half a step)
+// remains.  For fp16 gradients that would be as much as their own rounding, so a second fp16 matrix holds what the first
+// rounds off (22 bits together), unless dz is dy itself or zero (no activation, relu), and exact.  The weights' scales are
+// split the same way, see scale_prep_kernel.
 #include <cooperative_groups.h>
+#include <type_traits>
 #include <utility>
 #include "column_sum.cuh"
 #include "common.cuh"
@@ -103,7 +106,8 @@ scale_prep_kernel(const float *__restrict__ s0, const float *__restrict__ s1, in
 
 struct DzParams {
     const void *dy, *z, *u;     // z NULL: act is none; u given: gated
-    int64_t lddy, T, R, K, ldk; // ldk: row stride of a, a multiple of 64; K = used columns
+    int64_t lddy, T, R, K, ldk; // ldk: columns of a, a multiple of 64; K = used columns
+    int64_t lo;                 // 0, or ldk: what a rounds off goes lo columns behind it (the row stride is ldk + lo)
     const float *f;
     __half *a;
     float *unscale;
@@ -121,7 +125,12 @@ template <typename T, int ACT, bool GATED> __global__ void __launch_bounds__(256
     const int64_t t = blockIdx.x;
     const T *dy = (const T *)P.dy + t * P.lddy;
     const T *z = (const T *)P.z + t * P.R, *u = (const T *)P.u + t * P.R;
-    __half *a = P.a + t * P.ldk;
+    __half *a = P.a + t * (P.ldk + P.lo);
+    const auto put = [&](int64_t k, float v) {
+        const __half hi = __float2half_rn(v);
+        a[k] = hi;
+        if (P.lo) a[P.lo + k] = __float2half_rn(v - __half2float(hi));
+    };
     float scale = 1.0f;
     for (int pass = 0; pass < 2; ++pass) {
         float amax = 0.0f;
@@ -133,13 +142,13 @@ template <typename T, int ACT, bool GATED> __global__ void __launch_bounds__(256
                 const float vu = d * act_fwd<ACT>(zv) * P.f[P.R + r];
                 if (pass == 0) amax = fmaxf(amax, fmaxf(fabsf(vg), fabsf(vu)));
                 else {
-                    a[r] = __float2half_rn(vg * scale);
-                    a[P.R + r] = __float2half_rn(vu * scale);
+                    put(r, vg * scale);
+                    put(P.R + r, vu * scale);
                 }
             } else {
                 const float v = d * act_bwd<ACT>(zv) * P.f[r];
                 if (pass == 0) amax = fmaxf(amax, fabsf(v));
-                else a[r] = __float2half_rn(v * scale);
+                else put(r, v * scale);
             }
         }
         if (pass == 0) {
@@ -155,7 +164,7 @@ template <typename T, int ACT, bool GATED> __global__ void __launch_bounds__(256
             if (threadIdx.x == 0) P.unscale[t] = pow2_of(-e);
         }
     }
-    for (int64_t k = P.K + threadIdx.x; k < P.ldk; k += 256) a[k] = __float2half_rn(0.0f);
+    for (int64_t k = P.K + threadIdx.x; k < P.ldk; k += 256) put(k, 0.0f);
 }
 
 // The same with a row in registers (R a multiple of 8, 16-byte aligned rows, R <= 8 TPR NV): dz is computed once, rows are
@@ -164,6 +173,7 @@ template <typename T, int ACT, bool GATED> __global__ void __launch_bounds__(256
 template <typename T, int ACT, bool GATED, int TPR, int NV>
 __global__ void __launch_bounds__(TPR) dz_rows_kernel(const DzParams P, float *partial) {
     constexpr int M = GATED ? 2 : 1, W = TPR / 32;
+    constexpr bool kLow = std::is_same<T, __half>::value && (GATED || (ACT != FORGE_ACT_NONE && ACT != FORGE_ACT_RELU));
     __shared__ float slot[2][W];
     const int R = (int)P.R, tid = threadIdx.x;
     float db[NV][8];
@@ -229,7 +239,7 @@ __global__ void __launch_bounds__(TPR) dz_rows_kernel(const DzParams P, float *p
         const int e2 = row_exponent(amax);
         const float scale = pow2_of(e2);
         if (tid == 0) P.unscale[t] = pow2_of(-e2);
-        __half *a = P.a + t * P.ldk;
+        __half *a = P.a + t * (P.ldk + P.lo);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int r = (tid + i * TPR) * 8;
@@ -239,9 +249,17 @@ __global__ void __launch_bounds__(TPR) dz_rows_kernel(const DzParams P, float *p
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[m][i][e] *= scale;
                     store8(a + m * R + r, v[m][i]);
+                    if (kLow && P.lo) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[m][i][e] -= __half2float(__float2half_rn(v[m][i][e]));
+                        store8(a + P.lo + m * R + r, v[m][i]);
+                    }
                 }
         }
-        for (int64_t k = P.K + tid; k < P.ldk; k += TPR) a[k] = __float2half_rn(0.0f);
+        for (int64_t k = P.K + tid; k < P.ldk; k += TPR) {
+            a[k] = __float2half_rn(0.0f);
+            if (kLow && P.lo) a[P.lo + k] = __float2half_rn(0.0f);
+        }
     }
     if (!GATED && partial)
 #pragma unroll
@@ -289,14 +307,19 @@ bool rows_ok(const void *p, int64_t ld, int64_t n, int64_t T) {
 }
 
 struct BwdLayout {       // byte offsets into the workspace of a backward pass
-    int64_t ldk, a, unscale, pairs, f, group, partial, total;
+    int64_t ldk, lo, a, unscale, pairs, f, group, partial, total;
 };
-BwdLayout bwd_layout(int64_t T, int64_t C, int64_t R, int gs, int mats) {
+// whether dz has bits below its fp16 rounding that the gradient's type can see
+bool dz_has_low(int dtype, int act, int mats) {
+    return dtype == FORGE_DTYPE_F16 && (mats == 2 || (act != FORGE_ACT_NONE && act != FORGE_ACT_RELU));
+}
+BwdLayout bwd_layout(int64_t T, int64_t C, int64_t R, int gs, int mats, bool low) {
     BwdLayout L{};
     const auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
     L.ldk = cdiv(mats * R, (int64_t)64) * 64;
+    L.lo = low ? L.ldk : 0;
     L.a = 0;
-    L.unscale = up(T * L.ldk * 2);
+    L.unscale = up(T * (L.ldk + L.lo) * 2);
     L.pairs = L.unscale + up(T * 4);
     L.f = L.pairs + up(mats * R * cdiv(C, (int64_t)gs) * 4);
     L.group = L.f + up(mats * R * 4);
@@ -386,18 +409,24 @@ extern "C" int forge_int4_gated(const void *x, int64_t ldx, int dtype, const int
     return run_fwd(P, dtype, true, (cudaStream_t)stream);
 }
 
-extern "C" int64_t forge_int4_backward_workspace_bytes(int64_t T, int64_t C, int64_t R, int gs, int mats) {
+static int64_t workspace_bytes(int64_t T, int64_t C, int64_t R, int gs, int mats, bool low) {
     if (T < 0 || C <= 0 || R <= 0 || gs <= 0 || mats < 1 || mats > 2 || T > kMaxTokens || C > kMaxDim || R > kMaxDim) return 0;
-    return bwd_layout(T, C, R, gs, mats).total;
+    return bwd_layout(T, C, R, gs, mats, low).total;
+}
+extern "C" int64_t forge_int4_backward_workspace_bytes(int64_t T, int64_t C, int64_t R, int gs, int mats) {
+    return workspace_bytes(T, C, R, gs, mats, true);
+}
+extern "C" int64_t forge_int4_backward_workspace_bytes_for(int dtype, int act, int64_t T, int64_t C, int64_t R, int gs, int mats) {
+    return workspace_bytes(T, C, R, gs, mats, dz_has_low(dtype, act, mats));
 }
 
 static int backward(const char *who, const void *dy, int64_t lddy, int dtype, const int32_t *p0, const float *s0,
                     const int32_t *p1, const float *s1, int gs, int64_t T, int64_t C, int64_t R, const void *z, const void *u,
                     int act, void *dx, void *dbias, void *ws, int32_t *status, cudaStream_t st) {
     const int mats = p1 ? 2 : 1;
-    const BwdLayout L = bwd_layout(T, C, R, gs, mats);
-    uint8_t *base = (uint8_t *)ws;
     const bool bf16 = dtype == FORGE_DTYPE_BF16;
+    const BwdLayout L = bwd_layout(T, C, R, gs, mats, dz_has_low(dtype, act, mats));
+    uint8_t *base = (uint8_t *)ws;
     float *partial = (float *)(base + L.partial);
     int parts = 0;
     const int64_t G = cdiv(C, (int64_t)gs);
@@ -405,7 +434,7 @@ static int backward(const char *who, const void *dy, int64_t lddy, int dtype, co
         scale_prep_kernel<<<(unsigned)cdiv(mats * R, (int64_t)kKBlock) * kPrepCtas, 512, 0, st>>>(
             s0, s1, R, mats * R, G, (__half2 *)(base + L.pairs), (float *)(base + L.f), (float *)(base + L.group));
         FORGE_NOTE_LAUNCH();
-        DzParams D{dy, z, u, lddy, T, R, mats * R, L.ldk, (const float *)(base + L.f), (__half *)(base + L.a),
+        DzParams D{dy, z, u, lddy, T, R, mats * R, L.ldk, L.lo, (const float *)(base + L.f), (__half *)(base + L.a),
                    (float *)(base + L.unscale)};
         float *pp = dbias ? partial : nullptr;
         if (mats == 2) parts = bf16 ? launch_dz<__nv_bfloat16, true>(D, act, pp, st) : launch_dz<__half, true>(D, act, pp, st);
@@ -418,7 +447,7 @@ static int backward(const char *who, const void *dy, int64_t lddy, int dtype, co
         launch_column_sum(partial, parts, R, dbias, dtype, st);
     }
     if (!dx || T == 0) return check_launch(who);
-    Int4Dgrad P{(const __half *)(base + L.a), L.ldk, (const float *)(base + L.unscale),
+    Int4Dgrad P{(const __half *)(base + L.a), L.ldk, L.lo, (const float *)(base + L.unscale),
                 {(const uint32_t *)p0, (const uint32_t *)p1}, (const __half2 *)(base + L.pairs), (const float *)(base + L.group),
                 gs, mats, T, C, R, G, dx, status,
                 C % 16 == 0 && ((uintptr_t)p0 | (uintptr_t)p1) % 8 == 0};

@@ -24,8 +24,8 @@ struct Int4Fwd {
 };
 
 struct Int4Dgrad {
-    const __half *a;             // [T, ldk]: dz times powers of two
-    int64_t ldk;
+    const __half *a;             // [T, ldk + lo]: dz times powers of two, in fp16, and behind it what that rounds off
+    int64_t ldk, lo;             // lo: 0, or ldk when the low parts are there (fp16 gradients only)
     const float *unscale;        // [T]
     const uint32_t *packed[2];
     const __half2 *pairs;        // [mats * R, G]: normalised scales, hi and lo part

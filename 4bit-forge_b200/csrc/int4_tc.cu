@@ -13,6 +13,10 @@
 // many scales there, so they have to be in the operand: W' = fp16((nibble - 8) * s'), s' the scale without its row's power
 // of two (which dz carries exactly) and without that of its channel group in the chunk, kept as an fp16 pair (hi, lo).  Chunks
 // of 512 weight rows are added up in registers, times the group's power: again one factor for a thread, which has one channel.
+// fp16 gradients have 11 bits themselves, and dz and W' rounded to 11 bits would nearly double their error (4.0e-4 against
+// 2.1e-4).  For them both are pairs of fp16 numbers (22 bits), and a stage is 64 weight rows: their high parts in the upper half
+// of its W' tile and their low parts in the lower one, dz's high and low parts in its two sub-tiles, and three products, high x
+// high, low x high, high x low (two where dz is dy itself, whose low part is zero).
 //
 // A CTA (one per SM, 640 threads): warps 0-7 add finished chunks to the sums and run the epilogue, warps 8-11 and 12-15
 // turn packed words into 16-bit operand tiles, one stage each in turn (words read ahead into registers, tiles written with
@@ -200,6 +204,13 @@ __device__ __forceinline__ uint32_t scaled(uint32_t v, __half2 hi, __half2 lo) {
     return *reinterpret_cast<const uint32_t *>(&r);
 }
 
+// What `scaled` rounds off, itself rounded to fp16: (nibble - 8) hi - W' is exact, so 2^-22 of W' is left.
+__device__ __forceinline__ uint32_t scaled_low(uint32_t v, __half2 hi, __half2 lo, uint32_t w) {
+    const __half2 q = *reinterpret_cast<const __half2 *>(&v);
+    const __half2 r = __hfma2(q, lo, __hfma2(q, hi, __hneg2(*reinterpret_cast<const __half2 *>(&w))));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+
 constexpr uint32_t kZeroWord = 0x88888888u;
 
 __device__ __forceinline__ bool elect_one() {
@@ -302,12 +313,14 @@ template <typename T, int MODE, int CH, int NT, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_constant__ TcParams P,
                                                               const __grid_constant__ CUtensorMap tmap) {
     constexpr bool kBf16 = MODE != kDgrad && std::is_same<T, __nv_bfloat16>::value;
+    constexpr bool kSplit = MODE == kDgrad && std::is_same<T, __half>::value;     // both operands in high and low parts
+    constexpr int kStageK = kSplit ? kKT / 2 : kKT;                   // K rows of a stage
     constexpr int kBRows = PAIR ? NT / 2 : NT;                        // tokens that this CTA loads
     constexpr int kSubB = kBRows * 128, kBBytes = 2 * kSubB, kStageBytes = kABytes + kBBytes;
     constexpr int kStages = kRing / kStageBytes < 8 ? kRing / kStageBytes : 8;
     constexpr int kCols = NT / 2;                                     // tokens of a summing warp
     constexpr int kTileCols = MODE == kGated ? 64 : kMT;              // output columns of a tile
-    constexpr int kPerStage = CH < kKT ? kKT / CH : 1, kStagesPer = CH > kKT ? CH / kKT : 1;
+    constexpr int kPerStage = CH < kKT ? kKT / CH : 1, kStagesPer = CH > kKT ? CH / kStageK : 1;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *smem_al = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -627,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                 // whole halves inside one matrix, and a tile inside its columns: no test and little address work per load
                 const bool whole = P.d.vec8 && tile_col(tile) + kMT <= (int)P.d.C;
                 const auto fetch = [&](int st, int h, Half &H) {
-                    const int kb = st * kKT + h * 64;
+                    const int kb = st * kStageK + h * 64;
                     if (whole && kb + 64 <= K && (kb + 64 <= R || kb >= R)) {
                         const uint32_t *src = (kb >= R ? w1 : w0) + (int64_t)((kb >= R ? kb - R : kb) + k0) * CP;
                         const __half2 *ss = sp + (int64_t)(kb + k0) * G;
@@ -653,45 +666,54 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                         H.s[p] = k < K && in0 ? __ldg(sp + (int64_t)k * G) : __half2(__ushort_as_half(0), __ushort_as_half(0));
                     }
                 };
-                const auto unpack = [&](uint32_t at, const Half &H) {
+                // kHigh, kLow: the parts that are written, the low one 64 K rows behind the high one
+                const auto unpack = [&](uint32_t at, const Half &H, bool kHigh, bool kLow) {
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
                         const __half2 hi = __low2half2(H.s[p]), lo = __high2half2(H.s[p]);
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            uint4 v = word_to_half<false>((e == 0) != swap ? H.w[p].x : H.w[p].y);
-                            v = make_uint4(scaled(v.x, hi, lo), scaled(v.y, hi, lo), scaled(v.z, hi, lo), scaled(v.w, hi, lo));
-                            sts128(at + p * 2048 + (e == 0 ? xa : xb), v);
+                            const uint4 v = word_to_half<false>((e == 0) != swap ? H.w[p].x : H.w[p].y);
+                            const uint4 w = make_uint4(scaled(v.x, hi, lo), scaled(v.y, hi, lo), scaled(v.z, hi, lo), scaled(v.w, hi, lo));
+                            const uint32_t dst = at + p * 2048 + (e == 0 ? xa : xb);
+                            if (kHigh) sts128(dst, w);
+                            if (kLow)
+                                sts128(dst + 8192, make_uint4(scaled_low(v.x, hi, lo, w.x), scaled_low(v.y, hi, lo, w.y),
+                                                              scaled_low(v.z, hi, lo, w.z), scaled_low(v.w, hi, lo, w.w)));
                         }
                     }
                 };
                 const int first = st0 + (PAIR ? (group + base) & 1 : 0);
-                Half b[2];                                            // both halves of a stage, or one of two stages
-                if (first < st1) fetch(first, PAIR ? 0 : group, b[0]);
-                if (PAIR ? first < st1 : first + 1 < st1) fetch(PAIR ? first : first + 1, PAIR ? 1 : group, b[1]);
-                for (int stb = first; stb < st1 && ok; stb += 2) {
+                constexpr bool kBoth = PAIR && !kSplit;               // b: both halves of a stage, or one of two stages
+                constexpr int kAhead = kBoth ? 1 : 2;
+                const int half = PAIR || kSplit ? 0 : group;
+                Half b[2];
+                if (first < st1) fetch(first, half, b[0]);
+                if (kBoth ? first < st1 : first + kTurn < st1) fetch(kBoth ? first : first + kTurn, kBoth ? 1 : half, b[1]);
+                for (int stb = first; stb < st1 && ok; stb += kTurn * kAhead) {
 #pragma unroll
-                    for (int a = 0; a < (PAIR ? 1 : 2); ++a) {
-                        const int st = stb + a;
+                    for (int a = 0; a < kAhead; ++a) {
+                        const int st = stb + a * kTurn;
                         if (st >= st1) break;
                         const uint32_t it = (uint32_t)(base + st - st0), s = it % kStages;
                         ok = wait_on(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
                         if (!ok) break;
                         const uint32_t at = smem_base + s * kStageBytes + d0;
-                        if constexpr (PAIR) {
-                            unpack(at, b[0]);
-                            unpack(at + 8192, b[1]);
-                        } else {
-                            unpack(at + group * 8192, b[a]);
+                        if constexpr (kBoth) {
+                            unpack(at, b[0], true, false);
+                            unpack(at + 8192, b[1], true, false);
+                        } else if constexpr (!kSplit) {
+                            unpack(at + group * 8192, b[a], true, false);
+                        } else if constexpr (PAIR) {
+                            unpack(at, b[a], true, true);
+                        } else {                                      // one group the high parts, the other the low ones
+                            if (group == 0) unpack(at, b[a], true, false);
+                            else unpack(at, b[a], false, true);
                         }
                         publish(s);
-                        if (st + 2 < st1) {
-                            if constexpr (PAIR) {
-                                fetch(st + 2, 0, b[0]);
-                                fetch(st + 2, 1, b[1]);
-                            } else {
-                                fetch(st + 2, group, b[a]);
-                            }
+                        if (st + kTurn * kAhead < st1) {
+                            fetch(st + kTurn * kAhead, half, b[a]);
+                            if constexpr (kBoth) fetch(st + kTurn * kAhead, 1, b[1]);
                         }
                     }
                 }
@@ -713,14 +735,16 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                         ok = wait_on(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
                         if (!ok) break;
                         const uint32_t dst = smem_base + s * kStageBytes + kABytes;
+                        const int x0 = st * kStageK, x1 = kSplit ? (int)P.d.lo + x0 : x0 + 64;    // (the low parts lie behind the high ones)
+                        const bool both = !kSplit || P.d.lo != 0;
                         if constexpr (PAIR) {
-                            if (member == 0) mbar_arrive_expect_tx(b_full + 8 * s, 2 * kBBytes);
-                            tma_load_2d_pair(dst, &tmap, st * kKT, t0, even_cta(b_full + 8 * s));
-                            tma_load_2d_pair(dst + kSubB, &tmap, st * kKT + 64, t0, even_cta(b_full + 8 * s));
+                            if (member == 0) mbar_arrive_expect_tx(b_full + 8 * s, both ? 2 * kBBytes : kBBytes);
+                            tma_load_2d_pair(dst, &tmap, x0, t0, even_cta(b_full + 8 * s));
+                            if (both) tma_load_2d_pair(dst + kSubB, &tmap, x1, t0, even_cta(b_full + 8 * s));
                         } else {
-                            mbar_arrive_expect_tx(b_full + 8 * s, kBBytes);
-                            tma_load_2d(dst, &tmap, st * kKT, t0, b_full + 8 * s);
-                            tma_load_2d(dst + kSubB, &tmap, st * kKT + 64, t0, b_full + 8 * s);
+                            mbar_arrive_expect_tx(b_full + 8 * s, both ? kBBytes : kSubB);
+                            tma_load_2d(dst, &tmap, x0, t0, b_full + 8 * s);
+                            if (both) tma_load_2d(dst + kSubB, &tmap, x1, t0, b_full + 8 * s);
                         }
                     }
                 }
@@ -730,7 +754,8 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
             // the whole warp walks the loop and one elected lane issues, so addresses and descriptors stay uniform
             uint32_t s = 0, phase = 0, chunk = 0;
             bool ok = !PAIR || member == 0;
-            constexpr int kStepsPer = (CH < kKT ? CH : kKT) / 16;     // k-steps of a chunk inside a stage
+            constexpr int kStepsPer = kSplit ? 12 : (CH < kKT ? CH : kKT) / 16;       // k-steps of a chunk inside a stage
+            const int steps = kSplit && P.d.lo == 0 ? 8 : kStepsPer;
             const uint64_t ad0 = MODE == kDgrad ? desc_mnmajor(smem_base) : desc_kmajor(smem_base);
             const uint64_t bd0 = desc_kmajor(smem_base + kABytes);
             for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
@@ -754,9 +779,12 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                             const uint32_t d = tmem_base + (chunk & 1u) * NT;
 #pragma unroll
                             for (int i = 0; i < kStepsPer; ++i) {
-                                const int kk = e * kStepsPer + i;
-                                const uint64_t a = ad + (MODE == kDgrad ? kk * 2048 : (kk >> 2) * kSubA + (kk & 3) * 32) / 16;
-                                const uint64_t bb = bd + ((kk >> 2) * kSubB + (kk & 3) * 32) / 16;
+                                if (kSplit && i >= steps) break;
+                                // split: high x high, low x high, high x low, four k-steps each
+                                const int kk = e * kStepsPer + i, ka = kSplit && i >= 8 ? i - 8 : kk;
+                                const int kb = !kSplit ? kk : i >= 8 ? i - 4 : i & 3;
+                                const uint64_t a = ad + (MODE == kDgrad ? ka * 2048 : (ka >> 2) * kSubA + (ka & 3) * 32) / 16;
+                                const uint64_t bb = bd + ((kb >> 2) * kSubB + (kb & 3) * 32) / 16;
                                 const uint32_t more = (i == 0 && first_stage) ? 0u : 1u;
                                 if constexpr (PAIR) umma_f16_pair(d, a, bb, idesc<MODE, kBf16>(2 * kMT, NT), more);
                                 else umma_f16(d, a, bb, idesc<MODE, kBf16>(kMT, NT), more);
@@ -921,8 +949,8 @@ int int4_fwd_tc(const Int4Fwd &F, bool bf16, bool gated, cudaStream_t st) {
 int int4_dgrad_tc(const Int4Dgrad &D, bool bf16, const char *who, cudaStream_t st) {
     TcParams P{};
     P.d = D; P.T = D.T; P.N = D.C; P.status = D.status;
-    P.nst = (int)cdiv(D.ldk, (int64_t)kKT);
-    const TokenSource src{D.a, false, D.T, D.ldk, D.ldk};
+    P.nst = (int)cdiv(D.ldk, (int64_t)(bf16 ? kKT : kKT / 2));
+    const TokenSource src{D.a, false, D.T, D.ldk + D.lo, D.ldk + D.lo};
     return bf16 ? launch_nt<__nv_bfloat16, kDgrad, kKBlock>(P, src, who, st) : launch_nt<__half, kDgrad, kKBlock>(P, src, who, st);
 }
 

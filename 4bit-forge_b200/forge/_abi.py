@@ -77,6 +77,7 @@ _PROTOS = {
     "forge_int4_gated": (_c_int, [_ptr, _c_i64, _c_int, _ptr, _ptr, _ptr, _ptr, _c_int, _c_i64, _c_i64, _c_i64, _c_int, _ptr,
                                   _ptr, _ptr, _ptr, _ptr]),
     "forge_int4_backward_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_int, _c_int]),
+    "forge_int4_backward_workspace_bytes_for": (_c_i64, [_c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_int, _c_int]),
     "forge_int4_linear_backward": (_c_int, [_ptr, _c_i64, _c_int, _ptr, _ptr, _c_int, _c_i64, _c_i64, _c_i64, _ptr, _c_int,
                                             _ptr, _ptr, _ptr, _ptr, _ptr]),
     "forge_int4_gated_backward": (_c_int, [_ptr, _c_i64, _c_int, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _c_int, _c_i64, _c_i64,

@@ -535,7 +535,8 @@ def int4_linear_backward(dy, packed, scales, gs: int = 128, preact=None, act: st
     """Gradients of int4_linear for frozen weights: dz = dy * act'(preact); returns (dx, dbias), dx = dz W [T, C] and
     dbias = the column sums of dz [R], both of dy's type, None where not wanted.  preact is the z of the forward call
     (not needed with act="none"); the residual's gradient is dy itself (forge_int4_linear_backward).  dz and W are rounded to
-    fp16 (2^-11 each) after powers of two are taken out of dz's rows and of W's rows and channel groups; sums in fp32."""
+    fp16 (2^-11 each; for fp16 gradients to pairs of fp16 numbers, 2^-21) after powers of two are taken out of dz's rows and of
+    W's rows and channel groups; sums in fp32."""
     dev = _on_device(dy, "dy")
     if dev is None:
         with torch.cuda.device(dy.device):
@@ -553,7 +554,7 @@ def int4_linear_backward(dy, packed, scales, gs: int = 128, preact=None, act: st
     dy, lddy = _rows(dy, T, R, False)
     dx = dy.new_empty((T, C)) if want_dx else None
     db = dy.new_empty((R,)) if want_dbias else None
-    ws = torch.empty(query("forge_int4_backward_workspace_bytes", T, C, R, gs, 1), dtype=torch.uint8, device=dy.device)
+    ws = torch.empty(query("forge_int4_backward_workspace_bytes_for", code, ac, T, C, R, gs, 1), dtype=torch.uint8, device=dy.device)
     call("forge_int4_linear_backward", dy.data_ptr(), lddy, code, packed.data_ptr(), scales.data_ptr(), gs, T, C, R, pz, ac,
          None if dx is None else dx.data_ptr(), None if db is None else db.data_ptr(), ws.data_ptr(), pst, stream_ptr(dev))
     return dx, db
@@ -601,7 +602,7 @@ def int4_gated_backward(dh, g, u, gate_packed, gate_scales, up_packed, up_scales
     g, u = _dense(g, "g", (T, R), dh.dtype, dev), _dense(u, "u", (T, R), dh.dtype, dev)
     dh, lddh = _rows(dh, T, R, False)
     dx = dh.new_empty((T, C))
-    ws = torch.empty(query("forge_int4_backward_workspace_bytes", T, C, R, gs, 2), dtype=torch.uint8, device=dh.device)
+    ws = torch.empty(query("forge_int4_backward_workspace_bytes_for", code, ac, T, C, R, gs, 2), dtype=torch.uint8, device=dh.device)
     call("forge_int4_gated_backward", dh.data_ptr(), lddh, code, g.data_ptr(), u.data_ptr(), gate_packed.data_ptr(),
          gate_scales.data_ptr(), up_packed.data_ptr(), up_scales.data_ptr(), gs, T, C, R, ac, dx.data_ptr(), ws.data_ptr(),
          pst, stream_ptr(dev))

@@ -372,12 +372,14 @@ int forge_int4_gated(const void *x, int64_t ldx, int dtype, const int32_t *gate_
  *   gated:   dx = (dh * u * act'(g)) Wg + (dh * act(g)) Wu
  * dx [T, C] and dbias [R] of x's type, dense; preact may be NULL when act is FORGE_ACT_NONE.  dz enters its product as
  * fp16 with a power of two per row of dz, the weight as fp16 with a power of two per weight row and another per channel
- * group and 512 weight rows (of gate and up together): each is off by 2^-11 at most, relative, as long as a scale is at least
- * 2^-25 times the largest of its row, or of its group in the 512 rows once the rows' powers are taken out.  A weight far
+ * group and 512 weight rows (of gate and up together): each is off by 2^-11 at most, relative (fp16 gradients: by 2^-21, both
+ * being pairs of fp16 numbers, in three products instead of one), as long as a scale is at least 2^-25 times the largest of its row, or of its group in the 512 rows once the rows' powers are taken out.  A weight far
  * below both loses bits, and so does an entry of dz that, times its weight row's power, is below 2^-29 of the largest of
  * its token.  The order of every sum is fixed.
  * ws: forge_int4_backward_workspace_bytes(T, C, R, gs, mats) bytes (mats 1 linear, 2 gated), 256-byte aligned. */
 int64_t forge_int4_backward_workspace_bytes(int64_t T, int64_t C, int64_t R, int gs, int mats);
+/* the same for one type and activation: about half of it but for fp16 with silu, gelu or a gate */
+int64_t forge_int4_backward_workspace_bytes_for(int dtype, int act, int64_t T, int64_t C, int64_t R, int gs, int mats);
 int forge_int4_linear_backward(const void *dy, int64_t lddy, int dtype, const int32_t *packed, const float *scales, int gs,
                                int64_t T, int64_t C, int64_t R, const void *preact, int act, void *dx, void *dbias, void *ws,
                                int32_t *status, void *stream);

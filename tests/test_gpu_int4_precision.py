@@ -2,9 +2,10 @@
 
 Tolerances, derived before the first run.  A sum over k of terms with independent signs has a norm of the root of the sum of
 the terms' squares, and so has the sum of their independent errors: a relative rounding of half a step h of every term
-contributes h / sqrt(3) at most, norm-wise (an error spread evenly over the step).  dz is rounded to fp16 (2^-11), the weight
-is rounded to fp16 (2^-11), and the result to its own type: sqrt((h_type^2 + 2 (2^-11)^2) / 3), and a tenth more for the
-spread of the norms of a few thousand entries and the fp32 sums."""
+contributes h / sqrt(3) at most, norm-wise (an error spread evenly over the step).  For bf16 gradients dz and the weight are
+rounded to fp16 (2^-11 each), and the result to its own type: sqrt((h_type^2 + 2 (2^-11)^2) / 3); for fp16 gradients dz and
+the weight keep 22 bits, so the result's rounding is all: h_type / sqrt(3).  A tenth more covers the spread of the norms of a
+few thousand entries and the fp32 sums."""
 import math
 
 import pytest
@@ -29,7 +30,7 @@ def words(codes):
 
 
 def norm_bound(dt):
-    return 1.1 * math.sqrt((HALF[dt] ** 2 + 2 * 2.0 ** -22) / 3)
+    return 1.1 * math.sqrt((HALF[dt] ** 2 + (2 * 2.0 ** -22 if dt == torch.bfloat16 else 0)) / 3)
 
 
 @pytest.mark.parametrize("T", [3, 70, 5000])
@@ -186,3 +187,20 @@ def test_block_norm_wise(T, dt):
     with torch.no_grad():
         assert off(blk(x, residual=res), want) <= 1.1 * 2.5 * HALF[dt] / math.sqrt(3)
     blk.check()
+
+
+@pytest.mark.parametrize("T,C,R", [(2, 384, 22), (40, 1032, 700), (200, 520, 1001), (2600, 1000, 1000)])
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu"])
+def test_fp16_gradients_are_off_by_their_own_rounding(T, C, R, act):
+    """dz and the weight rounded to 11 bits each would put the gradient off by sqrt(3) of its own rounding."""
+    g = torch.Generator(device=DEV).manual_seed(T + C)
+    p0, s0, W0 = matrix(R, C, 64, g)
+    z = torch.randn(T, R, generator=g, device=DEV).half()
+    dy = (torch.randn(T, R, generator=g, device=DEV) * torch.exp2(-8 * torch.rand(T, R, generator=g, device=DEV))).half()
+    Z = z.double()
+    sig = torch.sigmoid(Z)
+    d = {"none": torch.ones_like(Z), "relu": (Z > 0).double(), "silu": sig * (1 + Z * (1 - sig)),
+         "gelu": torch.special.ndtr(Z) + Z * torch.exp(-Z * Z / 2) / math.sqrt(2 * math.pi)}[act]
+    dz = dy.double() * d
+    dx, _ = ops().int4_linear_backward(dy, p0, s0, 64, preact=z, act=act)
+    assert off(dx, dz @ W0) <= norm_bound(torch.float16)

@@ -180,4 +180,10 @@ def test_the_backward_workspace_holds_the_powers_of_every_block_of_rows():
     for T, C, R, gs, mats in ((1, 8, 1, 32, 1), (5, 776, 513, 32, 2), (4096, 7168, 2048, 128, 2), (3, 40000, 700, 32, 1)):
         K, G = mats * R, -(-C // gs)
         n = lib.forge_int4_backward_workspace_bytes(T, C, R, gs, mats)
-        assert n >= T * (-(-K // 64) * 64) * 2 + T * 4 + K * G * 4 + K * 4 + -(-K // 512) * G * 4 + 64 * R * 4
+        rest = T * 4 + K * G * 4 + K * 4 + -(-K // 512) * G * 4 + 64 * R * 4
+        assert n >= T * (-(-K // 64) * 64) * 4 + rest              # high and low parts of dz
+        for dtype, act in ((_abi.BF16, "gelu"), (_abi.F16, "none"), (_abi.F16, "relu"), (_abi.F16, "silu")):
+            m = lib.forge_int4_backward_workspace_bytes_for(dtype, _abi.ACTS[act], T, C, R, gs, mats)
+            low = dtype == _abi.F16 and (mats == 2 or act == "silu")
+            assert m == n if low else T * (-(-K // 64) * 64) * 2 + rest <= m <= n
+    assert lib.forge_int4_backward_workspace_bytes_for(_abi.F16, 0, 1, 8, 8, 0, 1) == 0
