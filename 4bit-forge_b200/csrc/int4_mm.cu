@@ -33,12 +33,16 @@ namespace {
 // Both are powers of two, so they cost no bits.  With 2^12 at the top a product (nibble - 8) s' stays below 2^15, and it is a
 // normal fp16 number down to 2^-25 of its block's largest scale: only a scale that far below its row's AND below its block's
 // group loses bits.  A cluster takes a block, a CTA of it 64 rows and a warp four: the rows' powers stay in the warp, the
-// groups' maxima meet in shared memory.  Nothing but latency: 2048 rows of 32 groups take 4.7 us, 2 x 2048 rows of 56 groups
-// 6.3 us (one CTA per block: 20 and 22 us; without the groups' powers, a warp a row: 2.2 and 3.2 us).
+// groups' maxima meet in shared memory.  Nothing but latency: 2048 rows of 16 groups take 3.7 us, 2 x 2048 rows of 56 groups
+// 4.8 us (every scale read three times: 4.6 and 7.5 us; without the groups' powers, a warp a row: 2.2 and 3.8 us).
 constexpr int kPrepCtas = 8, kPrepRows = 4, kPrepGroups = 1024;      // a cluster's CTAs, a warp's rows, groups at a time
+constexpr int kPrepKept = 2;                  // a lane's groups whose scales stay in registers, read once
 static_assert(kPrepCtas * 16 * kPrepRows == kKBlock, "a cluster of 16 warps a CTA covers a block");
 __device__ __forceinline__ int exponent_of(float v) { return (int)((__float_as_uint(v) >> 23) & 255u) - 127; }
 __device__ __forceinline__ float finite_abs(float v) { return isfinite(v) ? fabsf(v) : 0.0f; }
+__device__ __forceinline__ float pow2_any(int e) {      // -149 <= e <= 127
+    return __uint_as_float(e < -126 ? 1u << (e + 149) : (uint32_t)(e + 127) << 23);
+}
 
 __global__ void __cluster_dims__(kPrepCtas) __launch_bounds__(512)
 scale_prep_kernel(const float *__restrict__ s0, const float *__restrict__ s1, int64_t R, int64_t K, int64_t G,
@@ -49,57 +53,76 @@ scale_prep_kernel(const float *__restrict__ s0, const float *__restrict__ s1, in
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t k0 = (int64_t)blockIdx.x * (16 * kPrepRows) + warp * kPrepRows, block = blockIdx.x / kPrepCtas;
     const float *row[kPrepRows];
-    float m[kPrepRows], inv[kPrepRows];
+    float kept[kPrepKept][kPrepRows], m[kPrepRows], inv[kPrepRows];
 #pragma unroll
     for (int i = 0; i < kPrepRows; ++i) {
         const int64_t k = k0 + i < K ? k0 + i : K - 1;
         row[i] = k < R ? s0 + k * G : s1 + (k - R) * G;
         m[i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kPrepKept; ++j) kept[j][i] = lane + 32 * j < G ? row[i][lane + 32 * j] : 0.0f;
     }
-#pragma unroll 2
-    for (int64_t g = lane; g < G; g += 32)
+    const int top_n = (int)imin64(G, kPrepGroups);
+    for (int g = threadIdx.x; g < top_n; g += 512) top[g] = 0;
+    for (int64_t g = lane + 32 * kPrepKept; g < G; g += 32)
 #pragma unroll
         for (int i = 0; i < kPrepRows; ++i) m[i] = fmaxf(m[i], finite_abs(row[i][g]));
 #pragma unroll
     for (int i = 0; i < kPrepRows; ++i) {
 #pragma unroll
+        for (int j = 0; j < kPrepKept; ++j) m[i] = fmaxf(m[i], finite_abs(kept[j][i]));
+#pragma unroll
         for (int o = 16; o > 0; o >>= 1) m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], o));
         const int e = m[i] > 0.0f ? exponent_of(m[i]) : 0;
-        inv[i] = scalbnf(1.0f, -e);
-        if (lane == 0 && k0 + i < K) f[k0 + i] = scalbnf(1.0f, e);
+        inv[i] = k0 + i < K ? pow2_any(-e) : 0.0f;            // (rows past the last one are no part of a maximum)
+        if (lane == 0 && k0 + i < K) f[k0 + i] = pow2_any(e);
     }
     for (int64_t g0 = 0; g0 < G; g0 += kPrepGroups) {
         const int n = (int)imin64(G - g0, kPrepGroups);
-        for (int g = threadIdx.x; g < n; g += 512) top[g] = 0;
+        if (g0 > 0)
+            for (int g = threadIdx.x; g < n; g += 512) top[g] = 0;
         __syncthreads();
-#pragma unroll 2
-        for (int g = lane; g < n; g += 32) {
+        const auto raise = [&](int g, const float (&v)[kPrepRows]) {
             float t = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kPrepRows; ++i)
-                if (k0 + i < K) t = fmaxf(t, finite_abs(row[i][g0 + g]) * inv[i]);
+            for (int i = 0; i < kPrepRows; ++i) t = fmaxf(t, finite_abs(v[i]) * inv[i]);
             atomicMax(top + g, __float_as_int(t));
-        }
+        };
+        const auto write = [&](int g, const float (&v)[kPrepRows]) {
+#pragma unroll
+            for (int i = 0; i < kPrepRows; ++i)
+                if (k0 + i < K) {
+                    const float x = v[i] * inv[i] * power[g];
+                    const __half hi = __float2half_rn(x);
+                    pairs[(k0 + i) * G + g0 + g] = __halves2half2(hi, __float2half_rn(x - __half2float(hi)));
+                }
+        };
+        // the groups of this turn, those in registers first
+        const auto each = [&](const auto &what) {
+            if (g0 == 0)
+#pragma unroll
+                for (int j = 0; j < kPrepKept; ++j)
+                    if (lane + 32 * j < n) what(lane + 32 * j, kept[j]);
+            for (int g = lane + (g0 == 0 ? 32 * kPrepKept : 0); g < n; g += 32) {
+                float v[kPrepRows];
+#pragma unroll
+                for (int i = 0; i < kPrepRows; ++i) v[i] = row[i][g0 + g];
+                what(g, v);
+            }
+        };
+        each(raise);
         cluster.sync();
         for (int g = threadIdx.x; g < n; g += 512) {
             int t = 0;
 #pragma unroll
             for (int r = 0; r < kPrepCtas; ++r) t = max(t, *cluster.map_shared_rank(top + g, r));
-            const int e = t == 0 ? 0 : max(exponent_of(__int_as_float(t)), -100);      // (2^(e - 11) stays a normal number)
-            power[g] = scalbnf(1.0f, 11 - e);
-            if (cluster.block_rank() == 0) group[block * G + g0 + g] = scalbnf(1.0f, e - 11);
+            const int e = t == 0 ? 0 : max(exponent_of(__int_as_float(t)), -100);      // 2^(e - 11) stays a normal number
+            power[g] = pow2_any(11 - e);
+            if (cluster.block_rank() == 0) group[block * G + g0 + g] = pow2_any(e - 11);
         }
         auto read = cluster.barrier_arrive();
         __syncthreads();
-#pragma unroll 2
-        for (int g = lane; g < n; g += 32)
-#pragma unroll
-            for (int i = 0; i < kPrepRows; ++i)
-                if (k0 + i < K) {
-                    const float v = row[i][g0 + g] * inv[i] * power[g];
-                    const __half hi = __float2half_rn(v);
-                    pairs[(k0 + i) * G + g0 + g] = __halves2half2(hi, __float2half_rn(v - __half2float(hi)));
-                }
+        each(write);
         cluster.barrier_wait(std::move(read));        // nobody clears or leaves its maxima while they are read
     }
 }
