@@ -337,9 +337,9 @@ int forge_sparse14_moe_w2(const uint64_t *w2, const void *X2_bf16, int64_t ldx, 
  *   scales[t, g] = max(max |y|, 1e-12) / 448,   y8 = e4m3(y / scales[t, g])
  * (a product with the rounded reciprocal, within 3 2^-24 of the quotient before it is rounded to e4m3):
  * scales [T, ceil(C/128)] fp32, the layout that forge_fp8_block_dequant reads when C is a multiple of 128.  Row strides
- * ldx, ldres in elements; y, scales and residual_out are dense and alias no input.  Any C, stride and alignment (16-byte aligned rows of a
- * multiple of 8 channels up to 16384 are read once, others twice; fp32 rows of more than 4096 channels are read once only
- * with a residual and from 5120 on). */
+ * ldx, ldres in elements; y, scales and residual_out are dense and alias no input.
+ * Any C, stride and alignment (16-byte aligned rows of a multiple of 8 channels up to 16384 are read once, others twice;
+ * fp32 rows of more than 4096 channels are read once only with a residual and from 5120 on). */
 int forge_rmsnorm(const void *x, int64_t ldx, const void *residual, int64_t ldres, const void *weight, int w_dtype,
                   int dtype, int64_t T, int64_t C, float eps, void *y, float *scales, void *residual_out, void *stream);
 /* Gradients at the normed rows x (the residual_out of the forward call where there was a residual):
@@ -372,10 +372,11 @@ int forge_int4_gated(const void *x, int64_t ldx, int dtype, const int32_t *gate_
  *   gated:   dx = (dh * u * act'(g)) Wg + (dh * act(g)) Wu
  * dx [T, C] and dbias [R] of x's type, dense; preact may be NULL when act is FORGE_ACT_NONE.  dz enters its product as
  * fp16 with a power of two per row of dz, the weight as fp16 with a power of two per weight row and another per channel
- * group and 512 weight rows (of gate and up together): each is off by 2^-11 at most, relative (fp16 gradients: by 2^-21, both
- * being pairs of fp16 numbers, in three products instead of one), as long as a scale is at least 2^-25 times the largest of its row, or of its group in the 512 rows once the rows' powers are taken out.  A weight far
- * below both loses bits, and so does an entry of dz that, times its weight row's power, is below 2^-29 of the largest of
- * its token.  The order of every sum is fixed.
+ * group and 512 weight rows (of gate and up together).  Each is off by 2^-11 at most, relative, as long as a scale is at
+ * least 2^-25 times the largest of its row, or of its group in the 512 rows once the rows' powers are taken out, and an
+ * entry of dz, times its weight row's power, at least 2^-29 times the largest of its token; what is smaller loses bits.
+ * For fp16 gradients both are pairs of fp16 numbers, in three products instead of one: 2^-21 down to 2^-14 times those
+ * largest values, then less.  The order of every sum is fixed.
  * ws: forge_int4_backward_workspace_bytes(T, C, R, gs, mats) bytes (mats 1 linear, 2 gated), 256-byte aligned. */
 int64_t forge_int4_backward_workspace_bytes(int64_t T, int64_t C, int64_t R, int gs, int mats);
 /* the same for one type and activation: about half of it but for fp16 with silu, gelu or a gate */
