@@ -666,8 +666,8 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                         H.s[p] = k < K && in0 ? __ldg(sp + (int64_t)k * G) : __half2(__ushort_as_half(0), __ushort_as_half(0));
                     }
                 };
-                // kHigh, kLow: the parts that are written, the low one 64 K rows behind the high one
-                const auto unpack = [&](uint32_t at, const Half &H, bool kHigh, bool kLow) {
+                // the parts that are asked for, the low one 64 K rows behind the high one
+                const auto unpack = [&](uint32_t at, const Half &H, bool high, bool low) {
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
                         const __half2 hi = __low2half2(H.s[p]), lo = __high2half2(H.s[p]);
@@ -676,8 +676,8 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                             const uint4 v = word_to_half<false>((e == 0) != swap ? H.w[p].x : H.w[p].y);
                             const uint4 w = make_uint4(scaled(v.x, hi, lo), scaled(v.y, hi, lo), scaled(v.z, hi, lo), scaled(v.w, hi, lo));
                             const uint32_t dst = at + p * 2048 + (e == 0 ? xa : xb);
-                            if (kHigh) sts128(dst, w);
-                            if (kLow)
+                            if (high) sts128(dst, w);
+                            if (low)
                                 sts128(dst + 8192, make_uint4(scaled_low(v.x, hi, lo, w.x), scaled_low(v.y, hi, lo, w.y),
                                                               scaled_low(v.z, hi, lo, w.z), scaled_low(v.w, hi, lo, w.w)));
                         }
@@ -735,7 +735,7 @@ __global__ void __launch_bounds__(kThreads, 1) int4_tc_kernel(const __grid_const
                         ok = wait_on(b_empty + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
                         if (!ok) break;
                         const uint32_t dst = smem_base + s * kStageBytes + kABytes;
-                        const int x0 = st * kStageK, x1 = kSplit ? (int)P.d.lo + x0 : x0 + 64;    // (the low parts lie behind the high ones)
+                        const int x0 = st * kStageK, x1 = kSplit ? (int)P.d.lo + x0 : x0 + 64;    // dz's low parts lie behind its high ones
                         const bool both = !kSplit || P.d.lo != 0;
                         if constexpr (PAIR) {
                             if (member == 0) mbar_arrive_expect_tx(b_full + 8 * s, both ? 2 * kBBytes : kBBytes);
